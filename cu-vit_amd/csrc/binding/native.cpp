@@ -42,10 +42,22 @@ struct Library {
     decltype(&cuvit_attention_bf16) attention_bf16;
     decltype(&cuvit_preprocess_u8) preprocess_u8;
     decltype(&cuvit_vit_forward) vit_forward;
+    decltype(&cuvit_rotary_f32) rotary_f32;
+    decltype(&cuvit_rotary_bf16) rotary_bf16;
+    decltype(&cuvit_qk_norm_rotary_f32) qk_norm_rotary_f32;
+    decltype(&cuvit_qk_norm_rotary_bf16) qk_norm_rotary_bf16;
+    decltype(&cuvit_qk_norm_rotary_backward_f32) qk_norm_rotary_backward_f32;
+    decltype(&cuvit_qk_norm_rotary_backward_bf16) qk_norm_rotary_backward_bf16;
+    decltype(&cuvit_qk_norm_rotary_workspace) qk_norm_rotary_workspace;
+    decltype(&cuvit_gated_gemm_f32) gated_gemm_f32;
+    decltype(&cuvit_gated_gemm_bf16) gated_gemm_bf16;
+    decltype(&cuvit_gated_backward_f32) gated_backward_f32;
+    decltype(&cuvit_gated_backward_bf16) gated_backward_bf16;
 };
 Library library{};
-PyObject* gemm_problem_type = nullptr;
-PyObject* preprocessing_type = nullptr;
+/// The problem structs' ctypes types.
+enum Problem { kGemm, kPreprocessing, kRotary, kQkNorm, kGated, kProblems };
+PyObject* problem_types[kProblems] = {};
 
 /// A plain torch tensor's fields, or false.
 const at::Tensor* plain_tensor(PyObject* object) {
@@ -289,7 +301,7 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (count != 7 || !storage(args[6], args[0], &type)) {
             return kNotPlain;
         }
-        const Struct view(args[4], gemm_problem_type, sizeof(cuvit_gemm_problem));
+        const Struct view(args[4], problem_types[kGemm], sizeof(cuvit_gemm_problem));
         const auto* const p = static_cast<const cuvit_gemm_problem*>(view.get());
         if (p == nullptr || p->m <= 0 || p->n <= 0 || p->k <= 0 || p->batch.count <= 0 ||
             (p->layout != CUVIT_GEMM_NO_TRANSPOSE && p->layout != CUVIT_GEMM_TRANSPOSED)) {
@@ -365,7 +377,7 @@ PyObject* preprocess(PyObject*, PyObject* const* a, Py_ssize_t count) {
         if (count != 7 || !positive(a[2], &batch) || !positive(a[3], &width) || !positive(a[4], &height)) {
             return kNotPlain;
         }
-        const Struct view(a[5], preprocessing_type, sizeof(cuvit_preprocessing));
+        const Struct view(a[5], problem_types[kPreprocessing], sizeof(cuvit_preprocessing));
         const auto* const settings = static_cast<const cuvit_preprocessing*>(view.get());
         if (settings == nullptr || settings->size <= 0 || !product(&in, {batch, height, width, 3}) ||
             !product(&out, {batch, 3, settings->size, settings->size})) {
@@ -405,16 +417,304 @@ PyObject* vit_forward(PyObject*, PyObject* const* a, Py_ssize_t count) {
     });
 }
 
-// (GemmProblem, Preprocessing, address of each of Library's functions in order)
+/// The GPU whose stream a launch goes to: current for None, else the stream's.
+bool device_of(PyObject* stream, int* out) {
+    if (stream == Py_None) {
+        *out = c10::hip::current_device();
+        return true;
+    }
+    PyObject* const index = PyObject_GetAttrString(stream, "device_index");
+    if (index == nullptr) {
+        PyErr_Clear();
+        return false;
+    }
+    const bool whole = PyLong_CheckExact(index);
+    *out = whole ? static_cast<int>(PyLong_AsLong(index)) : -1;
+    Py_DECREF(index);
+    if (PyErr_Occurred() != nullptr) {
+        PyErr_Clear();
+        return false;
+    }
+    return whole;
+}
+
+/// The operands of one launch: contiguous tensors on its GPU, or None where one
+/// may be missing. One that is not makes the whole not plain.
+class Operands {
+  public:
+    explicit Operands(PyObject* stream) { plain_ = device_of(stream, &device_) && stream_of(stream, &stream_); }
+
+    void* get(PyObject* object, at::ScalarType type, std::int64_t elements) {
+        void* const address = operand(object, type, elements);
+        if (address == nullptr || plain_tensor(object)->device().index() != device_) {
+            plain_ = false;
+        }
+        return address;
+    }
+    void* maybe(PyObject* object, at::ScalarType type, std::int64_t elements) {
+        return object == Py_None ? nullptr : get(object, type, elements);
+    }
+    float* floats(PyObject* object, std::int64_t elements) {
+        return static_cast<float*>(maybe(object, at::kFloat, elements));
+    }
+    bool plain() const { return plain_; }
+    cuvit_stream_t stream() const { return stream_; }
+
+  private:
+    bool plain_ = false;
+    int device_ = -1;
+    cuvit_stream_t stream_ = nullptr;
+};
+
+/// The floats that a rotation's positions and frequencies reach; 0 and 0 without
+/// a pair, when both may be missing.
+bool rotation_reach(const cuvit_rotation& r, int images, int tokens, std::int64_t* positions,
+                    std::int64_t* frequencies) {
+    if (r.axes < 0 || r.axes > 3 || r.position_stride < 0 || r.position_stride > (std::int64_t{1} << 31)) {
+        return false;
+    }
+    std::int64_t total = 0;
+    for (int axis = 0; axis < r.axes; ++axis) {
+        if (r.pairs[axis] < 0) {
+            return false;
+        }
+        total += r.pairs[axis];
+    }
+    *frequencies = total;
+    *positions = total > 0 ? (images - 1) * r.position_stride + static_cast<std::int64_t>(tokens) * r.axes : 0;
+    return true;
+}
+
+const std::uint16_t* bits(const void* p) { return static_cast<const std::uint16_t*>(p); }
+std::uint16_t* bits(void* p) { return static_cast<std::uint16_t*>(p); }
+const float* singles(const void* p) { return static_cast<const float*>(p); }
+float* singles(void* p) { return static_cast<float*>(p); }
+
+/// The elements that heads placed by strides reach.
+bool heads_reach(const cuvit_rotary_problem& p, const cuvit_head_strides& s, std::int64_t* out) {
+    constexpr std::int64_t kLimit = std::int64_t{1} << 40;
+    std::int64_t image, token;
+    if (!product(&image, {p.tokens, p.heads, p.head_dim}) || !product(&token, {p.heads, p.head_dim})) {
+        return false;
+    }
+    image = s.image != 0 ? s.image : image;
+    token = s.token != 0 ? s.token : token;
+    const std::int64_t head = s.head != 0 ? s.head : p.head_dim;
+    if (image < 0 || token < 0 || head < 0) {
+        return false;
+    }
+    std::int64_t spans[3];
+    if (!product(&spans[0], {p.images, image + 1}) || !product(&spans[1], {p.tokens, token + 1}) ||
+        !product(&spans[2], {p.heads, head + 1}) || spans[0] > kLimit || spans[1] > kLimit || spans[2] > kLimit) {
+        return false;
+    }
+    *out = (p.images - 1) * image + (p.tokens - 1) * token + (p.heads - 1) * head + p.head_dim;
+    return true;
+}
+
+// (x, positions, frequencies, out, problem, stream, bf16)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 7 || !storage(a[6], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[4], problem_types[kRotary], sizeof(cuvit_rotary_problem));
+        const auto* const p = static_cast<const cuvit_rotary_problem*>(view.get());
+        std::int64_t in, out, positions, frequencies;
+        if (p == nullptr || p->images <= 0 || p->tokens <= 0 || p->heads <= 0 || p->head_dim <= 0 ||
+            !heads_reach(*p, p->input, &in) || !heads_reach(*p, p->output, &out) ||
+            !rotation_reach(p->rotation, p->images, p->tokens, &positions, &frequencies)) {
+            return kNotPlain;
+        }
+        Operands operands(a[5]);
+        const void* const x = operands.get(a[0], type, in);
+        const float* const at = operands.floats(a[1], positions);
+        const float* const turns = operands.floats(a[2], frequencies);
+        void* const to = operands.get(a[3], type, out);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat ? library.rotary_f32(singles(x), at, turns, singles(to), p, operands.stream())
+                                      : library.rotary_bf16(bits(x), at, turns, bits(to), p, operands.stream());
+        });
+    });
+}
+
+/// The elements of a packed projection, or false for one that is not plain.
+bool packed_reach(const cuvit_qk_norm_problem* p, std::int64_t* out) {
+    return p != nullptr && p->images > 0 && p->tokens > 0 && p->heads > 0 && p->kv_heads > 0 && p->head_dim > 0 &&
+           product(out, {p->images, p->tokens, p->heads + 2 * static_cast<std::int64_t>(p->kv_heads), p->head_dim});
+}
+
+// (qkv, q_gamma, k_gamma, positions, frequencies, out, problem, q_beta, k_beta, stream, bf16)
+PyObject* qk_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 11 || !storage(a[10], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[6], problem_types[kQkNorm], sizeof(cuvit_qk_norm_problem));
+        const auto* const p = static_cast<const cuvit_qk_norm_problem*>(view.get());
+        std::int64_t values, positions, frequencies;
+        if (!packed_reach(p, &values) ||
+            !rotation_reach(p->rotation, p->images, p->tokens, &positions, &frequencies)) {
+            return kNotPlain;
+        }
+        Operands operands(a[9]);
+        const void* const x = operands.get(a[0], type, values);
+        const float* const q_gamma = operands.floats(a[1], p->head_dim);
+        const float* const k_gamma = operands.floats(a[2], p->head_dim);
+        const float* const at = operands.floats(a[3], positions);
+        const float* const turns = operands.floats(a[4], frequencies);
+        void* const to = operands.get(a[5], type, values);
+        const float* const q_beta = operands.floats(a[7], p->head_dim);
+        const float* const k_beta = operands.floats(a[8], p->head_dim);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat
+                       ? library.qk_norm_rotary_f32(singles(x), q_gamma, q_beta, k_gamma, k_beta, at, turns,
+                                                    singles(to), p, operands.stream())
+                       : library.qk_norm_rotary_bf16(bits(x), q_gamma, q_beta, k_gamma, k_beta, at, turns, bits(to), p,
+                                                     operands.stream());
+        });
+    });
+}
+
+// (qkv, q_gamma, k_gamma, positions, frequencies, grad_out, grad_qkv, problem, workspace, grad_q_gamma,
+//  grad_k_gamma, grad_q_beta, grad_k_beta, stream, bf16)
+PyObject* qk_norm_rotary_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 15 || !storage(a[14], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[7], problem_types[kQkNorm], sizeof(cuvit_qk_norm_problem));
+        const auto* const p = static_cast<const cuvit_qk_norm_problem*>(view.get());
+        std::int64_t values, positions, frequencies;
+        if (!packed_reach(p, &values) ||
+            !rotation_reach(p->rotation, p->images, p->tokens, &positions, &frequencies)) {
+            return kNotPlain;
+        }
+        const std::int64_t bytes = library.qk_norm_rotary_workspace(p);
+        Operands operands(a[13]);
+        const void* const x = operands.get(a[0], type, values);
+        const float* const q_gamma = operands.floats(a[1], p->head_dim);
+        const float* const k_gamma = operands.floats(a[2], p->head_dim);
+        const float* const at = operands.floats(a[3], positions);
+        const float* const turns = operands.floats(a[4], frequencies);
+        const void* const grad = operands.get(a[5], type, values);
+        void* const to = operands.get(a[6], type, values);
+        void* const workspace = operands.maybe(a[8], at::kByte, bytes);
+        float* const grad_q_gamma = operands.floats(a[9], p->head_dim);
+        float* const grad_k_gamma = operands.floats(a[10], p->head_dim);
+        float* const grad_q_beta = operands.floats(a[11], p->head_dim);
+        float* const grad_k_beta = operands.floats(a[12], p->head_dim);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat
+                       ? library.qk_norm_rotary_backward_f32(singles(x), q_gamma, k_gamma, at, turns, singles(grad),
+                                                             singles(to), grad_q_gamma, grad_q_beta, grad_k_gamma,
+                                                             grad_k_beta, workspace, bytes, p, operands.stream())
+                       : library.qk_norm_rotary_backward_bf16(bits(x), q_gamma, k_gamma, at, turns, bits(grad),
+                                                              bits(to), grad_q_gamma, grad_q_beta, grad_k_gamma,
+                                                              grad_k_beta, workspace, bytes, p, operands.stream());
+        });
+    });
+}
+
+/// The elements that C and the preactivations of a gated product reach.
+bool gated_reach(const cuvit_gated_problem* p, std::int64_t* c, std::int64_t* pre) {
+    if (p == nullptr || p->m <= 0 || p->n <= 0 || p->n > 0x3FFFFFFF) {
+        return false;
+    }
+    const std::int64_t ldc = p->ldc != 0 ? p->ldc : p->n;
+    const std::int64_t ld_pre = p->ld_preactivations != 0 ? p->ld_preactivations : 2 * p->n;
+    *c = (p->m - 1) * ldc + p->n;
+    *pre = (p->m - 1) * ld_pre + 2 * p->n;
+    return ldc >= p->n && ld_pre >= 2 * p->n;
+}
+
+// (a, b, bias, c, problem, preactivations, stream, bf16)
+PyObject* gated_gemm(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 8 || !storage(a[7], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[4], problem_types[kGated], sizeof(cuvit_gated_problem));
+        const auto* const p = static_cast<const cuvit_gated_problem*>(view.get());
+        std::int64_t c_reach, pre_reach;
+        if (!gated_reach(p, &c_reach, &pre_reach) || p->k <= 0) {
+            return kNotPlain;
+        }
+        const std::int64_t lda = p->lda != 0 ? p->lda : p->k;
+        const std::int64_t ldb = p->ldb != 0 ? p->ldb : p->k;
+        if (lda < p->k || ldb < p->k) {
+            return kNotPlain;
+        }
+        Operands operands(a[6]);
+        const void* const left = operands.get(a[0], type, (p->m - 1) * lda + p->k);
+        const void* const right = operands.get(a[1], type, (2 * static_cast<std::int64_t>(p->n) - 1) * ldb + p->k);
+        const float* const bias = operands.floats(a[2], 2 * static_cast<std::int64_t>(p->n));
+        void* const c = operands.get(a[3], type, c_reach);
+        void* const pre = operands.maybe(a[5], type, pre_reach);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat ? library.gated_gemm_f32(singles(left), singles(right), bias, singles(c),
+                                                               singles(pre), p, operands.stream())
+                                      : library.gated_gemm_bf16(bits(left), bits(right), bias, bits(c), bits(pre), p,
+                                                                operands.stream());
+        });
+    });
+}
+
+// (preactivations, grad, grad_preactivations, problem, stream, bf16)
+PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 6 || !storage(a[5], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[3], problem_types[kGated], sizeof(cuvit_gated_problem));
+        const auto* const p = static_cast<const cuvit_gated_problem*>(view.get());
+        std::int64_t c_reach, pre_reach;
+        if (!gated_reach(p, &c_reach, &pre_reach)) {
+            return kNotPlain;
+        }
+        Operands operands(a[4]);
+        const void* const pre = operands.get(a[0], type, pre_reach);
+        const void* const grad = operands.get(a[1], type, c_reach);
+        void* const to = operands.get(a[2], type, pre_reach);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat
+                       ? library.gated_backward_f32(singles(pre), singles(grad), singles(to), p, operands.stream())
+                       : library.gated_backward_bf16(bits(pre), bits(grad), bits(to), p, operands.stream());
+        });
+    });
+}
+
+// (GemmProblem, Preprocessing, RotaryProblem, QkNormProblem, GatedProblem, address of each of Library's functions in
+//  order)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     constexpr Py_ssize_t kFunctions = sizeof(Library) / sizeof(void*);
-    if (count != 2 + kFunctions) {
-        PyErr_SetString(PyExc_TypeError, "bind takes the two struct types and every function's address");
+    if (count != kProblems + kFunctions) {
+        PyErr_SetString(PyExc_TypeError, "bind takes the struct types and every function's address");
         return nullptr;
     }
     void* addresses[kFunctions];
     for (Py_ssize_t i = 0; i < kFunctions; ++i) {
-        addresses[i] = PyLong_AsVoidPtr(a[2 + i]);
+        addresses[i] = PyLong_AsVoidPtr(a[kProblems + i]);
         if (addresses[i] == nullptr) {
             if (PyErr_Occurred() == nullptr) {
                 PyErr_SetString(PyExc_ValueError, "a function's address is null");
@@ -423,10 +723,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
         }
     }
     __builtin_memcpy(&library, addresses, sizeof(library));
-    Py_INCREF(a[0]);
-    Py_INCREF(a[1]);
-    Py_XSETREF(gemm_problem_type, a[0]);
-    Py_XSETREF(preprocessing_type, a[1]);
+    for (int i = 0; i < kProblems; ++i) {
+        Py_INCREF(a[i]);
+        Py_XSETREF(problem_types[i], a[i]);
+    }
     Py_RETURN_NONE;
 }
 
@@ -434,7 +734,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CUVIT_FAST(bind),           CUVIT_FAST(layer_norm), CUVIT_FAST(softmax),
                          CUVIT_FAST(extract_patches), CUVIT_FAST(gemm),       CUVIT_FAST(attention),
-                         CUVIT_FAST(preprocess),     CUVIT_FAST(vit_forward), {nullptr, nullptr, 0, nullptr}};
+                         CUVIT_FAST(preprocess),     CUVIT_FAST(vit_forward), CUVIT_FAST(rotary),
+                         CUVIT_FAST(qk_norm_rotary), CUVIT_FAST(qk_norm_rotary_backward), CUVIT_FAST(gated_gemm),
+                         CUVIT_FAST(gated_backward), {nullptr, nullptr, 0, nullptr}};
 #undef CUVIT_FAST
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "The launchers' plain case.", -1, methods,

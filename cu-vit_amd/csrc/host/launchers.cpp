@@ -128,4 +128,66 @@ void launch_broadcast(std::uint16_t* destination, const std::uint16_t* source, s
         cuvit_broadcast_bf16(destination, source, count, destination_stride, batch, as_c(stream)));
 }
 
+void launch_rotary(const float* input, const float* positions, const float* frequencies, float* output,
+                   const RotaryProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_rotary_f32(input, positions, frequencies, output, &problem, as_c(stream)));
+}
+
+void launch_rotary(const std::uint16_t* input, const float* positions, const float* frequencies, std::uint16_t* output,
+                   const RotaryProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_rotary_bf16(input, positions, frequencies, output, &problem, as_c(stream)));
+}
+
+void launch_qk_norm_rotary(const float* qkv, const QkNormWeights& weights, const float* positions,
+                           const float* frequencies, float* out, const QkNormProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_qk_norm_rotary_f32(qkv, weights.q_gamma, weights.q_beta, weights.k_gamma, weights.k_beta,
+                                           positions, frequencies, out, &problem, as_c(stream)));
+}
+
+void launch_qk_norm_rotary(const std::uint16_t* qkv, const QkNormWeights& weights, const float* positions,
+                           const float* frequencies, std::uint16_t* out, const QkNormProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_qk_norm_rotary_bf16(qkv, weights.q_gamma, weights.q_beta, weights.k_gamma, weights.k_beta,
+                                           positions, frequencies, out, &problem, as_c(stream)));
+}
+
+void launch_qk_norm_rotary_backward(const float* qkv, const QkNormWeights& weights, const float* positions,
+                                    const float* frequencies, const float* grad_out, float* grad_qkv,
+                                    const QkNormGradients& gradients, const QkNormProblem& problem,
+                                    hipStream_t stream) {
+    throw_on_error(cuvit_qk_norm_rotary_backward_f32(
+        qkv, weights.q_gamma, weights.k_gamma, positions, frequencies, grad_out, grad_qkv, gradients.q_gamma,
+        gradients.q_beta, gradients.k_gamma, gradients.k_beta, gradients.workspace, gradients.workspace_bytes,
+        &problem, as_c(stream)));
+}
+
+void launch_qk_norm_rotary_backward(const std::uint16_t* qkv, const QkNormWeights& weights, const float* positions,
+                                    const float* frequencies, const std::uint16_t* grad_out, std::uint16_t* grad_qkv,
+                                    const QkNormGradients& gradients, const QkNormProblem& problem,
+                                    hipStream_t stream) {
+    throw_on_error(cuvit_qk_norm_rotary_backward_bf16(
+        qkv, weights.q_gamma, weights.k_gamma, positions, frequencies, grad_out, grad_qkv, gradients.q_gamma,
+        gradients.q_beta, gradients.k_gamma, gradients.k_beta, gradients.workspace, gradients.workspace_bytes,
+        &problem, as_c(stream)));
+}
+
+void launch_gated_gemm(const float* a, const float* b, const float* bias, float* c, float* preactivations,
+                       const GatedProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_gated_gemm_f32(a, b, bias, c, preactivations, &problem, as_c(stream)));
+}
+
+void launch_gated_gemm(const std::uint16_t* a, const std::uint16_t* b, const float* bias, std::uint16_t* c, std::uint16_t* preactivations,
+                       const GatedProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_gated_gemm_bf16(a, b, bias, c, preactivations, &problem, as_c(stream)));
+}
+
+void launch_gated_backward(const float* preactivations, const float* grad, float* grad_preactivations,
+                           const GatedProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_gated_backward_f32(preactivations, grad, grad_preactivations, &problem, as_c(stream)));
+}
+
+void launch_gated_backward(const std::uint16_t* preactivations, const std::uint16_t* grad, std::uint16_t* grad_preactivations,
+                           const GatedProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_gated_backward_bf16(preactivations, grad, grad_preactivations, &problem, as_c(stream)));
+}
+
 } // namespace cuvit

@@ -167,6 +167,87 @@ hipError_t attention_long_f32(const float* qkv, float* context, int images, int 
 hipError_t attention_long_bf16(const std::uint16_t* qkv, std::uint16_t* context, int images, int heads,
                                int tokens, hipStream_t stream);
 
+// rotary.hip and qk_norm_backward.hip. Strides and the problem's pairs are
+// resolved and checked.
+struct HeadStrides {
+    std::int64_t image;
+    std::int64_t token;
+    std::int64_t head;
+};
+struct Rotation {
+    const float* positions;
+    const float* frequencies;
+    std::int64_t position_stride;
+    int axes;
+    int pairs;      // of all axes
+    int first[2];   // the first pair of axes 1 and 2
+    bool adjacent;
+    bool inverse;
+};
+enum class HeadNorm { kNone, kRms, kLayer };
+/// Heads to normalise and rotate: `heads` of every token, the first `q_heads`
+/// with the first gamma and beta, the others with the second. `copied` more
+/// heads behind them are copied where the output is another tensor (packed
+/// tensors only: the same strides, images that follow one another).
+struct HeadArgs {
+    int images;
+    int tokens;
+    int heads;
+    int q_heads;
+    int copied;
+    int head_dim;
+    HeadStrides input;
+    HeadStrides output;
+    Rotation rotation;
+    HeadNorm norm;
+    float epsilon;
+    const float* gamma[2];
+    const float* beta[2];
+};
+hipError_t rotate_heads(const float* input, float* output, const HeadArgs& args, hipStream_t stream);
+hipError_t rotate_heads(const std::uint16_t* input, std::uint16_t* output, const HeadArgs& args,
+                        hipStream_t stream);
+
+/// The gradients of gamma and beta of the query and the key heads (null: not
+/// wanted) and the workspace for their partial sums.
+struct HeadGradients {
+    float* gamma[2];
+    float* beta[2];
+    float* workspace;
+};
+/// Bytes of that workspace, whatever the sizes.
+std::int64_t rotate_heads_workspace(int head_dim);
+/// Zeros for those that are wanted: sums over no tokens.
+hipError_t rotate_heads_no_tokens(const HeadGradients& gradients, int head_dim, hipStream_t stream);
+/// Gradients of rotate_heads with a norm; the `input` strides, packed ones,
+/// are the forward input's and the gradients' alike.
+hipError_t rotate_heads_backward(const float* input, const float* grad_output, float* grad_input,
+                                 const HeadGradients& gradients, const HeadArgs& args, hipStream_t stream);
+hipError_t rotate_heads_backward(const std::uint16_t* input, const std::uint16_t* grad_output,
+                                 std::uint16_t* grad_input, const HeadGradients& gradients, const HeadArgs& args,
+                                 hipStream_t stream);
+
+// gated.hip. Leading dimensions are resolved.
+enum class Gate { kSilu, kGelu, kGeluTanh };
+struct GatedArgs {
+    int m;
+    int n;
+    int k;
+    Gate gate;
+    int lda;
+    int ldb;
+    int ldc;
+    int ld_pre;
+};
+hipError_t gated_gemm(const float* a, const float* b, const float* bias, float* c, float* preactivations,
+                      const GatedArgs& args, hipStream_t stream);
+hipError_t gated_gemm(const std::uint16_t* a, const std::uint16_t* b, const float* bias, std::uint16_t* c,
+                      std::uint16_t* preactivations, const GatedArgs& args, hipStream_t stream);
+hipError_t gated_backward(const float* preactivations, const float* grad, float* grad_preactivations,
+                          const GatedArgs& args, hipStream_t stream);
+hipError_t gated_backward(const std::uint16_t* preactivations, const std::uint16_t* grad,
+                          std::uint16_t* grad_preactivations, const GatedArgs& args, hipStream_t stream);
+
 // Device facts used to shape grids, cached per device.
 int compute_units();
 

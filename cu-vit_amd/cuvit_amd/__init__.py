@@ -30,6 +30,11 @@ __all__ = [
     "gemm_problem", "WeightWriter", "WeightFile", "VisionTransformer",
     "NO_TRANSPOSE", "TRANSPOSED", "PRECISION_F32", "PRECISION_BF16",
     "Preprocessing", "RgbImage", "load_ppm", "preprocess", "preprocess_image", "cli_path",
+    "RotaryProblem", "QkNormProblem", "GatedProblem", "rotary_problem", "qk_norm_problem", "gated_problem",
+    "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "qk_norm_rotary_workspace",
+    "gated_gemm", "gated_backward",
+    "ROTARY_HALVES", "ROTARY_ADJACENT", "NORM_RMS", "NORM_LAYER",
+    "GATE_SILU", "GATE_GELU", "GATE_GELU_TANH",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -40,6 +45,16 @@ TRANSPOSED = 1
 
 PRECISION_F32 = 0
 PRECISION_BF16 = 1
+
+ROTARY_HALVES = 0
+ROTARY_ADJACENT = 1
+
+NORM_RMS = 0
+NORM_LAYER = 1
+
+GATE_SILU = 0
+GATE_GELU = 1
+GATE_GELU_TANH = 2
 
 OK = 0
 ERROR_INVALID_ARGUMENT = 1
@@ -160,6 +175,70 @@ class Preprocessing(ctypes.Structure):
                          (ctypes.c_float * 3)(*stddev))
 
 
+class Rotation(ctypes.Structure):
+    """cuvit_rotation: how a head's values pair up, how many pairs each axis
+    owns, and the floats from one image's positions to the next (0: shared)."""
+
+    _fields_ = [
+        ("pairing", ctypes.c_int32),
+        ("axes", ctypes.c_int),
+        ("pairs", ctypes.c_int * 3),
+        ("position_stride", ctypes.c_int64),
+    ]
+
+
+class HeadStrides(ctypes.Structure):
+    """cuvit_head_strides: elements from one image, token and head to the next;
+    0 selects the packed [images, tokens, heads, head_dim] one."""
+
+    _fields_ = [("image", ctypes.c_int64), ("token", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class RotaryProblem(ctypes.Structure):
+    """cuvit_rotary_problem."""
+
+    _fields_ = [
+        ("images", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("rotation", Rotation),
+        ("inverse", ctypes.c_uint8),
+        ("input", HeadStrides),
+        ("output", HeadStrides),
+    ]
+
+
+class QkNormProblem(ctypes.Structure):
+    """cuvit_qk_norm_problem."""
+
+    _fields_ = [
+        ("images", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("norm", ctypes.c_int32),
+        ("epsilon", ctypes.c_float),
+        ("rotation", Rotation),
+    ]
+
+
+class GatedProblem(ctypes.Structure):
+    """cuvit_gated_problem."""
+
+    _fields_ = [
+        ("m", ctypes.c_int),
+        ("n", ctypes.c_int),
+        ("k", ctypes.c_int),
+        ("activation", ctypes.c_int32),
+        ("lda", ctypes.c_int),
+        ("ldb", ctypes.c_int),
+        ("ldc", ctypes.c_int),
+        ("ld_preactivations", ctypes.c_int),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
@@ -189,6 +268,21 @@ _SIGNATURES = {
     "cuvit_attention_supported": (_I, [_I, _I]),
     "cuvit_attention_f32": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "cuvit_attention_bf16": (_I, [_P, _P, _I, _I, _I, _I, _P]),
+    "cuvit_rotary_problem_init": (None, [ctypes.POINTER(RotaryProblem), _I, _I, _I, _I, _I, ctypes.POINTER(_I), _I]),
+    "cuvit_rotary_f32": (_I, [_P, _P, _P, _P, ctypes.POINTER(RotaryProblem), _P]),
+    "cuvit_rotary_bf16": (_I, [_P, _P, _P, _P, ctypes.POINTER(RotaryProblem), _P]),
+    "cuvit_qk_norm_problem_init": (None, [ctypes.POINTER(QkNormProblem), _I, _I, _I, _I, _I,
+                                          ctypes.POINTER(_I), _I, _I]),
+    "cuvit_qk_norm_rotary_f32": (_I, [_P] * 8 + [ctypes.POINTER(QkNormProblem), _P]),
+    "cuvit_qk_norm_rotary_bf16": (_I, [_P] * 8 + [ctypes.POINTER(QkNormProblem), _P]),
+    "cuvit_qk_norm_rotary_workspace": (_L, [ctypes.POINTER(QkNormProblem)]),
+    "cuvit_qk_norm_rotary_backward_f32": (_I, [_P] * 12 + [_L, ctypes.POINTER(QkNormProblem), _P]),
+    "cuvit_qk_norm_rotary_backward_bf16": (_I, [_P] * 12 + [_L, ctypes.POINTER(QkNormProblem), _P]),
+    "cuvit_gated_problem_init": (None, [ctypes.POINTER(GatedProblem), _I, _I, _I, _I]),
+    "cuvit_gated_gemm_f32": (_I, [_P, _P, _P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_gemm_bf16": (_I, [_P, _P, _P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_backward_f32": (_I, [_P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_backward_bf16": (_I, [_P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
     "cuvit_weight_writer_create": (_I, [ctypes.POINTER(_P)]),
     "cuvit_weight_writer_add": (_I, [_P, ctypes.c_char_p, _I, ctypes.POINTER(_L), _P]),
     "cuvit_weight_writer_add_bf16": (_I, [_P, ctypes.c_char_p, _I, ctypes.POINTER(_L), _P]),
@@ -251,10 +345,14 @@ _NATIVE_FUNCTIONS = (
     "cuvit_layer_norm_f32", "cuvit_layer_norm_bf16", "cuvit_softmax_f32", "cuvit_softmax_bf16",
     "cuvit_extract_patches_f32", "cuvit_extract_patches_bf16", "cuvit_gemm_f32", "cuvit_gemm_bf16",
     "cuvit_attention_f32", "cuvit_attention_bf16", "cuvit_preprocess_u8", "cuvit_vit_forward",
+    "cuvit_rotary_f32", "cuvit_rotary_bf16", "cuvit_qk_norm_rotary_f32", "cuvit_qk_norm_rotary_bf16",
+    "cuvit_qk_norm_rotary_backward_f32", "cuvit_qk_norm_rotary_backward_bf16", "cuvit_qk_norm_rotary_workspace",
+    "cuvit_gated_gemm_f32", "cuvit_gated_gemm_bf16", "cuvit_gated_backward_f32", "cuvit_gated_backward_bf16",
 )
 
 
-_NATIVE_CALLS = ("layer_norm", "softmax", "extract_patches", "gemm", "attention", "preprocess", "vit_forward")
+_NATIVE_CALLS = ("layer_norm", "softmax", "extract_patches", "gemm", "attention", "preprocess", "vit_forward",
+                 "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "gated_gemm", "gated_backward")
 
 
 def _not_plain(*arguments) -> int:
@@ -303,7 +401,7 @@ class _NativeCalls:
                 native = _native_module(torch)
                 if native is not None:
                     lib = library()
-                    native.bind(GemmProblem, Preprocessing,
+                    native.bind(GemmProblem, Preprocessing, RotaryProblem, QkNormProblem, GatedProblem,
                                 *(ctypes.cast(getattr(lib, f), _P).value for f in _NATIVE_FUNCTIONS))
                 for call in _NATIVE_CALLS:
                     setattr(self, call, getattr(native, call) if native is not None else _not_plain)
@@ -580,6 +678,233 @@ def attention(qkv, context, images: int, heads: int, tokens: int, head_dim: int,
         qkv = _operand(qkv, "qkv", _storage(bf16), 3 * n)
         context = _operand(context, "context", _storage(bf16), n)
     check(fn(_ptr(qkv), _ptr(context), images, heads, tokens, head_dim, stream_handle(stream)))
+
+
+def _launch_device(stream, *operands) -> None:
+    """Refuses operands that are on another GPU than the launch: a kernel there
+    would reach into this one's memory, or fault."""
+    tensors = [x for x in operands if x is not None and not isinstance(x, int) and x.device.type == "cuda"]
+    if not tensors:
+        return
+    import torch
+
+    index = stream.device.index if stream is not None else torch.cuda.current_device()
+    for x in tensors:
+        if x.device.index != index:
+            raise InvalidArgument(ERROR_INVALID_ARGUMENT,
+                                  f"an operand is on {x.device}, the launch on cuda:{index}")
+
+
+def _pair_counts(pairs):
+    counts = [int(p) for p in pairs]
+    return len(counts), (ctypes.c_int * max(len(counts), 1))(*counts)
+
+
+def rotary_problem(images: int, tokens: int, heads: int, head_dim: int, pairs,
+                   pairing: int = ROTARY_HALVES) -> RotaryProblem:
+    """The rotation of packed [images, tokens, heads, head_dim] heads, ``pairs``
+    counting each axis' pairs (at most three axes; head_dim // 2 pairs in all
+    turn whole heads). A ladder of frequencies for an axis of n pairs is
+    ``base ** (-i / n)``, i from 0."""
+    problem = RotaryProblem()
+    axes, counts = _pair_counts(pairs)
+    library().cuvit_rotary_problem_init(ctypes.byref(problem), images, tokens, heads, head_dim, axes, counts, pairing)
+    return problem
+
+
+def qk_norm_problem(images: int, tokens: int, heads: int, head_dim: int, pairs=(),
+                    pairing: int = ROTARY_HALVES, norm: int = NORM_RMS, epsilon: float = 1.0e-6,
+                    kv_heads: Optional[int] = None) -> QkNormProblem:
+    """The norm (and rotation, if there are pairs) of a packed projection
+    [images, tokens, heads + 2 kv_heads, head_dim]; kv_heads as many as heads
+    unless given."""
+    problem = QkNormProblem()
+    axes, counts = _pair_counts(pairs)
+    library().cuvit_qk_norm_problem_init(ctypes.byref(problem), images, tokens, heads, head_dim, axes, counts,
+                                         pairing, norm)
+    problem.epsilon = epsilon
+    if kv_heads is not None:
+        problem.kv_heads = kv_heads
+    return problem
+
+
+def gated_problem(m: int, n: int, k: int, activation: int = GATE_SILU) -> GatedProblem:
+    """A gated product of packed operands: A [m, k], B [2 n, k], C [m, n]."""
+    problem = GatedProblem()
+    library().cuvit_gated_problem_init(ctypes.byref(problem), m, n, k, activation)
+    return problem
+
+
+def _rotation_operands(rotation: Rotation, images: int, tokens: int, positions, frequencies):
+    if not 0 <= rotation.axes <= 3 or rotation.position_stride < 0:
+        return _ptr(positions), _ptr(frequencies)  # the library names what is wrong
+    total = sum(rotation.pairs[:rotation.axes])
+    if total <= 0 or min(rotation.pairs[:rotation.axes]) < 0:
+        return _ptr(positions), _ptr(frequencies)
+    reach = (images - 1) * rotation.position_stride + tokens * rotation.axes
+    return (_operand(positions, "positions", "float32", reach),
+            _operand(frequencies, "frequencies", "float32", total))
+
+
+def rotary(x, positions, frequencies, out, problem: RotaryProblem, stream=None, bf16: Optional[bool] = None) -> None:
+    """Rotates heads by their tokens' positions on up to three axes (row and
+    column of a patch; time too): pair i of a token turns by
+    ``positions[token, axis of i] * frequencies[i]`` radians, the angle taken in
+    64 bits. x and out are [images, tokens, heads, head_dim], or as the problem's
+    strides say; out may be x. ``problem.inverse`` turns back, which is also the
+    gradient: grad_x is the inverse rotation of grad_out. An extension."""
+    status = _native_calls.rotary(x, positions, frequencies, out, problem, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(x)
+    fn = library().cuvit_rotary_bf16 if bf16 else library().cuvit_rotary_f32
+    p = problem
+    if _positive(p.images, p.tokens, p.heads, p.head_dim):
+        _launch_device(stream, x, positions, frequencies, out)
+
+        def reach(s: HeadStrides) -> int:
+            return ((p.images - 1) * (s.image or p.tokens * p.heads * p.head_dim)
+                    + (p.tokens - 1) * (s.token or p.heads * p.head_dim)
+                    + (p.heads - 1) * (s.head or p.head_dim) + p.head_dim)
+
+        positions, frequencies = _rotation_operands(p.rotation, p.images, p.tokens, positions, frequencies)
+        x = _operand(x, "x", _storage(bf16), reach(p.input))
+        out = _operand(out, "out", _storage(bf16), reach(p.output))
+    check(fn(_ptr(x), _ptr(positions), _ptr(frequencies), _ptr(out), ctypes.byref(problem), stream_handle(stream)))
+
+
+def _qk_norm_operands(p: QkNormProblem, bf16: bool, packed, weights, positions, frequencies):
+    values = p.images * p.tokens * (p.heads + 2 * p.kv_heads) * p.head_dim
+    positions, frequencies = _rotation_operands(p.rotation, p.images, p.tokens, positions, frequencies)
+    return ([_operand(x, name, _storage(bf16), values) for name, x in packed.items()],
+            [_operand(x, name, "float32", p.head_dim) for name, x in weights.items()], positions, frequencies)
+
+
+def qk_norm_rotary(qkv, q_gamma, k_gamma, positions, frequencies, out, problem: QkNormProblem, q_beta=None,
+                   k_beta=None, stream=None, bf16: Optional[bool] = None) -> None:
+    """Normalises each query and key head of a packed projection
+    [images, tokens, heads + 2 kv_heads, head_dim], scales (gamma), shifts (beta)
+    and rotates it, in one pass. out may be qkv: the value heads then stay, else
+    they are copied. With kv_heads = heads the result is attention()'s qkv.
+    gamma and beta are [head_dim] fp32, None for 1 and 0. An extension."""
+    status = _native_calls.qk_norm_rotary(qkv, q_gamma, k_gamma, positions, frequencies, out, problem, q_beta,
+                                          k_beta, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(qkv)
+    fn = library().cuvit_qk_norm_rotary_bf16 if bf16 else library().cuvit_qk_norm_rotary_f32
+    p = problem
+    if _positive(p.images, p.tokens, p.heads, p.kv_heads, p.head_dim):
+        _launch_device(stream, qkv, q_gamma, k_gamma, positions, frequencies, out, q_beta, k_beta)
+        (qkv, out), (q_gamma, k_gamma, q_beta, k_beta), positions, frequencies = _qk_norm_operands(
+            p, bf16, {"qkv": qkv, "out": out},
+            {"q_gamma": q_gamma, "k_gamma": k_gamma, "q_beta": q_beta, "k_beta": k_beta}, positions, frequencies)
+    check(fn(_ptr(qkv), _ptr(q_gamma), _ptr(q_beta), _ptr(k_gamma), _ptr(k_beta), _ptr(positions),
+             _ptr(frequencies), _ptr(out), ctypes.byref(problem), stream_handle(stream)))
+
+
+def qk_norm_rotary_workspace(problem: QkNormProblem) -> int:
+    """Bytes of the workspace that qk_norm_rotary_backward() sums in."""
+    return library().cuvit_qk_norm_rotary_workspace(ctypes.byref(problem))
+
+
+def qk_norm_rotary_backward(qkv, q_gamma, k_gamma, positions, frequencies, grad_out, grad_qkv,
+                            problem: QkNormProblem, workspace=None, grad_q_gamma=None, grad_k_gamma=None,
+                            grad_q_beta=None, grad_k_beta=None, stream=None, bf16: Optional[bool] = None) -> None:
+    """The gradients of qk_norm_rotary() from its input qkv and the gradient of
+    its whole packed output; grad_qkv may be grad_out. The gradients of gamma and
+    beta ([head_dim] fp32, overwritten, None: not computed) are summed in
+    ``workspace``, a uint8 tensor of qk_norm_rotary_workspace() bytes that one
+    call uses at a time: calls on several streams, and captured graphs that may
+    overlap, take one each."""
+    status = _native_calls.qk_norm_rotary_backward(qkv, q_gamma, k_gamma, positions, frequencies, grad_out, grad_qkv,
+                                                   problem, workspace, grad_q_gamma, grad_k_gamma, grad_q_beta,
+                                                   grad_k_beta, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(qkv)
+    fn = library().cuvit_qk_norm_rotary_backward_bf16 if bf16 else library().cuvit_qk_norm_rotary_backward_f32
+    p = problem
+    nbytes = qk_norm_rotary_workspace(p)
+    if _positive(p.images, p.tokens, p.heads, p.kv_heads, p.head_dim):
+        _launch_device(stream, qkv, q_gamma, k_gamma, positions, frequencies, grad_out, grad_qkv, workspace,
+                       grad_q_gamma, grad_k_gamma, grad_q_beta, grad_k_beta)
+        packed, weights, positions, frequencies = _qk_norm_operands(
+            p, bf16, {"qkv": qkv, "grad_out": grad_out, "grad_qkv": grad_qkv},
+            {"q_gamma": q_gamma, "k_gamma": k_gamma, "grad_q_gamma": grad_q_gamma, "grad_k_gamma": grad_k_gamma,
+             "grad_q_beta": grad_q_beta, "grad_k_beta": grad_k_beta}, positions, frequencies)
+        qkv, grad_out, grad_qkv = packed
+        q_gamma, k_gamma, grad_q_gamma, grad_k_gamma, grad_q_beta, grad_k_beta = weights
+        workspace = _operand(workspace, "workspace", "uint8", nbytes)
+    elif _positive(p.heads, p.head_dim):  # no tokens: the gradients are zeros
+        _launch_device(stream, grad_q_gamma, grad_k_gamma, grad_q_beta, grad_k_beta)
+        grad_q_gamma, grad_k_gamma, grad_q_beta, grad_k_beta = (
+            _operand(x, name, "float32", p.head_dim) for name, x in
+            (("grad_q_gamma", grad_q_gamma), ("grad_k_gamma", grad_k_gamma), ("grad_q_beta", grad_q_beta),
+             ("grad_k_beta", grad_k_beta)))
+    check(fn(_ptr(qkv), _ptr(q_gamma), _ptr(k_gamma), _ptr(positions), _ptr(frequencies), _ptr(grad_out),
+             _ptr(grad_qkv), _ptr(grad_q_gamma), _ptr(grad_q_beta), _ptr(grad_k_gamma), _ptr(grad_k_beta),
+             _ptr(workspace), nbytes, ctypes.byref(problem), stream_handle(stream)))
+
+
+def _gated_reach(p: GatedProblem):
+    """Elements that C and the preactivations reach, or None where a leading
+    dimension is too small (the library names it)."""
+    ldc, ld_pre = p.ldc or p.n, p.ld_preactivations or 2 * p.n
+    if ldc < p.n or ld_pre < 2 * p.n:
+        return None
+    return (p.m - 1) * ldc + p.n, (p.m - 1) * ld_pre + 2 * p.n
+
+
+def gated_gemm(a, b, bias, c, problem: GatedProblem, preactivations=None, stream=None,
+               bf16: Optional[bool] = None) -> None:
+    """C = activation(gate) * value with [gate, value] = A.B^T + bias: a gated
+    MLP's first product. B is a Linear layer's weight [2 n, k], the gate's n rows
+    first, bias [2 n] fp32 or None. A ``preactivations`` tensor [m, 2 n] receives
+    [gate, value], for gated_backward(). An extension."""
+    status = _native_calls.gated_gemm(a, b, bias, c, problem, preactivations, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(a)
+    fn = library().cuvit_gated_gemm_bf16 if bf16 else library().cuvit_gated_gemm_f32
+    p = problem
+    if _positive(p.m, p.n) and p.k >= 0:
+        _launch_device(stream, a, b, bias, c, preactivations)
+        reach = _gated_reach(p)
+        lda, ldb = p.lda or p.k, p.ldb or p.k
+        if reach is not None and lda >= p.k and ldb >= p.k:
+            t = _storage(bf16)
+            a = _operand(a, "A", t, (p.m - 1) * lda + p.k)
+            b = _operand(b, "B", t, (2 * p.n - 1) * ldb + p.k)
+            bias = _operand(bias, "bias", "float32", 2 * p.n)
+            c = _operand(c, "C", t, reach[0])
+            preactivations = _operand(preactivations, "preactivations", t, reach[1])
+    check(fn(_ptr(a), _ptr(b), _ptr(bias), _ptr(c), _ptr(preactivations), ctypes.byref(problem),
+             stream_handle(stream)))
+
+
+def gated_backward(preactivations, grad, grad_preactivations, problem: GatedProblem, stream=None,
+                   bf16: Optional[bool] = None) -> None:
+    """The gate's gradient: from the preactivations [m, 2 n] that gated_gemm()
+    kept and the gradient [m, n] of its result, the gradient of the
+    preactivations (which may take their place). The gradients of A and of the
+    weight are plain products with it. An extension."""
+    status = _native_calls.gated_backward(preactivations, grad, grad_preactivations, problem, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(preactivations)
+    fn = library().cuvit_gated_backward_bf16 if bf16 else library().cuvit_gated_backward_f32
+    p = problem
+    if _positive(p.m, p.n):
+        _launch_device(stream, preactivations, grad, grad_preactivations)
+        reach = _gated_reach(p)
+        if reach is not None:
+            t = _storage(bf16)
+            preactivations = _operand(preactivations, "preactivations", t, reach[1])
+            grad = _operand(grad, "grad", t, reach[0])
+            grad_preactivations = _operand(grad_preactivations, "grad_preactivations", t, reach[1])
+    check(fn(_ptr(preactivations), _ptr(grad), _ptr(grad_preactivations), ctypes.byref(problem),
+             stream_handle(stream)))
 
 
 class WeightWriter:

@@ -150,6 +150,176 @@ int cuvit_attention_bf16(const cuvit_bf16* qkv, cuvit_bf16* context, int images,
                          int tokens, int head_dim, cuvit_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Operators of rotary, gated ViT blocks. Extensions: the reference's block has
+ * additive positions, plain queries and keys and one GELU MLP. They follow the
+ * rules at the top of this file; storage is fp32 or bf16 (the _bf16 twins),
+ * everything between a load and a store is fp32, and each result is rounded
+ * once. A null problem is CUVIT_ERROR_INVALID_ARGUMENT before all else.
+ * ------------------------------------------------------------------------- */
+
+/* Which values of a head form a pair, `pairs` being the rotated pairs in all:
+ * value i with value pairs + i, or values 2 i and 2 i + 1. Values from
+ * 2 pairs on are not rotated. */
+typedef enum cuvit_rotary_pairing {
+    CUVIT_ROTARY_HALVES = 0,
+    CUVIT_ROTARY_ADJACENT = 1
+} cuvit_rotary_pairing;
+
+/* A rotation by positions on several axes (a patch's row and column, a video's
+ * time as well). Pair i of a token turns by positions[a] * frequencies[i]
+ * radians, a being the axis that owns pair i: the first pairs[0] pairs are axis
+ * 0's, the next pairs[1] axis 1's, and so on. Angles are formed and reduced in
+ * 64 bits, so far positions keep their fraction. Position 0 leaves finite
+ * values as they are (a class token's). Positions are [tokens, axes] fp32, the
+ * same for every image with position_stride 0, else each image's that many
+ * floats behind the last one's; frequencies are [pairs] fp32. No axes or no
+ * pairs: no rotation, and both may be null. */
+typedef struct cuvit_rotation {
+    int32_t pairing; /* cuvit_rotary_pairing */
+    int axes;        /* 0 to 3 */
+    int pairs[3];
+    int64_t position_stride;
+} cuvit_rotation;
+
+/* Elements from one image, token and head to the next; 0 selects the packed
+ * [images, tokens, heads, head_dim] one. */
+typedef struct cuvit_head_strides {
+    int64_t image;
+    int64_t token;
+    int64_t head;
+} cuvit_head_strides;
+
+typedef struct cuvit_rotary_problem {
+    int images;
+    int tokens;
+    int heads;
+    int head_dim; /* even, at most 512 */
+    cuvit_rotation rotation;
+    uint8_t inverse; /* turn back: the gradient of the rotation */
+    cuvit_head_strides input;
+    cuvit_head_strides output;
+} cuvit_rotary_problem;
+
+/* Fills *problem with packed layouts and positions that all images share;
+ * pairs holds @p axes counts (more than 3 are kept as a bad axis count). */
+void cuvit_rotary_problem_init(cuvit_rotary_problem* problem, int images, int tokens, int heads,
+                               int head_dim, int axes, const int* pairs, int pairing);
+
+/* Rotates heads: out = rotation(input). input == output (in place) is allowed
+ * with equal strides. Strides are not negative and no two of the output's
+ * heads overlap. More than 2^31 - 1 tokens in all are CUVIT_ERROR_LENGTH. */
+int cuvit_rotary_f32(const float* input, const float* positions, const float* frequencies,
+                     float* output, const cuvit_rotary_problem* problem, cuvit_stream_t stream);
+int cuvit_rotary_bf16(const cuvit_bf16* input, const float* positions, const float* frequencies,
+                      cuvit_bf16* output, const cuvit_rotary_problem* problem,
+                      cuvit_stream_t stream);
+
+typedef enum cuvit_norm {
+    CUVIT_NORM_RMS = 0,  /* x / sqrt(mean(x^2) + epsilon) */
+    CUVIT_NORM_LAYER = 1 /* the same of x - mean(x) */
+} cuvit_norm;
+
+/* The packed projection [images, tokens, heads + 2 kv_heads, head_dim]: query
+ * heads, then key heads, then value heads. */
+typedef struct cuvit_qk_norm_problem {
+    int images;
+    int tokens;
+    int heads;
+    int kv_heads;
+    int head_dim; /* even, at most 512 */
+    int32_t norm; /* cuvit_norm */
+    float epsilon; /* a positive normal float */
+    cuvit_rotation rotation;
+} cuvit_qk_norm_problem;
+
+/* kv_heads = heads, epsilon 1e-6; the rest as cuvit_rotary_problem_init. */
+void cuvit_qk_norm_problem_init(cuvit_qk_norm_problem* problem, int images, int tokens, int heads,
+                                int head_dim, int axes, const int* pairs, int pairing, int norm);
+
+/* Normalises every query and key head, scales (gamma [head_dim], null: 1),
+ * shifts (beta, null: 0) and rotates it, in one pass:
+ * out = rotation(norm(x) * gamma + beta). Value heads are copied bit for bit,
+ * or left alone in place (qkv == out), where the result is what
+ * cuvit_attention_* takes next. */
+int cuvit_qk_norm_rotary_f32(const float* qkv, const float* q_gamma, const float* q_beta,
+                             const float* k_gamma, const float* k_beta, const float* positions,
+                             const float* frequencies, float* out,
+                             const cuvit_qk_norm_problem* problem, cuvit_stream_t stream);
+int cuvit_qk_norm_rotary_bf16(const cuvit_bf16* qkv, const float* q_gamma, const float* q_beta,
+                              const float* k_gamma, const float* k_beta, const float* positions,
+                              const float* frequencies, cuvit_bf16* out,
+                              const cuvit_qk_norm_problem* problem, cuvit_stream_t stream);
+
+/* Its gradients. qkv is the forward's input, grad_out the gradient of its whole
+ * packed output; grad_qkv == grad_out (in place) is allowed, and value heads
+ * pass through as in the forward. The gradients of gamma and beta are sums over
+ * all images, tokens and heads in fp32, in an order that sizes and device fix,
+ * and overwrite their [head_dim] outputs; a null one is not computed. They need
+ * a workspace of cuvit_qk_norm_rotary_workspace() bytes, 16-byte aligned, used
+ * by one call at a time (calls that may overlap, replays of captured ones among
+ * them, take one each); with all four null it may be null. */
+int64_t cuvit_qk_norm_rotary_workspace(const cuvit_qk_norm_problem* problem);
+int cuvit_qk_norm_rotary_backward_f32(const float* qkv, const float* q_gamma, const float* k_gamma,
+                                      const float* positions, const float* frequencies,
+                                      const float* grad_out, float* grad_qkv, float* grad_q_gamma,
+                                      float* grad_q_beta, float* grad_k_gamma, float* grad_k_beta,
+                                      void* workspace, int64_t workspace_bytes,
+                                      const cuvit_qk_norm_problem* problem, cuvit_stream_t stream);
+int cuvit_qk_norm_rotary_backward_bf16(const cuvit_bf16* qkv, const float* q_gamma,
+                                       const float* k_gamma, const float* positions,
+                                       const float* frequencies, const cuvit_bf16* grad_out,
+                                       cuvit_bf16* grad_qkv, float* grad_q_gamma,
+                                       float* grad_q_beta, float* grad_k_gamma, float* grad_k_beta,
+                                       void* workspace, int64_t workspace_bytes,
+                                       const cuvit_qk_norm_problem* problem,
+                                       cuvit_stream_t stream);
+
+typedef enum cuvit_gate {
+    CUVIT_GATE_SILU = 0,     /* x / (1 + exp(-x)) */
+    CUVIT_GATE_GELU = 1,     /* the erf form, as cuvit_gelu_* */
+    CUVIT_GATE_GELU_TANH = 2 /* x / 2 (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
+} cuvit_gate;
+
+/* A gated product's sizes: A [m, k], B [2 n, k] (a Linear layer's weight: n
+ * rows of the gate, then n of the value), C [m, n]. A zero leading dimension
+ * selects the packed one. */
+typedef struct cuvit_gated_problem {
+    int m;
+    int n;
+    int k;
+    int32_t activation;     /* cuvit_gate */
+    int lda;
+    int ldb;
+    int ldc;
+    int ld_preactivations;  /* of [m, 2 n] */
+} cuvit_gated_problem;
+
+void cuvit_gated_problem_init(cuvit_gated_problem* problem, int m, int n, int k, int activation);
+
+/* C = activation(gate) * value, with [gate, value] = A.B^T + bias, bias [2 n]
+ * fp32 or null. With preactivations [m, 2 n] not null, [gate, value] is stored
+ * too, for cuvit_gated_backward_*. Rows of m up to 16 (single tokens) run
+ * another kernel than taller ones, whose sums over k are added in another
+ * order. k = 0 gives products of the bias. */
+int cuvit_gated_gemm_f32(const float* a, const float* b, const float* bias, float* c,
+                         float* preactivations, const cuvit_gated_problem* problem,
+                         cuvit_stream_t stream);
+int cuvit_gated_gemm_bf16(const cuvit_bf16* a, const cuvit_bf16* b, const float* bias,
+                          cuvit_bf16* c, cuvit_bf16* preactivations,
+                          const cuvit_gated_problem* problem, cuvit_stream_t stream);
+
+/* The gate's gradient: from preactivations [m, 2 n] and grad [m, n] (of C, its
+ * rows ldc apart) the gradient of the preactivations, rows ld_preactivations
+ * apart; grad_preactivations == preactivations is allowed. k, lda and ldb are
+ * not used. The gradients of A, B and bias are plain products and sums of it. */
+int cuvit_gated_backward_f32(const float* preactivations, const float* grad,
+                             float* grad_preactivations, const cuvit_gated_problem* problem,
+                             cuvit_stream_t stream);
+int cuvit_gated_backward_bf16(const cuvit_bf16* preactivations, const cuvit_bf16* grad,
+                              cuvit_bf16* grad_preactivations, const cuvit_gated_problem* problem,
+                              cuvit_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * bfloat16 I/O twins. An extension: the reference has no reduced-precision
  * path (README.md:472-473). Storage is bf16, every reduction and every
  * intermediate is fp32, gamma/beta/bias stay fp32, and each result is rounded

@@ -121,6 +121,68 @@ void launch_extract_patches(const std::uint16_t* images, std::uint16_t* patches,
 void launch_broadcast(std::uint16_t* destination, const std::uint16_t* source, std::int64_t count,
                       std::int64_t destination_stride, int batch, hipStream_t stream = nullptr);
 
+// Rotary, gated blocks (extensions; cuvit/capi.h says what each computes). The
+// problems are the C ABI's, filled by its init functions.
+using RotaryProblem = cuvit_rotary_problem;
+using QkNormProblem = cuvit_qk_norm_problem;
+using GatedProblem = cuvit_gated_problem;
+
+void launch_rotary(const float* input, const float* positions, const float* frequencies,
+                   float* output, const RotaryProblem& problem, hipStream_t stream = nullptr);
+void launch_rotary(const std::uint16_t* input, const float* positions, const float* frequencies,
+                   std::uint16_t* output, const RotaryProblem& problem,
+                   hipStream_t stream = nullptr);
+
+/// Scales and shifts of the query and key heads, [head_dim] each; null: 1 and 0.
+struct QkNormWeights {
+    const float* q_gamma = nullptr;
+    const float* q_beta = nullptr;
+    const float* k_gamma = nullptr;
+    const float* k_beta = nullptr;
+};
+
+void launch_qk_norm_rotary(const float* qkv, const QkNormWeights& weights, const float* positions,
+                           const float* frequencies, float* out, const QkNormProblem& problem,
+                           hipStream_t stream = nullptr);
+void launch_qk_norm_rotary(const std::uint16_t* qkv, const QkNormWeights& weights,
+                           const float* positions, const float* frequencies, std::uint16_t* out,
+                           const QkNormProblem& problem, hipStream_t stream = nullptr);
+
+/// Their gradients (null: not computed) and the workspace for them.
+struct QkNormGradients {
+    float* q_gamma = nullptr;
+    float* q_beta = nullptr;
+    float* k_gamma = nullptr;
+    float* k_beta = nullptr;
+    void* workspace = nullptr;
+    std::int64_t workspace_bytes = 0;
+};
+
+void launch_qk_norm_rotary_backward(const float* qkv, const QkNormWeights& weights,
+                                    const float* positions, const float* frequencies,
+                                    const float* grad_out, float* grad_qkv,
+                                    const QkNormGradients& gradients, const QkNormProblem& problem,
+                                    hipStream_t stream = nullptr);
+void launch_qk_norm_rotary_backward(const std::uint16_t* qkv, const QkNormWeights& weights,
+                                    const float* positions, const float* frequencies,
+                                    const std::uint16_t* grad_out, std::uint16_t* grad_qkv,
+                                    const QkNormGradients& gradients, const QkNormProblem& problem,
+                                    hipStream_t stream = nullptr);
+
+void launch_gated_gemm(const float* a, const float* b, const float* bias, float* c,
+                       float* preactivations, const GatedProblem& problem,
+                       hipStream_t stream = nullptr);
+void launch_gated_gemm(const std::uint16_t* a, const std::uint16_t* b, const float* bias,
+                       std::uint16_t* c, std::uint16_t* preactivations,
+                       const GatedProblem& problem, hipStream_t stream = nullptr);
+
+void launch_gated_backward(const float* preactivations, const float* grad,
+                           float* grad_preactivations, const GatedProblem& problem,
+                           hipStream_t stream = nullptr);
+void launch_gated_backward(const std::uint16_t* preactivations, const std::uint16_t* grad,
+                           std::uint16_t* grad_preactivations, const GatedProblem& problem,
+                           hipStream_t stream = nullptr);
+
 /// Throws the exception matching a C-ABI status (no-op on CUVIT_OK).
 void throw_on_error(int status);
 
