@@ -107,9 +107,10 @@ __device__ __forceinline__ std::uint32_t pack_bf16x2(float low, float high) {
 /// 5e-5 of normally distributed inputs land one ulp from the correctly
 /// rounded GELU. 17 instructions, two of them transcendental (rcp, exp2):
 /// the GELU of a GEMM epilogue costs about as much issue time as the MFMAs
-/// of a K = 768 product, so every instruction counts here. (gelu_cumulative is
-/// Phi alone.)
-__device__ __forceinline__ float gelu_cumulative(float x) {
+/// of a K = 768 product, so every instruction counts here. (@p Cumulative: Phi(x)
+/// alone.)
+template <bool Cumulative = false>
+__device__ __forceinline__ float gelu(float x) {
     const float w = fabsf(x) * 0.84932180028801907F;                              // sqrt(log2(e) / 2)
     const float t = __builtin_amdgcn_rcpf(fmaf(w, 0.41627730557884884F, 1.0F));  // 1 / (2 sqrt(log2 e))
     float q = -2.718776930e-01F;
@@ -121,10 +122,9 @@ __device__ __forceinline__ float gelu_cumulative(float x) {
     q = fmaf(q, t, 1.440642000e+00F);
     q = fmaf(q, t, -2.825698747e+00F);
     const float e = __builtin_amdgcn_exp2f(fmaf(-w, w, q));  // erfc(z) / 2 = t e
-    return x < 0.0F ? t * e : fmaf(-t, e, 1.0F);
+    const float phi = x < 0.0F ? t * e : fmaf(-t, e, 1.0F);
+    return Cumulative ? phi : x * phi;
 }
-
-__device__ __forceinline__ float gelu(float x) { return x * gelu_cumulative(x); }
 
 // -- 16-byte vectors ----------------------------------------------------------
 

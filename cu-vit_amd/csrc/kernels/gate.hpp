@@ -30,17 +30,17 @@ template <Gate G> __device__ __forceinline__ float gate_value(float x) {
     }
 }
 
-/// gate_value and its slope together.
-template <Gate G> __device__ __forceinline__ float gate_value(float x, float& slope) {
+/// gate_value and its slope together; @p Fine takes the erf form's Phi from erfcf,
+/// which fp32 results can tell from gelu's (4e-7 of it).
+template <Gate G, bool Fine> __device__ __forceinline__ float gate_value(float x, float& slope) {
     if constexpr (G == Gate::kSilu) {
         const float s = sigmoid(x);
         slope = s * fmaf(x, 1.0F - s, 1.0F);
         return x * s;
     } else if constexpr (G == Gate::kGelu) {
-        // Phi(x) + x phi(x), Phi from gelu's erfc: x Phi(x) is not divided by
-        // x, which may be 0.
+        // Phi(x) + x phi(x).
         const float phi = 0.3989422804014327F * __builtin_amdgcn_exp2f(x * x * -0.72134752044448170F);
-        const float cumulative = gelu_cumulative(x);
+        const float cumulative = Fine ? 0.5F * erfcf(x * -0.70710678118654752F) : gelu<true>(x);
         slope = fmaf(x, phi, cumulative);
         return x * cumulative;
     } else {

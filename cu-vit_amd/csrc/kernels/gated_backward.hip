@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kThreads) void gated_backward_kernel(const T* pre, 
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             float slope;
-            const float activation = gate_value<G>(gate[i], slope);
+            const float activation = gate_value<G, sizeof(T) == 4>(gate[i], slope);
             gate[i] = d[i] * value[i] * slope;
             value[i] = d[i] * activation;
         }
