@@ -289,8 +289,8 @@ int check_gated_layout(const cuvit_gated_problem& p, detail::GatedArgs* args) {
     if (p.activation < CUVIT_GATE_SILU || p.activation > CUVIT_GATE_GELU_TANH) {
         return fail(CUVIT_ERROR_INVALID_ARGUMENT, "Gated activation is not a cuvit_gate value");
     }
-    if (p.n > 0x3FFFFFFF) {
-        return fail(CUVIT_ERROR_LENGTH, "Gated products take at most 2^30 - 1 columns");
+    if (p.m > 0x3FFFFFFF || p.n > 0x3FFFFFFF) {
+        return fail(CUVIT_ERROR_LENGTH, "Gated products take at most 2^30 - 1 rows and columns");
     }
     args->gate = static_cast<detail::Gate>(p.activation);
     args->ldc = p.ldc != 0 ? p.ldc : p.n;

@@ -7,14 +7,20 @@
 // them where they lie, and the [m, 2 n] preactivations never leave the chip
 // unless they are asked for.
 //
-// gated_tile_kernel: any sizes, strides and alignment. Four wavefronts own 64 rows
-// x 64 outputs; operands go through registers into LDS, a stage of 128 bytes of k
-// ahead, at any value's address. MFMAs, fragments and the placement in LDS are the
-// GEMMs' (gemm_kernel.hpp, gemm_ring.hpp).
-#include "gate.hpp"
-#include "gemm_choice.hpp"
-#include "gemm_ring.hpp"
-#include "runs.hpp"
+// Three kernels: gated_rows_kernel for single tokens; gated_ring_kernel
+// (gated_ring.hpp) for operands whose rows are whole 16-byte chunks; and
+// gated_loose_kernel for any sizes, strides and alignment, where four wavefronts own 64
+// rows x 64 outputs and operands go through registers into LDS, a stage of 128
+// bytes of k ahead, at any value's address (3152 x 2048 x 767 in bf16: 61 us, x 768
+// on the ring 24.5). MFMAs, fragments and the placement in LDS are the GEMMs'
+// (gemm_kernel.hpp, gemm_ring.hpp).
+//
+// Bound: the MFMAs and what feeds them. 12608 x 2048 x 768 in bf16 takes 78 to 84 us
+// by card (1.01 to 0.94 PFLOP/s), the plain product of the same operands as one
+// library call 82; fp32 runs at the 137 TFLOP/s that the clock under its MFMAs
+// allows (6304 x 2048 x 768: 289 us).
+#include "gated_choice.hpp"
+#include "gated_ring.hpp"
 
 #include <type_traits>
 
@@ -22,51 +28,7 @@ namespace cuvit::detail {
 namespace gemm {
 namespace {
 
-/// Four consecutive values to any value's address, or the first @p count of them.
-template <typename T> __device__ __forceinline__ void store_quad(T* to, const float (&v)[4], int count) {
-    const Run<T, 4> run = round_run<T, 4>(v);
-    if (count >= 4) {
-        store_run_unaligned<T, 4>(to, run);
-    } else {
-        store_some<T, 4>(to, run, count);
-    }
-}
-
-/// A lane's four consecutive columns of one row, finished and stored.
-template <typename T, Gate G>
-__device__ __forceinline__ void finish_quad(const float (&gate_sum)[4], const float (&value_sum)[4],
-                                            const float (&gate_bias)[4], const float (&value_bias)[4], int row, int col,
-                                            T* c, T* pre, const GatedArgs& args) {
-    if (row >= args.m || col >= args.n) {
-        return;
-    }
-    const int count = args.n - col;
-    float gate[4], value[4], out[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        gate[e] = gate_sum[e] + gate_bias[e];
-        value[e] = value_sum[e] + value_bias[e];
-        out[e] = gate_value<G>(gate[e]) * value[e];
-    }
-    store_quad(c + static_cast<std::int64_t>(row) * args.ldc + col, out, count);
-    if (pre != nullptr) {
-        T* const to = pre + static_cast<std::int64_t>(row) * args.ld_pre + col;
-        store_quad(to, gate, count);
-        store_quad(to + args.n, value, count);
-    }
-}
-
-/// The bias of four columns of each half, 0 without one and past the last.
-__device__ __forceinline__ void read_bias(const float* bias, int col, int n, float (&gate)[4], float (&value)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const bool given = bias != nullptr && col + e < n;
-        gate[e] = given ? bias[col + e] : 0.0F;
-        value[e] = given ? bias[n + col + e] : 0.0F;
-    }
-}
-
-template <typename T> struct GatedTile {
+template <typename T> struct LooseTile {
     static constexpr int kE = Mma<T>::kEdge;
     static constexpr int kThreads = 256;
     static constexpr int kBM = 64;
@@ -80,10 +42,10 @@ template <typename T> struct GatedTile {
 };
 
 template <typename T, Gate G>
-__global__ __launch_bounds__(256) void gated_tile_kernel(const T* __restrict__ a, const T* __restrict__ b,
+__global__ __launch_bounds__(256) void gated_loose_kernel(const T* __restrict__ a, const T* __restrict__ b,
                                                          const float* __restrict__ bias, T* c, T* pre,
                                                          GatedArgs args) {
-    using S = GatedTile<T>;
+    using S = LooseTile<T>;
     constexpr int E = S::kE;
     __shared__ Vec16 stage[S::kRows * 8];
     const int tiles_n = (args.n + S::kBO - 1) / S::kBO;
@@ -125,13 +87,7 @@ __global__ __launch_bounds__(256) void gated_tile_kernel(const T* __restrict__ a
     };
 
     typename Mma<T>::Acc acc[S::kTM][2 * S::kTO];
-#pragma unroll
-    for (int i = 0; i < S::kTM; ++i)
-#pragma unroll
-        for (int j = 0; j < 2 * S::kTO; ++j)
-#pragma unroll
-            for (int r = 0; r < 4 * Mma<T>::kRuns; ++r)
-                acc[i][j][r] = 0.0F;
+    StartAtZero{}(acc);
     auto place = [](int row, int slot) { return row * 8 + (slot ^ ((row >> 1) & 7)); };
     if (args.k > 0) {
         load(0);
@@ -164,25 +120,110 @@ __global__ __launch_bounds__(256) void gated_tile_kernel(const T* __restrict__ a
                     Mma<T>::run(acc[i][j], fb[j], fa[i]);
         }
     }
+    const int first_col = col0 + wave_n * S::kTO * E;
 #pragma unroll
-    for (int o = 0; o < S::kTO; ++o)
+    for (int j = 0; j < 2 * S::kTO; ++j)
 #pragma unroll
-        for (int q = 0; q < Mma<T>::kRuns; ++q) {
-            const int col = col0 + (wave_n * S::kTO + o) * E + Mma<T>::column(lane, q);
-            float gate_bias[4], value_bias[4];
-            read_bias(bias, col, args.n, gate_bias, value_bias);
+        for (int q = 0; q < Mma<T>::kRuns; ++q)
 #pragma unroll
-            for (int i = 0; i < S::kTM; ++i) {
-                float gate[4], value[4];
+            for (int e = 0; e < 4; ++e) {
+                const int col = first_col + j / 2 * E + Mma<T>::column(lane, q) + e;
+                const float term = bias != nullptr && col < args.n ? bias[(j & 1) * args.n + col] : 0.0F;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    gate[e] = acc[i][2 * o][4 * q + e];
-                    value[e] = acc[i][2 * o + 1][4 * q + e];
+                for (int i = 0; i < S::kTM; ++i)
+                    acc[i][j][4 * q + e] += term;
+            }
+    finish_tiles<T, G, S::kTM, 2 * S::kTO>(acc, lane, row0 + wave_m * S::kTM * E, first_col, c, pre, args);
+}
+
+/// Sixteen MFMA rows against sixteen: bf16 by k-blocks of 32, fp32 of 16.
+template <typename T> struct RowMma;
+template <> struct RowMma<float> {
+    static constexpr int kBlock = 16;
+    __device__ __forceinline__ static void run(floatx4& acc, const Vec16& b, const Vec16& a) {
+        Mma<float>::run(acc, b, a);
+    }
+};
+template <> struct RowMma<std::uint16_t> {
+    static constexpr int kBlock = 32;
+    __device__ __forceinline__ static void run(floatx4& acc, const Vec16& b, const Vec16& a) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a),
+                                                      acc, 0, 0, 0);
+    }
+};
+
+/// Up to sixteen rows (single tokens): bound by reading B once. A workgroup takes
+/// eight outputs, their eight gate and eight value rows as one MFMA tile, so that
+/// 2048 outputs fill the chip; its wavefronts split K, two k-blocks (a cache line of
+/// each row) at a time, straight from memory into fragments, and add their parts in
+/// LDS in a fixed order. Any alignment. 1 x 2048 x 768 in bf16: 3.5 us, with the
+/// 64-row tile below 5.1.
+template <typename T, Gate G>
+__global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ a, const T* __restrict__ b,
+                                                         const float* __restrict__ bias, T* c, T* pre,
+                                                         GatedArgs args) {
+    constexpr int kWaves = 8;
+    constexpr int kV = Elem<T>::kPerVec;
+    constexpr int kPair = 2 * RowMma<T>::kBlock;
+    __shared__ float parts[kWaves][16][17];
+    const int lane = lane_id();
+    const int wave = static_cast<int>(threadIdx.x) / kWave;
+    const int out0 = static_cast<int>(blockIdx.x) * 8;
+    const int row = lane % 16;
+    // (Rows and outputs past the last repeat it: their sums are not stored.)
+    const int out = min(out0 + row % 8, args.n - 1);
+    const int chunk = lane / 16 * kV;
+    const T* const from_a = a + static_cast<std::int64_t>(min(row, args.m - 1)) * args.lda + chunk;
+    const T* const from_b = b + (static_cast<std::int64_t>(row < 8 ? 0 : args.n) + out) * args.ldb + chunk;
+    floatx4 acc{0.0F, 0.0F, 0.0F, 0.0F};
+    constexpr int kTogether = 2;
+    for (int k0 = wave * kPair; k0 < args.k; k0 += kTogether * kWaves * kPair) {
+        Run<T, kV> fa[2 * kTogether], fb[2 * kTogether];
+#pragma unroll
+        for (int p = 0; p < kTogether; ++p) {
+            const int at = k0 + p * kWaves * kPair;
+            if (at + kPair <= args.k) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    fb[2 * p + h] = load_run_unaligned<T, kV>(from_b + at + h * RowMma<T>::kBlock);
+                    fa[2 * p + h] = load_run_unaligned<T, kV>(from_a + at + h * RowMma<T>::kBlock);
                 }
-                finish_quad<T, G>(gate, value, gate_bias, value_bias, row0 + (wave_m * S::kTM + i) * E + lane % E, col,
-                                  c, pre, args);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int count = min(max(args.k - at - h * RowMma<T>::kBlock - chunk, 0), kV);
+                    fb[2 * p + h] = load_some<T, kV>(from_b + at + h * RowMma<T>::kBlock, count);
+                    fa[2 * p + h] = load_some<T, kV>(from_a + at + h * RowMma<T>::kBlock, count);
+                }
             }
         }
+#pragma unroll
+        for (int p = 0; p < 2 * kTogether; ++p)
+            RowMma<T>::run(acc, __builtin_bit_cast(Vec16, fb[p]), __builtin_bit_cast(Vec16, fa[p]));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        parts[wave][row][4 * (lane / 16) + e] = acc[e];
+    __syncthreads();
+    const int thread = static_cast<int>(threadIdx.x);
+    const int token = thread / 8;
+    const int column = thread % 8;
+    if (token >= args.m || out0 + column >= args.n) { // (m <= 16: threads past 128 too)
+        return;
+    }
+    float gate = bias != nullptr ? bias[out0 + column] : 0.0F;
+    float value = bias != nullptr ? bias[args.n + out0 + column] : 0.0F;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        gate += parts[w][token][column];
+        value += parts[w][token][8 + column];
+    }
+    Elem<T>::store(c + static_cast<std::int64_t>(token) * args.ldc + out0 + column, gate_value<G>(gate) * value);
+    if (pre != nullptr) {
+        T* const to = pre + static_cast<std::int64_t>(token) * args.ld_pre + out0 + column;
+        Elem<T>::store(to, gate);
+        Elem<T>::store(to + args.n, value);
+    }
 }
 
 /// @p run with the activation as a constant.
@@ -194,17 +235,87 @@ template <typename Run> hipError_t with_gate(Gate gate, Run&& run) {
     }
 }
 
+template <typename S, typename T>
+hipError_t launch_ring(const T* a, const T* b, const float* bias, T* c, T* pre, const GatedArgs& args,
+                       const TileMap& map, hipStream_t stream) {
+    const std::int64_t tiles_m = (static_cast<std::int64_t>(args.m) + S::kBM - 1) / S::kBM;
+    const std::int64_t tiles_n = (2 * static_cast<std::int64_t>(args.n) + S::kBN - 1) / S::kBN;
+    const std::int64_t tiles =
+        map.px > 0 ? 8 * ((tiles_m + map.px - 1) / map.px) * ((tiles_n + map.py - 1) / map.py) : tiles_m * tiles_n;
+    if (tiles > 0x7FFFFFFF) {
+        return hipErrorInvalidConfiguration;
+    }
+    return with_gate(args.gate, [&](auto gate) -> hipError_t {
+        constexpr auto kernel = gated_ring_kernel<T, S, decltype(gate)::value>;
+        if (const hipError_t opted = allow_lds<kernel>(kGatedLds<S>); opted != hipSuccess) {
+            return opted;
+        }
+        kernel<<<static_cast<unsigned int>(tiles), S::kThreads, kGatedLds<S>, stream>>>(a, b, bias, c, pre, args, map);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_tile(const float* a, const float* b, const float* bias, float* c, float* pre, const GatedArgs& args,
+                       hipStream_t stream) {
+    auto launch = [&](auto shape) {
+        return launch_ring<decltype(shape)>(a, b, bias, c, pre, args, TileMap{0, 0}, stream);
+    };
+    switch (choose_gated_f32(args, compute_units())) {
+    case GatedTileF32::k32x16Alone: return launch(RingShape<float, 2, 1, 1, 2, 3, true, true>{});
+    case GatedTileF32::k32x32: return launch(RingShape<float, 2, 2, 1, 2, 2, true>{});
+    case GatedTileF32::k32x32Alone: return launch(RingShape<float, 2, 2, 1, 2, 3, true>{});
+    default: return launch(RingShape<float, 2, 2, 2, 2, 2, true>{});
+    }
+}
+
+hipError_t launch_tile(const std::uint16_t* a, const std::uint16_t* b, const float* bias, std::uint16_t* c,
+                       std::uint16_t* pre, const GatedArgs& args, hipStream_t stream) {
+    using T = std::uint16_t;
+    const GatedChoice choice = choose_gated(args, compute_units());
+    auto launch = [&](auto shape) {
+        return launch_ring<decltype(shape)>(a, b, bias, c, pre, args, choice.map, stream);
+    };
+    switch (choice.tile) {
+    case GatedTile::k64x32Alone: return launch(RingShape<T, 2, 1, 1, 2, 4, true, true>{});
+    case GatedTile::k64x64: return launch(RingShape<T, 2, 2, 1, 2, 2>{});
+    case GatedTile::k64x64Alone: return launch(RingShape<T, 2, 2, 1, 2, 3>{});
+    case GatedTile::k128x64: return launch(RingShape<T, 4, 2, 1, 2, 2>{});
+    case GatedTile::k192x128: return launch(RingShape<T, 2, 4, 3, 2, 2>{});
+    case GatedTile::k256x128: return launch(RingShape<T, 2, 4, 4, 2, 2>{});
+    default: return launch(RingShape<T, 2, 4, 5, 2, 2>{});
+    }
+}
+
+/// Whether an operand's rows are whole 16-byte chunks that the ring's loads reach
+/// from a tile's first row.
+template <typename T> bool ring_operand(const T* base, int ld, int depth) {
+    return aligned16(base) && ld % Elem<T>::kPerVec == 0 && depth % Elem<T>::kPerVec == 0 &&
+           static_cast<std::int64_t>(320) * ld * static_cast<std::int64_t>(sizeof(T)) < kMaxSpan;
+}
+
 template <typename T>
 hipError_t launch_gated(const T* a, const T* b, const float* bias, T* c, T* pre, const GatedArgs& args,
                         hipStream_t stream) {
-    using S = GatedTile<T>;
+    if (args.m <= kGatedRows) {
+        const std::int64_t groups = (static_cast<std::int64_t>(args.n) + 7) / 8;
+        return with_gate(args.gate, [&](auto gate) -> hipError_t {
+            gated_rows_kernel<T, decltype(gate)::value>
+                <<<static_cast<unsigned int>(groups), 512, 0, stream>>>(a, b, bias, c, pre, args);
+            return hipGetLastError();
+        });
+    }
+    // (The bias is loaded from one descriptor, 32-bit offsets.)
+    if (ring_operand(a, args.lda, args.k) && ring_operand(b, args.ldb, args.k) && args.n < (1 << 27)) {
+        return launch_tile(a, b, bias, c, pre, args, stream);
+    }
+    using S = LooseTile<T>;
     const std::int64_t tiles = (static_cast<std::int64_t>(args.m) + S::kBM - 1) / S::kBM *
                                ((static_cast<std::int64_t>(args.n) + S::kBO - 1) / S::kBO);
     if (tiles > 0x7FFFFFFF) {
         return hipErrorInvalidConfiguration;
     }
     return with_gate(args.gate, [&](auto gate) -> hipError_t {
-        gated_tile_kernel<T, decltype(gate)::value>
+        gated_loose_kernel<T, decltype(gate)::value>
             <<<static_cast<unsigned int>(tiles), S::kThreads, 0, stream>>>(a, b, bias, c, pre, args);
         return hipGetLastError();
     });

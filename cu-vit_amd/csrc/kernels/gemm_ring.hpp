@@ -205,13 +205,30 @@ template <typename T, typename S> struct RingLoads {
 /// The barriers' own wait for it stays, and holds whatever the compiler moves.
 __device__ __forceinline__ void wait_fragments() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
-/// The k loop: acc += A.B^T over @p stages stages, the ring kept kSlots - 1
-/// stages ahead. On return no load is in flight and no wavefront reads the
-/// ring.
-template <typename T, typename S>
-__device__ __forceinline__ void ring_multiply(const RingLoads<T, S>& loads, const unsigned char* lds, int wave_m,
+/// The k loop: acc = A.B^T over @p stages stages of @p loads (RingLoads, or its
+/// like), the ring kept kSlots - 1 stages ahead. On return no load is in flight
+/// and no wavefront reads the ring. What acc starts from is @p start's to say,
+/// with the first stages' loads on their way: StartAtZero, or one with
+/// kAfterFirst that is called once the first stage, and all loaded before it, has
+/// landed.
+struct StartAtZero {
+    static constexpr bool kAfterFirst = false;
+    template <typename Acc, int TM, int TN> __device__ __forceinline__ void operator()(Acc (&acc)[TM][TN]) const {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int r = 0; r < static_cast<int>(sizeof(Acc) / 4); ++r)
+                    acc[i][j][r] = 0.F;
+    }
+};
+
+template <typename T, typename S, typename Loads, typename Start = StartAtZero>
+__device__ __forceinline__ void ring_multiply(const Loads& loads, const unsigned char* lds, int wave_m,
                                               int wave_n, int lane, bool loading, int stages,
-                                              typename Mma<T>::Acc (&acc)[S::kTM][S::kTN]) {
+                                              typename Mma<T>::Acc (&acc)[S::kTM][S::kTN],
+                                              const Start& start = {}) {
     constexpr int E = S::kEdge;
     constexpr int kBlocks = S::kBK / kKBlock<T>;  // k-blocks per stage
     constexpr int kPerBlock = kWave / E;          // 16-byte chunks of a row per k-block
@@ -224,13 +241,9 @@ __device__ __forceinline__ void ring_multiply(const RingLoads<T, S>& loads, cons
     for (int kb = 0; kb < kBlocks; ++kb) {
         fragment_column[kb] = static_cast<unsigned int>(S::place(lane % E, kPerBlock * kb + lane / E) * 16);
     }
-#pragma unroll
-    for (int i = 0; i < S::kTM; ++i)
-#pragma unroll
-        for (int j = 0; j < S::kTN; ++j)
-#pragma unroll
-            for (int r = 0; r < 4 * Mma<T>::kRuns; ++r)
-                acc[i][j][r] = 0.F;
+    if constexpr (!Start::kAfterFirst) {
+        start(acc);
+    }
     struct Fragments {
         Vec16 a[kBlocks][S::kTM];
         Vec16 b[kBlocks][S::kTN];
@@ -287,6 +300,9 @@ __device__ __forceinline__ void ring_multiply(const RingLoads<T, S>& loads, cons
         } else {
             asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S::kSlots - 1) * S::kLoads) : "memory");
         }
+        if constexpr (Start::kAfterFirst) {
+            start(acc);
+        }
         read(set[0], 0);
         int slot = 0;
         auto step = [&](int g, Fragments& now, Fragments& next) {
@@ -323,6 +339,10 @@ __device__ __forceinline__ void ring_multiply(const RingLoads<T, S>& loads, cons
 #pragma unroll
         for (int g = 0; g < S::kSlots - 1; ++g) {
             loads.issue(g, g);
+        }
+        if constexpr (Start::kAfterFirst) {
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S::kSlots - 2) * S::kLoads) : "memory");
+            start(acc);
         }
         int slot = 0;
         int free_slot = S::kSlots - 1;

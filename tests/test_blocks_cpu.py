@@ -152,7 +152,8 @@ MESSAGES = [
     (lambda l: call_gated(l, gated_problem(ldc=5)), 1, "A gated leading dimension is smaller than its row"),
     (lambda l: call_gated(l, gated_problem(ld_preactivations=11)), 1,
      "A gated leading dimension is smaller than its row"),
-    (lambda l: call_gated(l, gated_problem(n=2 ** 30)), 2, "Gated products take at most 2^30 - 1 columns"),
+    (lambda l: call_gated(l, gated_problem(n=2 ** 30)), 2, "Gated products take at most 2^30 - 1 rows and columns"),
+    (lambda l: call_gated(l, gated_problem(m=2 ** 30)), 2, "Gated products take at most 2^30 - 1 rows and columns"),
     (lambda l: call_gated_backward(l, None), 1, "Gated problem cannot be null"),
     (lambda l: call_gated_backward(l, gated_problem(), grad=None), 1, "Gated operands cannot be null"),
     (lambda l: call_gated_backward(l, gated_problem(), out=0x3000), 1,

@@ -43,6 +43,34 @@ def test_activations(dtype, kind, keep, bias):
     check(dtype, 33, 19, 77, kind, bias, keep)
 
 
+# One problem for each tile and more of its kind: rows and columns of tiles that
+# are cut, several to an XCD (test_gated_choice_cpu.py checks that they reach it).
+TILES = [("64x32 alone", 100, 150, 136), ("64x64 alone", 394, 2048, 768), ("64x64", 700, 1501, 264),
+         ("128x64", 1576, 2048, 768), ("192x128", 2308, 2048, 768), ("192x128", 4616, 1001, 72),
+         ("256x128", 3152, 2048, 768), ("320x128", 4616, 2048, 768), ("320x128", 9232, 1001, 72)]
+TILES_F32 = [("32x16 alone", 100, 150, 132), ("32x32 alone", 200, 1001, 132), ("32x32", 788, 1365, 100),
+             ("64x32", 3152, 2048, 260)]
+
+
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("dtype,name,m,n,k", [(torch.bfloat16, *t) for t in TILES] + [(torch.float32, *t) for t in TILES_F32])
+def test_each_tile(dtype, name, m, n, k, keep):
+    """Against 64 bits on the GPU, and twice the same bits."""
+    a, w, b = (t.to(DEV) for t in operands(dtype, m, n, k))
+    problem = cuvit.gated_problem(m, n, k, cuvit.GATE_SILU)
+    results = []
+    for _ in range(2):
+        out = torch.full((m, n), 7.0, dtype=dtype, device=DEV)
+        pre = torch.full((m, 2 * n), 7.0, dtype=dtype, device=DEV) if keep else None
+        cuvit.gated_gemm(a, w, b, out, problem, preactivations=pre)
+        results.append((out, pre))
+    expected, bound, z, error = (t.cpu() for t in support.gated(a, w, b, 0, dtype))
+    assert support.worst(results[0][0], expected, bound) <= 1.0
+    assert torch.equal(results[0][0], results[1][0])
+    if keep:
+        assert support.worst(results[0][1], z, error) <= 1.0 and torch.equal(results[0][1], results[1][1])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m", [1, 2, 7, 15, 16, 17, 31, 33, 63, 64, 65, 130, 197])
 @pytest.mark.parametrize("n,k", [(64, 192), (65, 64), (200, 100), (17, 513)])
