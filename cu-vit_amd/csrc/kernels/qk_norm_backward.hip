@@ -110,10 +110,12 @@ __global__ __launch_bounds__(kThreads) void rotate_heads_backward_kernel(const T
             widen<T, U>(step.x[r], n[r]);
             widen<T, U>(step.d[r], d[r]);
         }
-        const float scale = normalise<Norm>(n[0], n[1], place, args.log_team, args.inverse_dim, args.epsilon);
+        const float scale = normalise<Norm, Vector>(n[0], n[1], place, args.log_team, args.inverse_dim, args.epsilon);
         if (args.rotation.pairs > 0) {
-            turn_runs<U, Vector, Adjacent>(d[0], d[1], lds + 2 * step.token * table_pitch(args.rotation.pairs), place,
-                                           args.rotation.pairs);
+            Turns<U> turns;
+            read_turns<U, Vector, Adjacent>(lds + 2 * step.token * table_pitch(args.rotation.pairs), place,
+                                            args.rotation.pairs, turns);
+            turn_runs<U, Adjacent>(d[0], d[1], turns, place, args.rotation.pairs);
         }
         float along = 0.0F; // sum of g n
         float sum = 0.0F;   // sum of g
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kThreads) void rotate_heads_backward_kernel(const T
 #pragma unroll
             for (int i = 0; i < U; ++i)
                 d[r][i] = scale * (d[r][i] - fmaf(n[r][i], along, sum));
-        write_runs<T, U, Vector>(grad_in + step.at, place, d[0], d[1]);
+        write_runs<T, U, Vector, Vector>(grad_in + step.at, place, d[0], d[1]);
     };
     Step now, next;
     read(0, 0, now);

@@ -176,14 +176,15 @@ __device__ __forceinline__ void read_runs(const T* from, const Place& place, Run
     }
 }
 
-template <typename T, int U, bool Vector>
-__device__ __forceinline__ void write_runs(T* to, const Place& place, const float (&first)[U], const float (&second)[U]) {
+template <typename T, int U, bool Vector, bool Streaming>
+__device__ __forceinline__ void write_runs(T* to, const Place& place, const float (&first)[U],
+                                           const float (&second)[U]) {
     const Run<T, U> runs[2] = {round_run<T, U>(first), round_run<T, U>(second)};
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         if constexpr (Vector) {
             if (place.count[r] > 0) {
-                store_run<T, U>(to + place.at[r], runs[r]);
+                store_run<T, U, Streaming>(to + place.at[r], runs[r]);
             }
         } else {
             store_some<T, U>(to + place.at[r], runs[r], place.count[r]);
@@ -193,9 +194,12 @@ __device__ __forceinline__ void write_runs(T* to, const Place& place, const floa
 
 /// Takes a head's mean from its runs (HeadNorm::kLayer) and returns the factor
 /// that makes their root mean square 1.
-template <HeadNorm Norm, int U>
+/// (With whole runs the lanes past the head are kept out of the sums; what they
+/// hold is not stored.)
+template <HeadNorm Norm, bool Vector, int U>
 __device__ __forceinline__ float normalise(float (&first)[U], float (&second)[U], const Place& place, int log_team,
                                            float inverse_dim, float epsilon) {
+    const bool past = Vector && place.count[0] == 0;
     if constexpr (Norm == HeadNorm::kLayer) {
         // The mean, and once more of what is left, so that rows far from zero
         // keep their deviations.
@@ -205,11 +209,11 @@ __device__ __forceinline__ float normalise(float (&first)[U], float (&second)[U]
 #pragma unroll
             for (int i = 0; i < U; ++i)
                 sum += first[i] + second[i];
-            const float mean = team_sum(sum, log_team) * inverse_dim;
+            const float mean = team_sum(past ? 0.0F : sum, log_team) * inverse_dim;
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                first[i] = i < place.count[0] ? first[i] - mean : 0.0F;
-                second[i] = i < place.count[1] ? second[i] - mean : 0.0F;
+                first[i] = Vector || i < place.count[0] ? first[i] - mean : 0.0F;
+                second[i] = Vector || i < place.count[1] ? second[i] - mean : 0.0F;
             }
         }
     }
@@ -217,7 +221,7 @@ __device__ __forceinline__ float normalise(float (&first)[U], float (&second)[U]
 #pragma unroll
     for (int i = 0; i < U; ++i)
         squares = fmaf(first[i], first[i], fmaf(second[i], second[i], squares));
-    return __builtin_amdgcn_rsqf(fmaf(team_sum(squares, log_team), inverse_dim, epsilon));
+    return __builtin_amdgcn_rsqf(fmaf(team_sum(past ? 0.0F : squares, log_team), inverse_dim, epsilon));
 }
 
 /// Copies @p width values of each of @p tokens tokens, from element @p skip of
@@ -231,7 +235,7 @@ __device__ __forceinline__ void copy_tokens(const T* in, T* out, std::int64_t pi
         const int t = i / pieces;
         const std::int64_t at = (row0 + t) * pitch + skip;
         if (whole) {
-            store16(out + at + (i - t * pieces) * kPerVec, load16(in + at + (i - t * pieces) * kPerVec));
+            store16_streaming(out + at + (i - t * pieces) * kPerVec, load16(in + at + (i - t * pieces) * kPerVec));
         } else {
             out[at + i - t * pieces] = in[at + i - t * pieces];
         }
@@ -260,46 +264,68 @@ template <int N, bool Vector> __device__ __forceinline__ void read_floats(const 
     }
 }
 
-/// Turns the pairs of a lane's runs. @p row is the token's row of the table; a
-/// value that is not rotated, whatever it holds, stays as it is.
+/// The cosines and sines of a lane's pairs: with halves of the pairs of both runs
+/// (U of them), with adjacent pairs of the first run's, then the second's.
+template <int U> struct Turns {
+    float c[U];
+    float s[U];
+};
+
+/// From a token's row of the table. Reads past the pairs stay in the table, which
+/// has a run to spare, and are not used.
 template <int U, bool Vector, bool Adjacent>
-__device__ __forceinline__ void turn_runs(float (&first)[U], float (&second)[U], const float* row, const Place& place,
-                                          int pairs) {
+__device__ __forceinline__ void read_turns(const float* row, const Place& place, int pairs, Turns<U>& turns) {
     const int pitch = table_pitch(pairs);
     if constexpr (Adjacent) {
-        auto turn = [&](float(&v)[U], int pair) {
-            // Reads past the pairs stay in the row's own padding or the next
-            // row (the table has a row's width to spare) and are not used.
-            if (pair >= pairs) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (place.pair[r] < pairs) {
+                float c[U / 2], s[U / 2];
+                read_floats<U / 2, Vector>(row + place.pair[r], c);
+                read_floats<U / 2, Vector>(row + pitch + place.pair[r], s);
+#pragma unroll
+                for (int i = 0; i < U / 2; ++i) {
+                    turns.c[r * (U / 2) + i] = c[i];
+                    turns.s[r * (U / 2) + i] = s[i];
+                }
+            }
+        }
+    } else if (place.turned) {
+        read_floats<U, Vector>(row + place.pair[0], turns.c);
+        read_floats<U, Vector>(row + pitch + place.pair[0], turns.s);
+    }
+}
+
+/// Turns the pairs of a lane's runs; a value that is not rotated, whatever it
+/// holds, stays as it is.
+template <int U, bool Adjacent>
+__device__ __forceinline__ void turn_runs(float (&first)[U], float (&second)[U], const Turns<U>& turns,
+                                          const Place& place, int pairs) {
+    if constexpr (Adjacent) {
+        auto turn = [&](float(&v)[U], int r) {
+            const int left = pairs - place.pair[r];
+            if (left <= 0) {
                 return;
             }
-            float c[U / 2], s[U / 2];
-            read_floats<U / 2, Vector>(row + pair, c);
-            read_floats<U / 2, Vector>(row + pitch + pair, s);
 #pragma unroll
             for (int i = 0; i < U / 2; ++i) {
+                const float c = turns.c[r * (U / 2) + i];
+                const float s = turns.s[r * (U / 2) + i];
                 const float x = v[2 * i];
                 const float y = v[2 * i + 1];
-                const bool turned = pair + i < pairs;
-                v[2 * i] = turned ? fmaf(x, c[i], -(y * s[i])) : x;
-                v[2 * i + 1] = turned ? fmaf(y, c[i], x * s[i]) : y;
+                v[2 * i] = i < left ? fmaf(x, c, -(y * s)) : x;
+                v[2 * i + 1] = i < left ? fmaf(y, c, x * s) : y;
             }
         };
-        turn(first, place.pair[0]);
-        turn(second, place.pair[1]);
-    } else {
-        if (!place.turned) {
-            return;
-        }
-        float c[U], s[U];
-        read_floats<U, Vector>(row + place.pair[0], c);
-        read_floats<U, Vector>(row + pitch + place.pair[0], s);
+        turn(first, 0);
+        turn(second, 1);
+    } else if (place.turned) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const float x = first[i];
             const float y = second[i];
-            first[i] = fmaf(x, c[i], -(y * s[i]));
-            second[i] = fmaf(y, c[i], x * s[i]);
+            first[i] = fmaf(x, turns.c[i], -(y * turns.s[i]));
+            second[i] = fmaf(y, turns.c[i], x * turns.s[i]);
         }
     }
 }

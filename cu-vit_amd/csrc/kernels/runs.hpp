@@ -28,11 +28,15 @@ template <typename T, int U> __device__ __forceinline__ Run<T, U> load_run(const
     return run;
 }
 
-template <typename T, int U> __device__ __forceinline__ void store_run(T* to, const Run<T, U>& run) {
-    if constexpr (Run<T, U>::kWords == 4) {
-        store16(to, Vec16{{run.w[0], run.w[1], run.w[2], run.w[3]}});
+/// With Streaming non-temporal (store16_streaming says what that gives). (A choice
+/// at run time loses it: the compiler makes one plain store of both.)
+template <typename T, int U, bool Streaming> __device__ __forceinline__ void store_run(T* to, const Run<T, U>& run) {
+    typedef std::uint32_t words __attribute__((ext_vector_type(Run<T, U>::kWords)));
+    const words v = __builtin_bit_cast(words, run);
+    if constexpr (Streaming) {
+        __builtin_nontemporal_store(v, reinterpret_cast<words*>(to));
     } else {
-        *reinterpret_cast<uint2*>(to) = make_uint2(run.w[0], run.w[1]);
+        *reinterpret_cast<words*>(to) = v;
     }
 }
 
