@@ -49,10 +49,15 @@ template <typename T, int U> __device__ __forceinline__ Run<T, U> load_run_unali
     return __builtin_bit_cast(RunType, static_cast<words>(*reinterpret_cast<const loose*>(from)));
 }
 
-template <typename T, int U> __device__ __forceinline__ void store_run_unaligned(T* to, const Run<T, U>& run) {
+template <typename T, int U, bool Streaming = false>
+__device__ __forceinline__ void store_run_unaligned(T* to, const Run<T, U>& run) {
     typedef std::uint32_t words __attribute__((ext_vector_type(Run<T, U>::kWords)));
     typedef words loose __attribute__((aligned(sizeof(T))));
-    *reinterpret_cast<loose*>(to) = __builtin_bit_cast(words, run);
+    if constexpr (Streaming) {
+        __builtin_nontemporal_store(__builtin_bit_cast(words, run), reinterpret_cast<loose*>(to));
+    } else {
+        *reinterpret_cast<loose*>(to) = __builtin_bit_cast(words, run);
+    }
 }
 
 /// The first @p count values of a run, one by one; the others are 0.
