@@ -9,10 +9,9 @@
 //
 // Three kernels: gated_rows_kernel for single tokens; gated_ring_kernel
 // (gated_ring.hpp) for operands whose rows are whole 16-byte chunks; and
-// gated_loose_kernel for any sizes, strides and alignment, where four wavefronts own 64
-// rows x 64 outputs and operands go through registers into LDS, a stage of 128
-// bytes of k ahead, at any value's address (3152 x 2048 x 767 in bf16: 61 us, x 768
-// on the ring 24.5). MFMAs, fragments and the placement in LDS are the GEMMs'
+// gated_loose_kernel for any sizes, strides and alignment, where operands
+// go through registers into LDS, a stage of 128 bytes of k ahead, at any value's
+// address (3152 x 2048 x 767 in bf16: 45 us, x 768 on the ring 24.7). MFMAs, fragments and the placement in LDS are the GEMMs'
 // (gemm_kernel.hpp, gemm_ring.hpp).
 //
 // Bound: the MFMAs and what feeds them. 12608 x 2048 x 768 in bf16 takes 78 to 84 us
@@ -28,24 +27,27 @@ namespace cuvit::detail {
 namespace gemm {
 namespace {
 
-template <typename T> struct LooseTile {
+/// 32 WM rows x 64 outputs, two wavefronts for each 32 rows.
+template <typename T, int WM> struct LooseTile {
     static constexpr int kE = Mma<T>::kEdge;
-    static constexpr int kThreads = 256;
-    static constexpr int kBM = 64;
+    static constexpr int kThreads = 2 * kWave * WM;
+    static constexpr int kBM = 32 * WM;
     static constexpr int kBO = 64;           // outputs
-    static constexpr int kTM = kBM / 2 / kE; // a wavefront's MFMA tiles of rows
+    static constexpr int kTM = 32 / kE;      // a wavefront's MFMA tiles of rows
     static constexpr int kTO = kBO / 2 / kE; // and of outputs
     static constexpr int kV = Elem<T>::kPerVec;
     static constexpr int kBK = 8 * kV;
     static constexpr int kRows = kBM + 2 * kBO; // of a stage: A's, then the gate's and the value's tiles in turn
-    static constexpr int kChunks = kRows * 8 / kThreads; // 16-byte chunks a thread loads
+    static constexpr int kStep = kThreads / 8;           // stage rows between a thread's chunks
+    static constexpr int kChunks = kRows / kStep;        // 16-byte chunks a thread loads
+    static_assert(kRows % kStep == 0 && kBM % kStep == 0, "whole chunks of either operand");
 };
 
-template <typename T, Gate G>
-__global__ __launch_bounds__(256) void gated_loose_kernel(const T* __restrict__ a, const T* __restrict__ b,
-                                                         const float* __restrict__ bias, T* c, T* pre,
-                                                         GatedArgs args) {
-    using S = LooseTile<T>;
+template <typename T, int WM, Gate G>
+__global__ __launch_bounds__(128 * WM) void gated_loose_kernel(const T* __restrict__ a, const T* __restrict__ b,
+                                                               const float* __restrict__ bias, T* c, T* pre,
+                                                               GatedArgs args) {
+    using S = LooseTile<T, WM>;
     constexpr int E = S::kE;
     __shared__ Vec16 stage[S::kRows * 8];
     const int tiles_n = (args.n + S::kBO - 1) / S::kBO;
@@ -56,21 +58,28 @@ __global__ __launch_bounds__(256) void gated_loose_kernel(const T* __restrict__ 
     const int wave_m = thread / kWave / 2;
     const int wave_n = thread / kWave % 2;
 
-    // The rows this thread loads: chunk thread % 8 of stage rows thread / 8 + 32 p.
+    // The rows this thread loads: chunk thread % 8 of stage rows
+    // thread / 8 + kStep p.
     // Rows past the operands' ends repeat the last one: their sums are not stored.
     const int chunk = thread % 8;
     const T* from[S::kChunks];
+    int left[S::kChunks]; // values from there to the operand's end, as far as it counts
 #pragma unroll
     for (int p = 0; p < S::kChunks; ++p) {
-        const int row = thread / 8 + 32 * p;
-        if (32 * p < S::kBM) {
-            from[p] = a + static_cast<std::int64_t>(min(row0 + row, args.m - 1)) * args.lda;
+        const int row = thread / 8 + S::kStep * p;
+        std::int64_t behind;
+        if (S::kStep * p < S::kBM) {
+            const int at = min(row0 + row, args.m - 1);
+            from[p] = a + static_cast<std::int64_t>(at) * args.lda;
+            behind = static_cast<std::int64_t>(args.m - 1 - at) * args.lda;
         } else {
             const int tile = (row - S::kBM) / E; // even: the gate's, odd: the value's
-            const int col = min(col0 + tile / 2 * E + (row - S::kBM) % E, args.n - 1);
-            from[p] = b + (static_cast<std::int64_t>((tile & 1) != 0 ? args.n : 0) + col) * args.ldb;
+            const int at = min(col0 + tile / 2 * E + (row - S::kBM) % E, args.n - 1) + ((tile & 1) != 0 ? args.n : 0);
+            from[p] = b + static_cast<std::int64_t>(at) * args.ldb;
+            behind = static_cast<std::int64_t>(2 * args.n - 1 - at) * args.ldb;
         }
         from[p] += chunk * S::kV;
+        left[p] = args.k - chunk * S::kV + static_cast<int>(behind < S::kV ? behind : S::kV);
     }
     Run<T, S::kV> held[S::kChunks];
     auto load = [&](int k0) {
@@ -79,10 +88,17 @@ __global__ __launch_bounds__(256) void gated_loose_kernel(const T* __restrict__ 
             for (int p = 0; p < S::kChunks; ++p)
                 held[p] = load_run_unaligned<T, S::kV>(from[p] + k0);
         } else {
+            // The last, cut stage: whole runs into the next row where there is one,
+            // and zeros for what is not this row's.
             const int count = min(max(args.k - k0 - chunk * S::kV, 0), S::kV);
 #pragma unroll
-            for (int p = 0; p < S::kChunks; ++p)
-                held[p] = load_some<T, S::kV>(from[p] + k0, count);
+            for (int p = 0; p < S::kChunks; ++p) {
+                if (left[p] - k0 >= S::kV) {
+                    held[p] = keep_some<T, S::kV>(load_run_unaligned<T, S::kV>(from[p] + k0), count);
+                } else {
+                    held[p] = load_some<T, S::kV>(from[p] + k0, count);
+                }
+            }
         }
     };
 
@@ -96,7 +112,7 @@ __global__ __launch_bounds__(256) void gated_loose_kernel(const T* __restrict__ 
         __syncthreads(); // the last stage is read
 #pragma unroll
         for (int p = 0; p < S::kChunks; ++p)
-            stage[place(thread / 8 + 32 * p, chunk)] = __builtin_bit_cast(Vec16, held[p]);
+            stage[place(thread / 8 + S::kStep * p, chunk)] = __builtin_bit_cast(Vec16, held[p]);
         __syncthreads();
         if (k0 + S::kBK < args.k) {
             load(k0 + S::kBK);
@@ -326,17 +342,31 @@ hipError_t launch_gated(const T* a, const T* b, const float* bias, T* c, T* pre,
     if (ring_operand(a, args.lda, args.k) && ring_operand(b, args.ldb, args.k) && args.n < (1 << 27)) {
         return launch_tile(a, b, bias, c, pre, args, stream);
     }
-    using S = LooseTile<T>;
-    const std::int64_t tiles = (static_cast<std::int64_t>(args.m) + S::kBM - 1) / S::kBM *
-                               ((static_cast<std::int64_t>(args.n) + S::kBO - 1) / S::kBO);
-    if (tiles > 0x7FFFFFFF) {
-        return hipErrorInvalidConfiguration;
+    auto loose = [&](auto rows) -> hipError_t {
+        constexpr int kWM = decltype(rows)::value;
+        using S = LooseTile<T, kWM>;
+        const std::int64_t tiles = (static_cast<std::int64_t>(args.m) + S::kBM - 1) / S::kBM *
+                                   ((static_cast<std::int64_t>(args.n) + S::kBO - 1) / S::kBO);
+        if (tiles > 0x7FFFFFFF) {
+            return hipErrorInvalidConfiguration;
+        }
+        return with_gate(args.gate, [&](auto gate) -> hipError_t {
+            gated_loose_kernel<T, kWM, decltype(gate)::value>
+                <<<static_cast<unsigned int>(tiles), S::kThreads, 0, stream>>>(a, b, bias, c, pre, args);
+            return hipGetLastError();
+        });
+    };
+    // bf16 takes 128 rows where such tiles fill the CUs twice, since what a stage
+    // loads, at addresses that cross cache lines, is what bounds it (3152 x 2048 x 767:
+    // 52 -> 45 us); fp32, bound by its MFMAs, gains nothing (193 and 203).
+    if constexpr (sizeof(T) == 2) {
+        const std::int64_t tall =
+            (static_cast<std::int64_t>(args.m) + 127) / 128 * ((static_cast<std::int64_t>(args.n) + 63) / 64);
+        if (tall >= 2 * static_cast<std::int64_t>(compute_units())) {
+            return loose(std::integral_constant<int, 4>{});
+        }
     }
-    return with_gate(args.gate, [&](auto gate) -> hipError_t {
-        gated_loose_kernel<T, decltype(gate)::value>
-            <<<static_cast<unsigned int>(tiles), S::kThreads, 0, stream>>>(a, b, bias, c, pre, args);
-        return hipGetLastError();
-    });
+    return loose(std::integral_constant<int, 2>{});
 }
 
 } // namespace

@@ -78,6 +78,18 @@ template <typename T, int U> __device__ __forceinline__ Run<T, U> load_some(cons
     return run;
 }
 
+/// The first @p count values of a run, the others 0 whatever they hold.
+template <typename T, int U> __device__ __forceinline__ Run<T, U> keep_some(Run<T, U> run, int count) {
+    constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
+#pragma unroll
+    for (int i = 0; i < Run<T, U>::kWords; ++i) {
+        const int kept = count - kPerWord * i; // of this word
+        const std::uint32_t part = kPerWord == 2 && kept == 1 ? 0xFFFFU : 0U;
+        run.w[i] &= kept >= kPerWord ? 0xFFFFFFFFU : part;
+    }
+    return run;
+}
+
 template <typename T, int U>
 __device__ __forceinline__ void store_some(T* to, const Run<T, U>& run, int count) {
 #pragma unroll
