@@ -251,8 +251,12 @@ hipError_t launch(const T* input, const T* grad_output, T* grad_input, const Hea
     const int share = (args.rows - 1) / kMaxGroups + 1;
     args.block_tokens = share > round ? share : round;
     const int groups = (args.rows - 1) / args.block_tokens + 1;
-    // Their turns at a time: within 16 KiB.
-    const int held = a.rotation.pairs > 0 ? 2048 / table_pitch(a.rotation.pairs) : 64;
+    // Their turns at a time: within 16 KiB, and 2^20 items (the kernel divides an
+    // item by the heads in fp32, exact as far as that).
+    const int most = a.q_heads > args.heads[1] ? a.q_heads : args.heads[1];
+    const int by_table = a.rotation.pairs > 0 ? 2048 / table_pitch(a.rotation.pairs) : 64;
+    const int by_items = (1 << 20) / most;
+    const int held = by_table < by_items ? by_table : by_items;
     args.chunk_tokens = args.block_tokens < held ? args.block_tokens : held;
     for (int part = 0; part < 2; ++part) {
         args.per_head[part] = 1.0F / static_cast<float>(args.heads[part]);
