@@ -7,7 +7,7 @@
 // them where they lie, and the [m, 2 n] preactivations never leave the chip
 // unless they are asked for.
 //
-// Three kernels: gated_rows_kernel for single tokens; gated_ring_kernel
+// Three kernels: gated_rows_kernel for single tokens and a few rows; gated_ring_kernel
 // (gated_ring.hpp) for operands whose rows are whole 16-byte chunks; and
 // gated_loose_kernel for any sizes, strides and alignment, where operands
 // go through registers into LDS, a stage of 128 bytes of k ahead, at any value's
@@ -168,20 +168,23 @@ template <> struct RowMma<std::uint16_t> {
     }
 };
 
-/// Up to sixteen rows (single tokens): bound by reading B once. A workgroup takes
+/// Up to 16 TM rows (single tokens): bound by reading B once. A workgroup takes
 /// eight outputs, their eight gate and eight value rows as one MFMA tile, so that
 /// 2048 outputs fill the chip; its wavefronts split K, two k-blocks (a cache line of
 /// each row) at a time, straight from memory into fragments, and add their parts in
-/// LDS in a fixed order. Any alignment. 1 x 2048 x 768 in bf16: 3.5 us, with the
-/// 64-row tile below 5.1.
-template <typename T, Gate G>
+/// LDS in a fixed order. Any alignment. In bf16, us (the 64-row tiles below): 1 x
+/// 2048 x 768 3.5 (5.1), 32 rows of it 4.3 (5.1); 64 rows 6.0 (5.2), so those come
+/// here only where the tiles would be the loose kernel's, 64 x 1958 x 741 12.7 (13.0),
+/// in fp32 11.0 (34.9).
+template <typename T, int TM, Gate G>
 __global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ a, const T* __restrict__ b,
                                                          const float* __restrict__ bias, T* c, T* pre,
                                                          GatedArgs args) {
     constexpr int kWaves = 8;
     constexpr int kV = Elem<T>::kPerVec;
-    constexpr int kPair = 2 * RowMma<T>::kBlock;
-    __shared__ float parts[kWaves][16][17];
+    constexpr int kBlock = RowMma<T>::kBlock;
+    constexpr int kPair = 2 * kBlock;
+    __shared__ float parts[kWaves][16 * TM][17];
     const int lane = lane_id();
     const int wave = static_cast<int>(threadIdx.x) / kWave;
     const int out0 = static_cast<int>(blockIdx.x) * 8;
@@ -189,42 +192,51 @@ __global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ a
     // (Rows and outputs past the last repeat it: their sums are not stored.)
     const int out = min(out0 + row % 8, args.n - 1);
     const int chunk = lane / 16 * kV;
-    const T* const from_a = a + static_cast<std::int64_t>(min(row, args.m - 1)) * args.lda + chunk;
+    const T* from_a[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+        from_a[i] = a + static_cast<std::int64_t>(min(16 * i + row, args.m - 1)) * args.lda + chunk;
     const T* const from_b = b + (static_cast<std::int64_t>(row < 8 ? 0 : args.n) + out) * args.ldb + chunk;
-    floatx4 acc{0.0F, 0.0F, 0.0F, 0.0F};
-    constexpr int kTogether = 2;
+    floatx4 acc[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+        acc[i] = floatx4{0.0F, 0.0F, 0.0F, 0.0F};
+    constexpr int kTogether = TM == 1 ? 2 : 1;
     for (int k0 = wave * kPair; k0 < args.k; k0 += kTogether * kWaves * kPair) {
-        Run<T, kV> fa[2 * kTogether], fb[2 * kTogether];
+        Run<T, kV> fa[TM][2 * kTogether], fb[2 * kTogether];
 #pragma unroll
         for (int p = 0; p < kTogether; ++p) {
             const int at = k0 + p * kWaves * kPair;
-            if (at + kPair <= args.k) {
+            const bool whole = at + kPair <= args.k;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    fb[2 * p + h] = load_run_unaligned<T, kV>(from_b + at + h * RowMma<T>::kBlock);
-                    fa[2 * p + h] = load_run_unaligned<T, kV>(from_a + at + h * RowMma<T>::kBlock);
-                }
-            } else {
+            for (int h = 0; h < 2; ++h) {
+                const int k = at + h * kBlock;
+                const int count = min(max(args.k - k - chunk, 0), kV);
+                auto load = [&](const T* from) {
+                    return whole ? load_run_unaligned<T, kV>(from + k) : load_some<T, kV>(from + k, count);
+                };
+                fb[2 * p + h] = load(from_b);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int count = min(max(args.k - at - h * RowMma<T>::kBlock - chunk, 0), kV);
-                    fb[2 * p + h] = load_some<T, kV>(from_b + at + h * RowMma<T>::kBlock, count);
-                    fa[2 * p + h] = load_some<T, kV>(from_a + at + h * RowMma<T>::kBlock, count);
-                }
+                for (int i = 0; i < TM; ++i)
+                    fa[i][2 * p + h] = load(from_a[i]);
             }
         }
 #pragma unroll
         for (int p = 0; p < 2 * kTogether; ++p)
-            RowMma<T>::run(acc, __builtin_bit_cast(Vec16, fb[p]), __builtin_bit_cast(Vec16, fa[p]));
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                RowMma<T>::run(acc[i], __builtin_bit_cast(Vec16, fb[p]), __builtin_bit_cast(Vec16, fa[i][p]));
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        parts[wave][row][4 * (lane / 16) + e] = acc[e];
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            parts[wave][16 * i + row][4 * (lane / 16) + e] = acc[i][e];
     __syncthreads();
     const int thread = static_cast<int>(threadIdx.x);
-    const int token = thread / 8;
+    const int token = thread / 8; // up to 64 of them
     const int column = thread % 8;
-    if (token >= args.m || out0 + column >= args.n) { // (m <= 16: threads past 128 too)
+    if (token >= args.m || out0 + column >= args.n) {
         return;
     }
     float gate = bias != nullptr ? bias[out0 + column] : 0.0F;
@@ -330,16 +342,26 @@ template <typename T> bool ring_operand(const T* base, int ld, int depth) {
 template <typename T>
 hipError_t launch_gated(const T* a, const T* b, const float* bias, T* c, T* pre, const GatedArgs& args,
                         hipStream_t stream) {
-    if (args.m <= kGatedRows) {
+    auto rows = [&](auto tiles) -> hipError_t {
         const std::int64_t groups = (static_cast<std::int64_t>(args.n) + 7) / 8;
         return with_gate(args.gate, [&](auto gate) -> hipError_t {
-            gated_rows_kernel<T, decltype(gate)::value>
+            gated_rows_kernel<T, decltype(tiles)::value, decltype(gate)::value>
                 <<<static_cast<unsigned int>(groups), 512, 0, stream>>>(a, b, bias, c, pre, args);
             return hipGetLastError();
         });
+    };
+    const bool whole_chunks = ring_operand(a, args.lda, args.k) && ring_operand(b, args.ldb, args.k);
+    if (args.m <= kGatedRows / 4) {
+        return rows(std::integral_constant<int, 1>{});
+    }
+    if (args.m <= kGatedRows / 2) {
+        return rows(std::integral_constant<int, 2>{});
+    }
+    if (args.m <= kGatedRows && !whole_chunks) {
+        return rows(std::integral_constant<int, 4>{});
     }
     // (The bias is loaded from one descriptor, 32-bit offsets.)
-    if (ring_operand(a, args.lda, args.k) && ring_operand(b, args.ldb, args.k) && args.n < (1 << 27)) {
+    if (whole_chunks && args.n < (1 << 27)) {
         return launch_tile(a, b, bias, c, pre, args, stream);
     }
     auto loose = [&](auto rows) -> hipError_t {

@@ -9,8 +9,9 @@ namespace cuvit::detail {
 enum class GatedTile { k64x32Alone, k64x64, k64x64Alone, k128x64, k192x128, k256x128, k320x128 };
 enum class GatedTileF32 { k32x16Alone, k32x32, k32x32Alone, k64x32 };
 
-/// Rows up to which a product is one of single tokens (the row kernel).
-constexpr int kGatedRows = 16;
+/// Rows that the kernel for few rows takes at most, four MFMA tiles of 16 (half as
+/// many of operands that the ring takes too).
+constexpr int kGatedRows = 64;
 
 /// The product with 2 n columns whose tile grid the gated one's is.
 inline GemmArgs gated_grid(const GatedArgs& args) {

@@ -246,14 +246,13 @@ hipError_t launch(const T* input, const T* grad_output, T* grad_input, const Hea
     args.rotation = a.rotation;
     const int teams = kThreads >> args.log_team;
     // Workgroups of a part: kMaxGroups of them, or fewer with one full round each.
-    const int fewest = a.q_heads < args.heads[1] ? a.q_heads : args.heads[1];
-    const int round = teams / fewest > 0 ? teams / fewest : 1;
+    const int most = a.q_heads > args.heads[1] ? a.q_heads : args.heads[1];
+    const int round = teams / most > 0 ? teams / most : 1;
     const int share = (args.rows - 1) / kMaxGroups + 1;
     args.block_tokens = share > round ? share : round;
     const int groups = (args.rows - 1) / args.block_tokens + 1;
     // Their turns at a time: within 16 KiB, and 2^20 items (the kernel divides an
     // item by the heads in fp32, exact as far as that).
-    const int most = a.q_heads > args.heads[1] ? a.q_heads : args.heads[1];
     const int by_table = a.rotation.pairs > 0 ? 2048 / table_pitch(a.rotation.pairs) : 64;
     const int by_items = (1 << 20) / most;
     const int held = by_table < by_items ? by_table : by_items;
@@ -310,7 +309,8 @@ hipError_t pick(const T* input, const T* grad_output, T* grad_input, const HeadG
     if (whole(4)) {
         return launch<T, 4, true>(input, grad_output, grad_input, gradients, a, stream);
     }
-    return launch<T, 8, false>(input, grad_output, grad_input, gradients, a, stream);
+    return loose_runs_of_four(a) ? launch<T, 4, false>(input, grad_output, grad_input, gradients, a, stream)
+                                 : launch<T, 8, false>(input, grad_output, grad_input, gradients, a, stream);
 }
 
 } // namespace

@@ -230,7 +230,8 @@ template <typename T> hipError_t pick(const T* input, T* output, const HeadArgs&
             return launch<T, 4, true>(input, output, a, stream);
         }
     }
-    return launch<T, 8, false>(input, output, a, stream);
+    return loose_runs_of_four(a) ? launch<T, 4, false>(input, output, a, stream)
+                                 : launch<T, 8, false>(input, output, a, stream);
 }
 
 } // namespace

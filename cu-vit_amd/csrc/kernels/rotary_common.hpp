@@ -8,8 +8,9 @@
 //              values the unrotated rest is split in halves the same way
 //   adjacent   pairs (2 i, 2 i + 1): any runs of whole pairs; with whole runs
 //              (Vector) the halves of the head, else 2 U values in a row
-// With Vector a run is one 16- or 8-byte access; without, the values are moved
-// one by one, for any sizes and alignment.
+// With Vector every run is one 16- or 8-byte access at a multiple of its size;
+// without, whole runs are one at any value's address and the values of a cut one
+// are moved one by one (any sizes and alignment).
 #pragma once
 
 #include "launch.hpp"
@@ -171,7 +172,11 @@ __device__ __forceinline__ void read_runs(const T* from, const Place& place, Run
                 runs[r] = load_run<T, U>(from + place.at[r]);
             }
         } else {
-            runs[r] = load_some<T, U>(from + place.at[r], place.count[r]);
+            if (place.count[r] == U) {
+                runs[r] = load_run_unaligned<T, U>(from + place.at[r]);
+            } else {
+                runs[r] = load_some<T, U>(from + place.at[r], place.count[r]);
+            }
         }
     }
 }
@@ -187,7 +192,11 @@ __device__ __forceinline__ void write_runs(T* to, const Place& place, const floa
                 store_run<T, U, Streaming>(to + place.at[r], runs[r]);
             }
         } else {
-            store_some<T, U>(to + place.at[r], runs[r], place.count[r]);
+            if (place.count[r] == U) {
+                store_run_unaligned<T, U>(to + place.at[r], runs[r]);
+            } else {
+                store_some<T, U>(to + place.at[r], runs[r], place.count[r]);
+            }
         }
     }
 }
@@ -342,6 +351,12 @@ inline bool whole_runs(int unit, std::size_t element, std::uintptr_t addresses, 
                        int pairs, bool adjacent) {
     const bool runs = head_dim % (2 * unit) == 0 && (adjacent || pairs % unit == 0);
     return runs && addresses % (unit * element) == 0 && strides % unit == 0;
+}
+
+/// The runs of a kernel without Vector: of four, or of eight where those of four
+/// would take more lanes than a wavefront has.
+inline bool loose_runs_of_four(const HeadArgs& a) {
+    return lanes_of_head(4, a.rotation.adjacent, a.head_dim, a.rotation.pairs) <= kWave;
 }
 
 /// The least l with 2^l >= @p lanes.

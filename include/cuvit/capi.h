@@ -298,8 +298,8 @@ void cuvit_gated_problem_init(cuvit_gated_problem* problem, int m, int n, int k,
 
 /* C = activation(gate) * value, with [gate, value] = A.B^T + bias, bias [2 n]
  * fp32 or null. With preactivations [m, 2 n] not null, [gate, value] is stored
- * too, for cuvit_gated_backward_*. Rows of m up to 16 (single tokens) run
- * another kernel than taller ones, whose sums over k are added in another
+ * too, for cuvit_gated_backward_*. Up to 64 rows (single tokens among them) run
+ * other kernels than taller products, which add the sums over k in another
  * order. k = 0 gives products of the bias. More than 2^30 - 1 rows or columns are
  * CUVIT_ERROR_LENGTH. */
 int cuvit_gated_gemm_f32(const float* a, const float* b, const float* bias, float* c,
