@@ -304,7 +304,8 @@ hipError_t launch_ring(const T* a, const T* b, const float* bias, T* c, T* pre, 
 hipError_t launch_tile(const float* a, const float* b, const float* bias, float* c, float* pre, const GatedArgs& args,
                        hipStream_t stream) {
     auto launch = [&](auto shape) {
-        return launch_ring<decltype(shape)>(a, b, bias, c, pre, args, TileMap{0, 0}, stream);
+        using S = decltype(shape);
+        return launch_ring<S>(a, b, bias, c, pre, args, gated_map_f32(args, S::kBM, S::kBN, compute_units()), stream);
     };
     switch (choose_gated_f32(args, compute_units())) {
     case GatedTileF32::k32x16Alone: return launch(RingShape<float, 2, 1, 1, 2, 3, true, true>{});

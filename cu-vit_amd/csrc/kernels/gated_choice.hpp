@@ -100,4 +100,15 @@ inline GatedTileF32 choose_gated_f32(const GatedArgs& args, int units) {
     return large_cost < static_cast<double>(small) ? GatedTileF32::k64x32 : GatedTileF32::k32x32;
 }
 
+/// The fp32 XCD split: none where the columns of tiles are a multiple of the XCDs,
+/// since tiles in row-major order then give each XCD columns of its own (6304 x 2048
+/// x 768: 293 us so, 305 in blocks); else balanced_map's blocks, without which every
+/// XCD reads all of B (2308 x 1365 x 512: 147 MB fetched, 65 -> 59 us).
+inline gemm::TileMap gated_map_f32(const GatedArgs& args, int bm, int bn, int units) {
+    const GemmArgs grid = gated_grid(args);
+    int rounds = 0;
+    return (grid.n + bn - 1) / bn % kXcds == 0 ? gemm::TileMap{0, 0}
+                                               : balanced_map(grid, bm, bn, units >= kXcds ? units / kXcds : 1, &rounds);
+}
+
 } // namespace cuvit::detail
