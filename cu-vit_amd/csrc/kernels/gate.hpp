@@ -45,7 +45,8 @@ template <Gate G, bool Fine> __device__ __forceinline__ float gate_value(float x
         return x * cumulative;
     } else {
         const float s = sigmoid(gelu_tanh_argument(x));
-        const float argument_slope = fmaf(x * x, 0.21406444881780075F, 1.5957691216057308F);
+        // (Held finite: s (1 - s) is 0 long before, and 0 times infinity would be NaN.)
+        const float argument_slope = fmaf(fminf(x * x, 1.0e30F), 0.21406444881780075F, 1.5957691216057308F);
         slope = fmaf(x * s * (1.0F - s), argument_slope, s);
         return x * s;
     }

@@ -228,6 +228,20 @@ def test_gradient_rows_apart_and_far_gates(dtype):
         assert bool((out[:, 2 * n:] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_gradient_of_gates_whose_squares_overflow(dtype, kind):
+    """Slopes of 0 and 1, activations of 0 and the gate: exact, as d and value are 1."""
+    gate = torch.tensor([1e15, 1.8e19, 1e20, 3e38], dtype=dtype)
+    gate = torch.cat([-gate, gate, gate.new_zeros(3)])  # 11: a whole run and a cut one
+    z = torch.cat([gate, torch.ones_like(gate)]).to(DEV)
+    out = torch.full_like(z, 7.0)
+    cuvit.gated_backward(z, torch.ones_like(gate).to(DEV), out, cuvit.gated_problem(1, 11, 1, kind))
+    slopes = torch.tensor([0.0] * 4 + [1.0] * 4 + [0.5] * 3, dtype=dtype)
+    assert torch.equal(out[:11].cpu(), slopes)
+    assert torch.equal(out[11:].cpu(), gate.clamp(min=0))
+
+
 def test_refused_tensors():
     a, w, b = (t.to(DEV) for t in operands(torch.float32, 4, 6, 8))
     out = torch.full((4, 6), 7.0, device=DEV)
