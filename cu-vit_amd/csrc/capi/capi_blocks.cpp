@@ -325,7 +325,11 @@ int gated_gemm(const T* a, const T* b, const float* bias, T* c, T* preactivation
     if (args.lda < p.k || args.ldb < p.k) {
         return fail(CUVIT_ERROR_INVALID_ARGUMENT, "A gated leading dimension is smaller than its row");
     }
-    return from_hip(detail::gated_gemm(a, b, bias, c, preactivations, args, as_hip(stream)), "gated_gemm launch");
+    const hipError_t launched = detail::gated_gemm(a, b, bias, c, preactivations, args, as_hip(stream));
+    if (launched == hipErrorInvalidConfiguration) {
+        return fail(CUVIT_ERROR_LENGTH, "Gated products take less than 2^32 threads");
+    }
+    return from_hip(launched, "gated_gemm launch");
 }
 
 template <typename T>

@@ -278,7 +278,7 @@ hipError_t launch_ring(const T* a, const T* b, const float* bias, T* c, T* pre, 
     const std::int64_t tiles_n = (2 * static_cast<std::int64_t>(args.n) + S::kBN - 1) / S::kBN;
     const std::int64_t tiles =
         map.px > 0 ? 8 * ((tiles_m + map.px - 1) / map.px) * ((tiles_n + map.py - 1) / map.py) : tiles_m * tiles_n;
-    if (tiles > 0x7FFFFFFF) {
+    if (!launchable(tiles, S::kThreads)) {
         return hipErrorInvalidConfiguration;
     }
     auto run = [&](auto chosen) -> hipError_t {
@@ -345,6 +345,9 @@ hipError_t launch_gated(const T* a, const T* b, const float* bias, T* c, T* pre,
                         hipStream_t stream) {
     auto rows = [&](auto tiles) -> hipError_t {
         const std::int64_t groups = (static_cast<std::int64_t>(args.n) + 7) / 8;
+        if (!launchable(groups, 512)) {
+            return hipErrorInvalidConfiguration;
+        }
         return with_gate(args.gate, [&](auto gate) -> hipError_t {
             gated_rows_kernel<T, decltype(tiles)::value, decltype(gate)::value>
                 <<<static_cast<unsigned int>(groups), 512, 0, stream>>>(a, b, bias, c, pre, args);
@@ -370,7 +373,7 @@ hipError_t launch_gated(const T* a, const T* b, const float* bias, T* c, T* pre,
         using S = LooseTile<T, kWM>;
         const std::int64_t tiles = (static_cast<std::int64_t>(args.m) + S::kBM - 1) / S::kBM *
                                    ((static_cast<std::int64_t>(args.n) + S::kBO - 1) / S::kBO);
-        if (tiles > 0x7FFFFFFF) {
+        if (!launchable(tiles, S::kThreads)) {
             return hipErrorInvalidConfiguration;
         }
         return with_gate(args.gate, [&](auto gate) -> hipError_t {

@@ -227,7 +227,11 @@ hipError_t rotate_heads_backward(const std::uint16_t* input, const std::uint16_t
                                  std::uint16_t* grad_input, const HeadGradients& gradients, const HeadArgs& args,
                                  hipStream_t stream);
 
-// gated.hip. Leading dimensions are resolved.
+/// Whether a launch's threads can be counted in 32 bits, as HIP does.
+inline bool launchable(std::int64_t blocks, int threads) { return blocks <= 0xFFFFFFFF / threads; }
+
+// gated.hip. Leading dimensions are resolved. hipErrorInvalidConfiguration for a
+// grid that is not launchable.
 enum class Gate { kSilu, kGelu, kGeluTanh };
 struct GatedArgs {
     int m;

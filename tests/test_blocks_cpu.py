@@ -154,6 +154,8 @@ MESSAGES = [
      "A gated leading dimension is smaller than its row"),
     (lambda l: call_gated(l, gated_problem(n=2 ** 30)), 2, "Gated products take at most 2^30 - 1 rows and columns"),
     (lambda l: call_gated(l, gated_problem(m=2 ** 30)), 2, "Gated products take at most 2^30 - 1 rows and columns"),
+    (lambda l: call_gated(l, gated_problem(m=1, n=2 ** 29, k=7)), 2, "Gated products take less than 2^32 threads"),
+    (lambda l: call_gated(l, gated_problem(m=50, n=2 ** 27, k=7)), 2, "Gated products take less than 2^32 threads"),
     (lambda l: call_gated_backward(l, None), 1, "Gated problem cannot be null"),
     (lambda l: call_gated_backward(l, gated_problem(), grad=None), 1, "Gated operands cannot be null"),
     (lambda l: call_gated_backward(l, gated_problem(), out=0x3000), 1,
