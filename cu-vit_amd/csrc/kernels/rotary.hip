@@ -5,8 +5,8 @@
 // instructions with a norm, 3 without.
 //
 // Results go out non-temporally (64 x 197 tokens of 24 heads of 64 in bf16, with
-// their values copied: 26.0 -> 23.5 us, a copy of the same bytes 23.2; 4 x 3136 of
-// 12, rotated, 9.5 -> 8.2, a copy 6.7), but in place, where the lines are in the
+// their values copied: 26.0 -> 20.8 us, a plain copy of the same bytes 23.3; 4 x 3136
+// of 12, rotated, 9.5 -> 8.3, a copy 6.8), but in place, where the lines are in the
 // caches and what reads them comes next.
 //
 // A workgroup takes whole tokens with all their heads, as many as its teams have
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kThreads) void rotate_heads_kernel(const T* in, T* 
             if (item < items) {
                 const T* const from =
                     in + token_offset(args.input, args.flat_input, row0 + token[k], args.tokens) + head[k] * args.input.head;
-read_runs<T, U, Vector>(from, place, raw[k]);
+                read_runs<T, U, Vector>(from, place, raw[k]);
             }
         }
     };
@@ -174,11 +174,14 @@ hipError_t launch(const T* input, T* output, const HeadArgs& a, hipStream_t stre
                           a.input.token % kPerVec == 0 && aligned16(input) && aligned16(output);
     }
     // Tokens for two rounds of a workgroup's teams, fewer while the chip has
-    // workgroups to spare.
+    // workgroups to spare, and no more than 2^23 workgroups, whose threads HIP
+    // counts in 32 bits.
     const int teams = kThreads >> args.log_team;
     const int full = 2 * teams / a.heads > 0 ? 2 * teams / a.heads : 1;
     const int spread = args.rows / (4 * compute_units()) + 1;
+    const int least = (args.rows >> 23) + 1;
     args.block_tokens = full < spread ? full : spread;
+    args.block_tokens = args.block_tokens > least ? args.block_tokens : least;
     const std::size_t lds =
         4 * (table_floats(args.block_tokens, rotation.pairs) +
              (a.norm != HeadNorm::kNone ? static_cast<std::size_t>(4) * ((a.head_dim + 3) / 4 * 4) + 8 : 0));

@@ -217,3 +217,18 @@ def test_offsets_past_32_bits():
     expected = compare(x, at, [16, 16], False)
     for i in range(2):
         assert torch.equal(far[i * (2 ** 31 + 64):][:x[i].numel()].reshape(x[i].shape), expected[i])
+
+
+def test_more_tokens_than_workgroups():
+    """2^24 tokens of more heads than a workgroup has teams for (40 GB in place):
+    each head as if it were the only one."""
+    tokens, heads = 2 ** 24 + 5, 600
+    at = (torch.arange(tokens, device=DEV) % 10007).float()[:, None]
+    turns = ladder([1]).to(DEV)
+    alone = torch.ones(1, tokens, 1, 2, dtype=torch.bfloat16, device=DEV)
+    cuvit.rotary(alone, at, turns, alone, cuvit.rotary_problem(1, tokens, 1, 2, [1]))
+    x = torch.ones(1, tokens, heads, 2, dtype=torch.bfloat16, device=DEV)
+    cuvit.rotary(x, at, turns, x, cuvit.rotary_problem(1, tokens, heads, 2, [1]))
+    for first in range(0, tokens, 2 ** 20):
+        part = slice(first, min(first + 2 ** 20, tokens))
+        assert bool((x[:, part] == alone[:, part]).all()), first
