@@ -9,9 +9,10 @@
 //
 // Three kernels: gated_rows_kernel for single tokens and a few rows; gated_ring_kernel
 // (gated_ring.hpp) for operands whose rows are whole 16-byte chunks; and
-// gated_loose_kernel for any sizes, strides and alignment, where operands
-// go through registers into LDS, a stage of 128 bytes of k ahead, at any value's
-// address (3152 x 2048 x 767 in bf16: 45 us, x 768 on the ring 24.7). MFMAs, fragments and the placement in LDS are the GEMMs'
+// gated_loose_kernel for any sizes, strides and alignment, where operands go through
+// registers into LDS, a stage of 128 bytes of k ahead (two ahead: 788 x 2048 x 767 in
+// bf16 18.4 -> 20.6 us), at any value's address (3152 x 2048 x 767: 45 us, x 768 on the
+// ring 24.7). MFMAs, fragments and the placement in LDS are the GEMMs'
 // (gemm_kernel.hpp, gemm_ring.hpp).
 //
 // Bound: the MFMAs and what feeds them. 12608 x 2048 x 768 in bf16 takes 78 to 84 us
@@ -27,14 +28,14 @@ namespace cuvit::detail {
 namespace gemm {
 namespace {
 
-/// 32 WM rows x 64 outputs, two wavefronts for each 32 rows.
-template <typename T, int WM> struct LooseTile {
+/// WM x 2 wavefronts of TM x TO MFMA tiles of outputs.
+template <typename T, int WM, int TM, int TO> struct LooseTile {
     static constexpr int kE = Mma<T>::kEdge;
     static constexpr int kThreads = 2 * kWave * WM;
-    static constexpr int kBM = 32 * WM;
-    static constexpr int kBO = 64;           // outputs
-    static constexpr int kTM = 32 / kE;      // a wavefront's MFMA tiles of rows
-    static constexpr int kTO = kBO / 2 / kE; // and of outputs
+    static constexpr int kBM = kE * TM * WM;
+    static constexpr int kBO = 2 * kE * TO;  // outputs
+    static constexpr int kTM = TM;           // a wavefront's MFMA tiles of rows
+    static constexpr int kTO = TO;           // and of outputs
     static constexpr int kV = Elem<T>::kPerVec;
     static constexpr int kBK = 8 * kV;
     static constexpr int kRows = kBM + 2 * kBO; // of a stage: A's, then the gate's and the value's tiles in turn
@@ -43,11 +44,10 @@ template <typename T, int WM> struct LooseTile {
     static_assert(kRows % kStep == 0 && kBM % kStep == 0, "whole chunks of either operand");
 };
 
-template <typename T, int WM, Gate G>
-__global__ __launch_bounds__(128 * WM) void gated_loose_kernel(const T* __restrict__ a, const T* __restrict__ b,
-                                                               const float* __restrict__ bias, T* c, T* pre,
-                                                               GatedArgs args) {
-    using S = LooseTile<T, WM>;
+template <typename T, typename S, Gate G>
+__global__ __launch_bounds__(S::kThreads) void gated_loose_kernel(const T* __restrict__ a, const T* __restrict__ b,
+                                                                  const float* __restrict__ bias, T* c, T* pre,
+                                                                  GatedArgs args) {
     constexpr int E = S::kE;
     __shared__ Vec16 stage[S::kRows * 8];
     const int tiles_n = (args.n + S::kBO - 1) / S::kBO;
@@ -175,7 +175,7 @@ template <> struct RowMma<std::uint16_t> {
 /// LDS in a fixed order. Any alignment. In bf16, us (the 64-row tiles below): 1 x
 /// 2048 x 768 3.5 (5.1), 32 rows of it 4.3 (5.1); 64 rows 6.0 (5.2), so those come
 /// here only where the tiles would be the loose kernel's, 64 x 1958 x 741 12.7 (13.0),
-/// in fp32 11.0 (34.9).
+/// in fp32 11.0 (65 rows in tiles 15.9).
 template <typename T, int TM, Gate G>
 __global__ __launch_bounds__(512) void gated_rows_kernel(const T* __restrict__ a, const T* __restrict__ b,
                                                          const float* __restrict__ bias, T* c, T* pre,
@@ -368,31 +368,35 @@ hipError_t launch_gated(const T* a, const T* b, const float* bias, T* c, T* pre,
     if (whole_chunks && args.n < (1 << 27)) {
         return launch_tile(a, b, bias, c, pre, args, stream);
     }
-    auto loose = [&](auto rows) -> hipError_t {
-        constexpr int kWM = decltype(rows)::value;
-        using S = LooseTile<T, kWM>;
+    auto loose = [&](auto tile) -> hipError_t {
+        using S = decltype(tile);
         const std::int64_t tiles = (static_cast<std::int64_t>(args.m) + S::kBM - 1) / S::kBM *
                                    ((static_cast<std::int64_t>(args.n) + S::kBO - 1) / S::kBO);
         if (!launchable(tiles, S::kThreads)) {
             return hipErrorInvalidConfiguration;
         }
         return with_gate(args.gate, [&](auto gate) -> hipError_t {
-            gated_loose_kernel<T, kWM, decltype(gate)::value>
+            gated_loose_kernel<T, S, decltype(gate)::value>
                 <<<static_cast<unsigned int>(tiles), S::kThreads, 0, stream>>>(a, b, bias, c, pre, args);
             return hipGetLastError();
         });
     };
-    // bf16 takes 128 rows where such tiles fill the CUs twice, since what a stage
-    // loads, at addresses that cross cache lines, is what bounds it (3152 x 2048 x 767:
-    // 52 -> 45 us); fp32, bound by its MFMAs, gains nothing (193 and 203).
+    auto tiles = [&](int rows) {
+        return (static_cast<std::int64_t>(args.m) + rows - 1) / rows * ((static_cast<std::int64_t>(args.n) + 63) / 64);
+    };
+    const std::int64_t units = compute_units();
     if constexpr (sizeof(T) == 2) {
-        const std::int64_t tall =
-            (static_cast<std::int64_t>(args.m) + 127) / 128 * ((static_cast<std::int64_t>(args.n) + 63) / 64);
-        if (tall >= 2 * static_cast<std::int64_t>(compute_units())) {
-            return loose(std::integral_constant<int, 4>{});
-        }
+        // 64 x 64 outputs; 128 x 64 where such tiles fill the CUs twice, since what a
+        // stage loads, at addresses that cross cache lines, is what bounds it (3152 x
+        // 2048 x 767: 52 -> 45 us), and for the same reason no smaller ones (of 32 x 64:
+        // 788 x 2048 x 767 18.2 and 24.7).
+        return tiles(128) >= 2 * units ? loose(LooseTile<T, 4, 1, 1>{}) : loose(LooseTile<T, 2, 1, 1>{});
+    } else {
+        // fp32 is bound by the MFMAs of the CUs that have a tile: 32 x 32 outputs, 64 x 64
+        // from four of these a CU on (64 x 64 against 32 x 32, in us: 100 x 2048 x 767 34.6
+        // and 14.9; 788 x 1365 x 513 45.7 and 32.9; 3152 x 1365 x 513 104 and 108).
+        return tiles(64) >= 4 * units ? loose(LooseTile<T, 2, 2, 2>{}) : loose(LooseTile<T, 2, 1, 1>{});
     }
-    return loose(std::integral_constant<int, 2>{});
 }
 
 } // namespace

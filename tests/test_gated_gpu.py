@@ -106,6 +106,26 @@ def test_layers(dtype, m, n, k):
     assert support.worst(out, expected, bound) <= 1.0 and support.worst(pre, z, error) <= 1.0
 
 
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(65, 31, 33), (100, 1365, 513), (394, 683, 257), (788, 1365, 77), (3152, 1365, 131),
+                                   (2100, 2048, 63)])
+def test_tiles_of_loose_rows(dtype, m, n, k, keep):
+    """Rows that are no whole 16-byte chunks, from a few tiles to several a CU:
+    against 64 bits on the GPU, and twice the same bits."""
+    a, w, b = (t.to(DEV) for t in operands(dtype, m, n, k))
+    results = []
+    for _ in range(2):
+        out = torch.full((m, n), 7.0, dtype=dtype, device=DEV)
+        pre = torch.full((m, 2 * n), 7.0, dtype=dtype, device=DEV) if keep else None
+        cuvit.gated_gemm(a, w, b, out, cuvit.gated_problem(m, n, k), preactivations=pre)
+        results.append((out, pre))
+    expected, bound, z, error = (t.cpu() for t in support.gated(a, w, b, 0, dtype))
+    assert support.worst(results[0][0], expected, bound) <= 1.0 and torch.equal(results[0][0], results[1][0])
+    if keep:
+        assert support.worst(results[0][1], z, error) <= 1.0 and torch.equal(results[0][1], results[1][1])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m", [1, 9, 16, 17, 100])
 @pytest.mark.parametrize("n,k,extra", [(72, 64, 8), (72, 64, 1), (33, 50, 3), (128, 128, 4)])
