@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void rotate_heads_backward_kernel(const T
             Turns<U> turns;
             read_turns<U, Vector, Adjacent>(lds + 2 * step.token * table_pitch(args.rotation.pairs), place,
                                             args.rotation.pairs, turns);
-            turn_runs<U, Adjacent>(d[0], d[1], turns, place, args.rotation.pairs);
+            turn_runs<U, Vector, Adjacent>(d[0], d[1], turns, place, args.rotation.pairs);
         }
         float along = 0.0F; // sum of g n
         float sum = 0.0F;   // sum of g

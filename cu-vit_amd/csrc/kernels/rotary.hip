@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kThreads) void rotate_heads_kernel(const T* in, T* 
                 Turns<U> turns;
                 read_turns<U, Vector, Adjacent>(table + 2 * token[k] * table_pitch(args.rotation.pairs), place,
                                                 args.rotation.pairs, turns);
-                turn_runs<U, Adjacent>(first, second, turns, place, args.rotation.pairs);
+                turn_runs<U, Vector, Adjacent>(first, second, turns, place, args.rotation.pairs);
             }
             T* const to = out + token_offset(args.output, args.flat_output, row0 + token[k], args.tokens) +
                           head[k] * args.output.head;

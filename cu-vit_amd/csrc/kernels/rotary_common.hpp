@@ -280,8 +280,9 @@ template <int U> struct Turns {
     float s[U];
 };
 
-/// From a token's row of the table. Reads past the pairs stay in the table, which
-/// has a run to spare, and are not used.
+/// From a token's row of the table. A cut run reads past the pairs, within the
+/// table, which has a run to spare: what lies there is another row's or was never
+/// written, and turn_runs keeps it out.
 template <int U, bool Vector, bool Adjacent>
 __device__ __forceinline__ void read_turns(const float* row, const Place& place, int pairs, Turns<U>& turns) {
     const int pitch = table_pitch(pairs);
@@ -306,8 +307,9 @@ __device__ __forceinline__ void read_turns(const float* row, const Place& place,
 }
 
 /// Turns the pairs of a lane's runs; a value that is not rotated, whatever it
-/// holds, stays as it is.
-template <int U, bool Adjacent>
+/// holds, stays as it is, and so do the zeros behind a cut run, whose turns are
+/// whatever the table holds there (0 times infinity would be NaN in a head's sums).
+template <int U, bool Vector, bool Adjacent>
 __device__ __forceinline__ void turn_runs(float (&first)[U], float (&second)[U], const Turns<U>& turns,
                                           const Place& place, int pairs) {
     if constexpr (Adjacent) {
@@ -333,8 +335,9 @@ __device__ __forceinline__ void turn_runs(float (&first)[U], float (&second)[U],
         for (int i = 0; i < U; ++i) {
             const float x = first[i];
             const float y = second[i];
-            first[i] = fmaf(x, turns.c[i], -(y * turns.s[i]));
-            second[i] = fmaf(y, turns.c[i], x * turns.s[i]);
+            const bool there = Vector || i < place.count[0];
+            first[i] = there ? fmaf(x, turns.c[i], -(y * turns.s[i])) : x;
+            second[i] = there ? fmaf(y, turns.c[i], x * turns.s[i]) : y;
         }
     }
 }
