@@ -185,7 +185,7 @@ hipError_t launch(const T* input, T* output, const HeadArgs& a, hipStream_t stre
     const std::size_t lds =
         4 * (table_floats(args.block_tokens, rotation.pairs) +
              (a.norm != HeadNorm::kNone ? static_cast<std::size_t>(4) * ((a.head_dim + 3) / 4 * 4) + 8 : 0));
-    const dim3 grid(static_cast<unsigned int>((args.rows + args.block_tokens - 1) / args.block_tokens),
+    const dim3 grid(static_cast<unsigned int>((args.rows - 1) / args.block_tokens + 1), // (rows reach 2^31 - 1)
                     args.copied > 0 ? 2U : 1U);
     auto run = [&](auto kernel) -> hipError_t {
         if (const hipError_t opted = allow_lds<decltype(kernel)::kValue>(lds); opted != hipSuccess) {
