@@ -13,6 +13,7 @@
 // it touches nothing and returns -1, and the Python code, which names what is
 // wrong, takes the call from the start. Nothing is kept between calls.
 #include "cuvit/capi.h"
+#include "reach.hpp"
 
 #include <ATen/core/Tensor.h>
 #include <c10/hip/HIPStream.h>
@@ -22,9 +23,11 @@
 #include <climits>
 #include <cstddef>
 #include <cstdint>
-#include <initializer_list>
 
 namespace {
+
+using cuvit::binding::heads_reach;
+using cuvit::binding::product;
 
 constexpr long kNotPlain = -1;
 
@@ -86,19 +89,6 @@ bool positive(PyObject* object, int* out) {
         return false;
     }
     *out = static_cast<int>(value);
-    return true;
-}
-
-/// The product of positive numbers, or false past 2^62.
-bool product(std::int64_t* out, std::initializer_list<std::int64_t> factors) {
-    std::int64_t total = 1;
-    for (const std::int64_t f : factors) {
-        if (f > (std::int64_t{1} << 62) / total) {
-            return false;
-        }
-        total *= f;
-    }
-    *out = total;
     return true;
 }
 
@@ -489,28 +479,6 @@ const std::uint16_t* bits(const void* p) { return static_cast<const std::uint16_
 std::uint16_t* bits(void* p) { return static_cast<std::uint16_t*>(p); }
 const float* singles(const void* p) { return static_cast<const float*>(p); }
 float* singles(void* p) { return static_cast<float*>(p); }
-
-/// The elements that heads placed by strides reach.
-bool heads_reach(const cuvit_rotary_problem& p, const cuvit_head_strides& s, std::int64_t* out) {
-    constexpr std::int64_t kLimit = std::int64_t{1} << 40;
-    std::int64_t image, token;
-    if (!product(&image, {p.tokens, p.heads, p.head_dim}) || !product(&token, {p.heads, p.head_dim})) {
-        return false;
-    }
-    image = s.image != 0 ? s.image : image;
-    token = s.token != 0 ? s.token : token;
-    const std::int64_t head = s.head != 0 ? s.head : p.head_dim;
-    if (image < 0 || token < 0 || head < 0) {
-        return false;
-    }
-    std::int64_t spans[3];
-    if (!product(&spans[0], {p.images, image + 1}) || !product(&spans[1], {p.tokens, token + 1}) ||
-        !product(&spans[2], {p.heads, head + 1}) || spans[0] > kLimit || spans[1] > kLimit || spans[2] > kLimit) {
-        return false;
-    }
-    *out = (p.images - 1) * image + (p.tokens - 1) * token + (p.heads - 1) * head + p.head_dim;
-    return true;
-}
 
 // (x, positions, frequencies, out, problem, stream, bf16)
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t count) {

@@ -1,5 +1,5 @@
 """Rotations and norms of 2^31 - 2 tokens, one less than a call may have: every
-image as if it were the only one."""
+image as if it were the only one; and strides that no tensor holds."""
 
 from __future__ import annotations
 
@@ -61,3 +61,17 @@ def test_qk_norm_and_its_gradients():
     alone = torch.empty_like(qkv, device=DEV)
     cuvit.qk_norm_rotary(qkv.to(DEV), *there, alone, single)
     assert images_are(x, alone)
+
+
+def test_strides_that_no_tensor_holds_are_refused():
+    x = torch.full((2, 5, 3, 64), 7.0, device=DEV)
+    out = torch.full_like(x, 7.0)
+    at, turns = torch.zeros(5, 1, device=DEV), torch.zeros(32, device=DEV)
+    for name in ("image", "token", "head"):
+        for stride in (2 ** 40, 2 ** 62, 2 ** 63 - 1):
+            problem = cuvit.rotary_problem(2, 5, 3, 64, [32])
+            setattr(problem.input, name, stride)
+            assert cuvit._native_calls.rotary(x, at, turns, out, problem, None, None) == -1
+            with pytest.raises(cuvit.InvalidArgument, match="x holds 1920 elements"):
+                cuvit.rotary(x, at, turns, out, problem)
+    assert bool((out == 7.0).all())
