@@ -15,6 +15,8 @@ namespace {
 constexpr int kMaxHeads = 65535;
 constexpr int kMaxHeadDim = 512;
 constexpr std::int64_t kMaxTokens = 0x7FFFFFFF;
+/// A gated product's k: its kernels step past the end by up to 1024 values, in int.
+constexpr int kMaxDepth = 0x7FFFFFFF - 4095;
 
 hipStream_t as_hip(cuvit_stream_t stream) { return reinterpret_cast<hipStream_t>(stream); }
 
@@ -318,6 +320,9 @@ int gated_gemm(const T* a, const T* b, const float* bias, T* c, T* preactivation
     }
     if (const int s = check_gated_layout(p, &args); s != CUVIT_OK) {
         return s;
+    }
+    if (p.k > kMaxDepth) {
+        return fail(CUVIT_ERROR_LENGTH, "Gated products take a k of at most 2^31 - 4096");
     }
     args.k = p.k;
     args.lda = p.lda != 0 ? p.lda : p.k;

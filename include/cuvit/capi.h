@@ -300,9 +300,9 @@ void cuvit_gated_problem_init(cuvit_gated_problem* problem, int m, int n, int k,
  * fp32 or null. With preactivations [m, 2 n] not null, [gate, value] is stored
  * too, for cuvit_gated_backward_*. Up to 64 rows (single tokens among them) run
  * other kernels than taller products, which add the sums over k in another
- * order. k = 0 gives products of the bias. More than 2^30 - 1 rows or columns are
- * CUVIT_ERROR_LENGTH, and so is a grid of 2^32 threads or more (2^26 columns of up
- * to 64 rows, 2^34 outputs or more of others). */
+ * order. k = 0 gives products of the bias. More than 2^30 - 1 rows or columns or a k
+ * above 2^31 - 4096 are CUVIT_ERROR_LENGTH, and so is a grid of 2^32 threads or more
+ * (2^26 columns of up to 64 rows, 2^34 outputs or more of others). */
 int cuvit_gated_gemm_f32(const float* a, const float* b, const float* bias, float* c,
                          float* preactivations, const cuvit_gated_problem* problem,
                          cuvit_stream_t stream);
