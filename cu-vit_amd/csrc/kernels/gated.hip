@@ -15,8 +15,8 @@
 // ring 24.7). MFMAs, fragments and the placement in LDS are the GEMMs'
 // (gemm_kernel.hpp, gemm_ring.hpp).
 //
-// Bound: the MFMAs and what feeds them. 12608 x 2048 x 768 in bf16 takes 78 to 84 us
-// by card (1.01 to 0.94 PFLOP/s), the plain product of the same operands as one
+// Bound: the MFMAs and what feeds them. 12608 x 2048 x 768 in bf16 takes 77 to 84 us
+// by card (1.03 to 0.94 PFLOP/s), the plain product of the same operands as one
 // library call 82; fp32 runs at the 137 TFLOP/s that the clock under its MFMAs
 // allows (6304 x 2048 x 768: 289 us).
 #include "gated_choice.hpp"
