@@ -28,6 +28,7 @@ namespace {
 
 using cuvit::binding::heads_reach;
 using cuvit::binding::product;
+using cuvit::binding::rows_reach;
 
 constexpr long kNotPlain = -1;
 
@@ -56,10 +57,16 @@ struct Library {
     decltype(&cuvit_gated_gemm_bf16) gated_gemm_bf16;
     decltype(&cuvit_gated_backward_f32) gated_backward_f32;
     decltype(&cuvit_gated_backward_bf16) gated_backward_bf16;
+    decltype(&cuvit_packed_attention_f32) packed_attention_f32;
+    decltype(&cuvit_packed_attention_bf16) packed_attention_bf16;
+    decltype(&cuvit_packed_attention_workspace) packed_attention_workspace;
+    decltype(&cuvit_packed_attention_backward_f32) packed_attention_backward_f32;
+    decltype(&cuvit_packed_attention_backward_bf16) packed_attention_backward_bf16;
+    decltype(&cuvit_packed_attention_backward_workspace) packed_attention_backward_workspace;
 };
 Library library{};
 /// The problem structs' ctypes types.
-enum Problem { kGemm, kPreprocessing, kRotary, kQkNorm, kGated, kProblems };
+enum Problem { kGemm, kPreprocessing, kRotary, kQkNorm, kGated, kPackedAttention, kProblems };
 PyObject* problem_types[kProblems] = {};
 
 /// A plain torch tensor's fields, or false.
@@ -447,6 +454,9 @@ class Operands {
     float* floats(PyObject* object, std::int64_t elements) {
         return static_cast<float*>(maybe(object, at::kFloat, elements));
     }
+    std::int32_t* numbers(PyObject* object, std::int64_t elements) {
+        return static_cast<std::int32_t*>(maybe(object, at::kInt, elements));
+    }
     bool plain() const { return plain_; }
     cuvit_stream_t stream() const { return stream_; }
 
@@ -672,8 +682,140 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
     });
 }
 
-// (GemmProblem, Preprocessing, RotaryProblem, QkNormProblem, GatedProblem, address of each of Library's functions in
-//  order)
+/// What the operands of packed attention reach, in the problem's strides; false for
+/// a problem without tokens, keys or heads, or whose strides no tensor holds.
+struct PackedReach {
+    std::int64_t q, k, v, out;
+    bool of(const cuvit_packed_attention_problem* p) {
+        return p != nullptr && p->sequences > 0 && p->sequences < INT_MAX &&
+               rows_reach(p->tokens, p->heads, p->head_dim, p->q, &q) &&
+               rows_reach(p->kv_tokens, p->kv_heads, p->head_dim, p->k, &k) &&
+               rows_reach(p->kv_tokens, p->kv_heads, p->head_dim, p->v, &v) &&
+               rows_reach(p->tokens, p->heads, p->head_dim, p->out, &out);
+    }
+};
+
+/// q, k and v, or a projection that holds all three where @p k and @p v are None and
+/// the problem's strides are a projection's.
+struct PackedOperands {
+    char* q = nullptr;
+    char* k = nullptr;
+    char* v = nullptr;
+    bool of(Operands& operands, PyObject* q_object, PyObject* k_object, PyObject* v_object, at::ScalarType type,
+            const PackedReach& reach, const cuvit_packed_attention_problem& p) {
+        if (k_object != Py_None || v_object != Py_None) {
+            q = static_cast<char*>(operands.get(q_object, type, reach.q));
+            k = static_cast<char*>(operands.get(k_object, type, reach.k));
+            v = static_cast<char*>(operands.get(v_object, type, reach.v));
+            return operands.plain();
+        }
+        const std::int64_t size = type == at::kFloat ? 4 : 2;
+        const std::int64_t to_k = static_cast<std::int64_t>(p.heads) * p.head_dim;
+        const std::int64_t to_v = to_k + static_cast<std::int64_t>(p.kv_heads) * p.head_dim;
+        const std::int64_t slots = to_v + static_cast<std::int64_t>(p.kv_heads) * p.head_dim;
+        for (const cuvit_token_strides* s : {&p.q, &p.k, &p.v}) {
+            if (s->token < slots || (s->head != 0 && s->head != p.head_dim)) {
+                return false;
+            }
+        }
+        std::int64_t whole = reach.q;
+        whole = to_k + reach.k > whole ? to_k + reach.k : whole;
+        whole = to_v + reach.v > whole ? to_v + reach.v : whole;
+        q = p.kv_tokens == p.tokens ? static_cast<char*>(operands.get(q_object, type, whole)) : nullptr;
+        if (q == nullptr || !operands.plain()) {
+            return false;
+        }
+        k = q + to_k * size;
+        v = q + to_v * size;
+        return true;
+    }
+};
+
+// (q, k, v, starts, out, problem, kv_starts, kv_lengths, lse, workspace, stream, bf16)
+PyObject* packed_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 12 || !storage(a[11], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[5], problem_types[kPackedAttention], sizeof(cuvit_packed_attention_problem));
+        const auto* const p = static_cast<const cuvit_packed_attention_problem*>(view.get());
+        PackedReach reach;
+        if (!reach.of(p)) {
+            return kNotPlain;
+        }
+        Operands operands(a[10]);
+        PackedOperands x;
+        if (!x.of(operands, a[0], a[1], a[2], type, reach, *p)) {
+            return kNotPlain;
+        }
+        const std::int64_t sequences = p->sequences;
+        const std::int64_t bytes = library.packed_attention_workspace(p);
+        const std::int32_t* const starts = operands.numbers(a[3], sequences + 1);
+        void* const out = operands.get(a[4], type, reach.out);
+        const std::int32_t* const kv_starts = operands.numbers(a[6], sequences + 1);
+        const std::int32_t* const kv_lengths = operands.numbers(a[7], sequences);
+        float* const lse = operands.floats(a[8], static_cast<std::int64_t>(p->tokens) * p->heads);
+        void* const workspace = operands.maybe(a[9], at::kByte, bytes);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat
+                       ? library.packed_attention_f32(singles(x.q), singles(x.k), singles(x.v), starts, kv_starts,
+                                                      kv_lengths, singles(out), lse, workspace, bytes, p,
+                                                      operands.stream())
+                       : library.packed_attention_bf16(bits(x.q), bits(x.k), bits(x.v), starts, kv_starts, kv_lengths,
+                                                       bits(out), lse, workspace, bytes, p, operands.stream());
+        });
+    });
+}
+
+// (q, k, v, starts, out, lse, grad_out, grad_q, grad_k, grad_v, problem, kv_starts, kv_lengths, workspace, stream, bf16)
+PyObject* packed_attention_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 16 || !storage(a[15], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[10], problem_types[kPackedAttention], sizeof(cuvit_packed_attention_problem));
+        const auto* const p = static_cast<const cuvit_packed_attention_problem*>(view.get());
+        PackedReach reach;
+        if (!reach.of(p) || (a[1] == Py_None && a[2] == Py_None) != (a[8] == Py_None && a[9] == Py_None)) {
+            return kNotPlain;
+        }
+        Operands operands(a[14]);
+        PackedOperands x, to;
+        if (!x.of(operands, a[0], a[1], a[2], type, reach, *p) || !to.of(operands, a[7], a[8], a[9], type, reach, *p)) {
+            return kNotPlain;
+        }
+        const std::int64_t sequences = p->sequences;
+        const std::int64_t bytes = library.packed_attention_backward_workspace(p);
+        const std::int32_t* const starts = operands.numbers(a[3], sequences + 1);
+        const void* const out = operands.get(a[4], type, reach.out);
+        const float* const lse = operands.floats(a[5], static_cast<std::int64_t>(p->tokens) * p->heads);
+        const void* const grad = operands.get(a[6], type, reach.out);
+        const std::int32_t* const kv_starts = operands.numbers(a[11], sequences + 1);
+        const std::int32_t* const kv_lengths = operands.numbers(a[12], sequences);
+        void* const workspace = operands.maybe(a[13], at::kByte, bytes);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat
+                       ? library.packed_attention_backward_f32(
+                             singles(x.q), singles(x.k), singles(x.v), starts, kv_starts, kv_lengths, singles(out), lse,
+                             singles(grad), singles(to.q), singles(to.k), singles(to.v), workspace, bytes, p,
+                             operands.stream())
+                       : library.packed_attention_backward_bf16(
+                             bits(x.q), bits(x.k), bits(x.v), starts, kv_starts, kv_lengths, bits(out), lse, bits(grad),
+                             bits(to.q), bits(to.k), bits(to.v), workspace, bytes, p, operands.stream());
+        });
+    });
+}
+
+// (GemmProblem, Preprocessing, RotaryProblem, QkNormProblem, GatedProblem, PackedAttentionProblem, address of each of
+//  Library's functions in order)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     constexpr Py_ssize_t kFunctions = sizeof(Library) / sizeof(void*);
     if (count != kProblems + kFunctions) {
@@ -704,7 +846,8 @@ PyMethodDef methods[] = {CUVIT_FAST(bind),           CUVIT_FAST(layer_norm), CUV
                          CUVIT_FAST(extract_patches), CUVIT_FAST(gemm),       CUVIT_FAST(attention),
                          CUVIT_FAST(preprocess),     CUVIT_FAST(vit_forward), CUVIT_FAST(rotary),
                          CUVIT_FAST(qk_norm_rotary), CUVIT_FAST(qk_norm_rotary_backward), CUVIT_FAST(gated_gemm),
-                         CUVIT_FAST(gated_backward), {nullptr, nullptr, 0, nullptr}};
+                         CUVIT_FAST(gated_backward), CUVIT_FAST(packed_attention),
+                         CUVIT_FAST(packed_attention_backward), {nullptr, nullptr, 0, nullptr}};
 #undef CUVIT_FAST
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "The launchers' plain case.", -1, methods,

@@ -47,4 +47,24 @@ inline bool heads_reach(const cuvit_rotary_problem& p, const cuvit_head_strides&
     return true;
 }
 
+/// The elements that the rows of packed attention reach, @p heads heads of @p tokens
+/// tokens, or false for strides that no tensor holds.
+inline bool rows_reach(std::int64_t tokens, std::int64_t heads, std::int64_t head_dim, const cuvit_token_strides& s,
+                       std::int64_t* out) {
+    constexpr std::int64_t kLimit = std::int64_t{1} << 40;
+    std::int64_t token;
+    if (tokens <= 0 || heads <= 0 || head_dim <= 0 || !product(&token, {heads, head_dim})) {
+        return false;
+    }
+    token = s.token != 0 ? s.token : token;
+    const std::int64_t head = s.head != 0 ? s.head : head_dim;
+    std::int64_t span;
+    if (token < 0 || token > kLimit || head < 0 || head > kLimit || !product(&span, {tokens, token + 1}) ||
+        span > kLimit || !product(&span, {heads, head + 1}) || span > kLimit) {
+        return false;
+    }
+    *out = (tokens - 1) * token + (heads - 1) * head + head_dim;
+    return true;
+}
+
 } // namespace cuvit::binding

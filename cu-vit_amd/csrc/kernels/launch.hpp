@@ -252,6 +252,56 @@ hipError_t gated_backward(const float* preactivations, const float* grad, float*
 hipError_t gated_backward(const std::uint16_t* preactivations, const std::uint16_t* grad,
                           std::uint16_t* grad_preactivations, const GatedArgs& args, hipStream_t stream);
 
+// packed_attention.hip and packed_backward.hip. Strides are resolved and checked:
+// whole 16-byte pieces, a token's at least a head's values.
+struct TokenStrides {
+    std::int64_t token;
+    std::int64_t head;
+};
+struct PackedArgs {
+    int sequences;
+    int tokens;
+    int kv_tokens;
+    int heads;
+    int kv_heads;
+    int group; // query heads to a key head
+    int head_dim;
+    float scale;
+    bool causal;
+    TokenStrides q;
+    TokenStrides k;
+    TokenStrides v;
+    TokenStrides out;
+    const std::int32_t* starts;     // [sequences + 1]
+    const std::int32_t* kv_starts;  // the same of keys
+    const std::int32_t* kv_lengths; // [sequences], or null
+};
+hipError_t packed_attention(const float* q, const float* k, const float* v, float* out, float* lse, void* workspace,
+                            const PackedArgs& args, hipStream_t stream);
+hipError_t packed_attention(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v, std::uint16_t* out,
+                            float* lse, void* workspace, const PackedArgs& args, hipStream_t stream);
+/// Bytes of its workspace (0: none is needed).
+std::int64_t packed_attention_workspace(const PackedArgs& args);
+
+/// What a gradient's call takes beside the forward's operands; the gradients'
+/// strides are their operands'.
+template <typename T> struct PackedGradients {
+    const T* out;
+    const float* lse;
+    const T* grad_out;
+    T* grad_q;
+    T* grad_k;
+    T* grad_v;
+    void* workspace;
+};
+hipError_t packed_attention_backward(const float* q, const float* k, const float* v,
+                                     const PackedGradients<float>& gradients, const PackedArgs& args,
+                                     hipStream_t stream);
+hipError_t packed_attention_backward(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v,
+                                     const PackedGradients<std::uint16_t>& gradients, const PackedArgs& args,
+                                     hipStream_t stream);
+std::int64_t packed_attention_backward_workspace(const PackedArgs& args);
+
 // Device facts used to shape grids, cached per device.
 int compute_units();
 

@@ -1,0 +1,349 @@
+// The gradients of attention over packed sequences. With p = exp(scale q.k - lse) the
+// weights, anew from the kept log-sum-exp, d the result's gradient and
+// delta = sum(d out) = sum(p (d.v)) of a row:
+//   ds = p (d.v - delta),  grad_q = scale ds.k,  grad_k = scale ds^T.q,  grad_v = p^T.d.
+//
+// Two launches. The first takes tiles of rows, as the forward does, and walks the keys:
+// delta, kept for the second, and grad_q. The second takes tiles of keys and walks the
+// rows that see them, one query head of the group after another: grad_k and grad_v. So
+// every gradient is summed in registers by one wavefront, in an order that sizes alone
+// fix, at the cost of computing logits and d.v twice (7 products for 5); sums across
+// workgroups would need atomics, whose order changes results, or fp32 copies of grad_q.
+#include "packed.hpp"
+
+namespace cuvit::detail {
+namespace packed {
+namespace {
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void query_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                                  const T* __restrict__ v,
+                                                                  PackedGradients<T> gradients, PackedArgs args,
+                                                                  int slots) {
+    using R = Rows<T, D>;
+    using Acc = typename Mma<T>::Acc;
+    constexpr int E = R::kE;
+    constexpr int K = kBlockRows<T, D>;
+    constexpr int kTile = E * kWaves;
+    using Loads = Stage<T, D, K>;
+    extern __shared__ Vec16 lds_vectors[];
+    unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
+    const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
+    if (item.head < 0) {
+        return; // the whole workgroup, before any barrier (so below)
+    }
+    const Spot spot = find(args.starts, args.sequences, args.tokens, args.group, kTile, item.slot);
+    if (spot.sequence < 0) {
+        return;
+    }
+    const Span span = span_of(args, spot.sequence);
+    const int rows = span.queries * args.group;
+    const int first_row = spot.tile * kTile;
+    if (first_row >= rows) {
+        return;
+    }
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    const int row = first_row + wave * E + lane % E;
+    const bool there = row < rows;
+    const int query = row / args.group;
+    const int head = item.head * args.group + row % args.group;
+    const int behind = span.keys - span.queries;
+    const auto sees = [&](int r) {
+        return args.causal ? min(max(min(r, rows - 1) / args.group + 1 + behind, 0), span.keys) : span.keys;
+    };
+    const int seen = there ? sees(row) : 0;
+    const int wave_least = __builtin_amdgcn_readfirstlane(sees(first_row + wave * E));
+    const int wave_most = first_row + wave * E < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + wave * E + E - 1)) : 0;
+    const int most = __builtin_amdgcn_readfirstlane(sees(first_row + kTile - 1));
+
+    const Loads k_loads(k + span.first_key * args.k.token + item.head * args.k.head, args.k.token, args.head_dim, wave,
+                        lane);
+    const Loads v_loads(v + span.first_key * args.v.token + item.head * args.v.head, args.v.token, args.head_dim, wave,
+                        lane);
+    auto issue = [&](int first, int buffer) {
+        const unsigned int to = lds_base + static_cast<unsigned int>(buffer * 2 * Loads::kBytes);
+        k_loads.issue(first, span.keys - first, to, wave);
+        v_loads.issue(first, span.keys - first, to + Loads::kBytes, wave);
+    };
+    if (most > 0) {
+        issue(0, 0);
+    }
+    const std::int64_t token = static_cast<std::int64_t>(span.first_query) + query;
+    const std::int64_t place = token * args.out.token + head * args.out.head;
+    Vec16 qf[R::kBlocks], df[R::kBlocks];
+    load_rows<T, D>(there ? q + token * args.q.token + head * args.q.head : nullptr, args.head_dim, lane, qf);
+    load_rows<T, D>(there ? gradients.grad_out + place : nullptr, args.head_dim, lane, df);
+    float delta = 0.F;
+    {
+        Vec16 of[R::kBlocks];
+        load_rows<T, D>(there ? gradients.out + place : nullptr, args.head_dim, lane, of);
+#pragma unroll
+        for (int b = 0; b < R::kBlocks; ++b) {
+#pragma unroll
+            for (int e = 0; e < R::kV; ++e) {
+                delta = fmaf(Elem<T>::get(df[b], e), Elem<T>::get(of[b], e), delta);
+            }
+        }
+    }
+    delta = combine_column<T>(delta, Sum{});
+    float shift = 0.F;
+    if (there) {
+        shift = -gradients.lse[token * args.heads + head] * kLog2e;
+        if (lane < E) {
+            static_cast<float*>(gradients.workspace)[token * args.heads + head] = delta;
+        }
+    }
+    const float c = args.scale * kLog2e;
+    Acc acc[R::kTiles];
+#pragma unroll
+    for (int t = 0; t < R::kTiles; ++t) {
+        acc[t] = Acc{};
+    }
+    int buffer = 0;
+    for (int first = 0; first < most; first += K) {
+        landed(); // and every wavefront is done with the other buffer
+        if (first + K < most) {
+            issue(first + K, buffer ^ 1);
+        }
+        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes;
+        const unsigned char* const values = keys + Loads::kBytes;
+        buffer ^= 1;
+        if (first >= wave_most) {
+            continue;
+        }
+#pragma unroll
+        for (int t = 0; t < K / E; ++t) {
+            Acc x{}, y{};
+#pragma unroll
+            for (int b = 0; b < R::kBlocks; ++b) {
+                Mma<T>::run(x, R::along(keys, t * E + lane % E, b, lane), qf[b]);
+                Mma<T>::run(y, R::along(values, t * E + lane % E, b, lane), df[b]);
+            }
+#pragma unroll
+            for (int i = 0; i < kRegisters<T>; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, shift)) * (y[i] - delta);
+            }
+            if (first + K > wave_least) {
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    x[i] = first + t * E + row_of<T>(lane, i) < seen ? x[i] : 0.F;
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < kParts<T>; ++p) {
+                const Vec16 weights = weights_of<T>(x, p);
+#pragma unroll
+                for (int d = 0; d < R::kTiles; ++d) {
+                    Mma<T>::run(acc[d], R::across(keys, t * E + 16 * p, d, lane), weights);
+                }
+            }
+        }
+    }
+    if (there) {
+        store_row<T, D>(gradients.grad_q + token * args.q.token + head * args.q.head, acc, args.scale, args.head_dim,
+                        lane);
+    }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void key_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                                const T* __restrict__ v, PackedGradients<T> gradients,
+                                                                PackedArgs args, int slots) {
+    using R = Rows<T, D>;
+    using Acc = typename Mma<T>::Acc;
+    constexpr int E = R::kE;
+    constexpr int Q = kBlockRows<T, D>; // queries of a block
+    constexpr int kTile = E * kWaves;
+    using Loads = Stage<T, D, Q>;
+    extern __shared__ Vec16 lds_vectors[];
+    unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
+    // Behind the tiles: the block's log-sum-exps (times -log2 e) and deltas, two buffers.
+    float* const numbers = reinterpret_cast<float*>(lds + 4 * Loads::kBytes);
+    const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
+    if (item.head < 0) {
+        return; // the whole workgroup, before any barrier (so below)
+    }
+    const Spot spot = find(args.kv_starts, args.sequences, args.kv_tokens, 1, kTile, item.slot);
+    if (spot.sequence < 0) {
+        return;
+    }
+    const Span span = span_of(args, spot.sequence);
+    const int first_key = spot.tile * kTile;
+    if (first_key >= span.keys) {
+        return;
+    }
+    const int lane = lane_id();
+    const int thread = static_cast<int>(threadIdx.x);
+    const int wave = __builtin_amdgcn_readfirstlane(thread / kWave);
+    const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    const int key = first_key + wave * E + lane % E;
+    const bool there = key < span.keys;
+    // Query i sees key j from i = j - (keys - queries) on.
+    const int behind = span.keys - span.queries;
+    const int from = args.causal ? max(key - behind, 0) : 0; // the first query that sees the lane's key
+    const int wave_most = __builtin_amdgcn_readfirstlane(args.causal ? max(first_key + wave * E + E - 1 - behind, 0) : 0);
+    const int wave_least = __builtin_amdgcn_readfirstlane(args.causal ? max(first_key + wave * E - behind, 0) : 0);
+    const int start = __builtin_amdgcn_readfirstlane(args.causal ? max(first_key - behind, 0) / Q * Q : 0);
+
+    const std::int64_t token = static_cast<std::int64_t>(span.first_key) + key;
+    Vec16 kf[R::kBlocks], vf[R::kBlocks];
+    load_rows<T, D>(there ? k + token * args.k.token + item.head * args.k.head : nullptr, args.head_dim, lane, kf);
+    load_rows<T, D>(there ? v + token * args.v.token + item.head * args.v.head : nullptr, args.head_dim, lane, vf);
+    const float c = args.scale * kLog2e;
+    Acc grad_k[R::kTiles], grad_v[R::kTiles];
+#pragma unroll
+    for (int t = 0; t < R::kTiles; ++t) {
+        grad_k[t] = Acc{};
+        grad_v[t] = Acc{};
+    }
+    const std::int64_t first_query = span.first_query;
+    for (int g = 0; g < args.group; ++g) {
+        const int head = item.head * args.group + g;
+        const Loads q_loads(q + first_query * args.q.token + head * args.q.head, args.q.token, args.head_dim, wave, lane);
+        const Loads d_loads(gradients.grad_out + first_query * args.out.token + head * args.out.head, args.out.token,
+                            args.head_dim, wave, lane);
+        auto issue = [&](int first, int buffer) {
+            const unsigned int to = lds_base + static_cast<unsigned int>(buffer * 2 * Loads::kBytes);
+            q_loads.issue(first, span.queries - first, to, wave);
+            d_loads.issue(first, span.queries - first, to + Loads::kBytes, wave);
+        };
+        // A row's two numbers by one thread each, kept until the tile's turn.
+        const int which = thread / Q;
+        const int number = thread % Q;
+        auto fetch = [&](int first) -> float {
+            if (which > 1 || first + number >= span.queries) {
+                return which == 0 ? -INFINITY : 0.F; // (a row that is not there has weights of 0)
+            }
+            const std::int64_t at = (first_query + first + number) * args.heads + head;
+            return which == 0 ? -gradients.lse[at] * kLog2e : static_cast<const float*>(gradients.workspace)[at];
+        };
+        if (start >= span.queries) {
+            break; // no query sees these keys
+        }
+        __syncthreads(); // the last head's blocks are done with
+        issue(start, 0);
+        float held = fetch(start);
+        int buffer = 0;
+        for (int first = start; first < span.queries; first += Q) {
+            if (which < 2) {
+                numbers[(buffer * 2 + which) * Q + number] = held;
+            }
+            landed();
+            if (first + Q < span.queries) {
+                issue(first + Q, buffer ^ 1);
+                held = fetch(first + Q);
+            }
+            const unsigned char* const queries = lds + buffer * 2 * Loads::kBytes;
+            const unsigned char* const grads = queries + Loads::kBytes;
+            const float* const shifts = numbers + buffer * 2 * Q;
+            const float* const deltas = shifts + Q;
+            buffer ^= 1;
+            if (first + Q <= wave_least) {
+                continue;
+            }
+#pragma unroll
+            for (int t = 0; t < Q / E; ++t) {
+                Acc x{}, y{};
+#pragma unroll
+                for (int b = 0; b < R::kBlocks; ++b) {
+                    Mma<T>::run(x, R::along(queries, t * E + lane % E, b, lane), kf[b]);
+                    Mma<T>::run(y, R::along(grads, t * E + lane % E, b, lane), vf[b]);
+                }
+#pragma unroll
+                for (int run = 0; run < Mma<T>::kRuns; ++run) {
+                    const int at = t * E + Mma<T>::column(lane, run);
+                    const Vec16 s = load16(shifts + at);
+                    const Vec16 d = load16(deltas + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * run + e;
+                        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, __uint_as_float(s.w[e])));
+                        y[i] -= __uint_as_float(d.w[e]);
+                    }
+                }
+                if (first < wave_most) {
+#pragma unroll
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        x[i] = first + t * E + row_of<T>(lane, i) >= from ? x[i] : 0.F;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    y[i] *= x[i];
+                }
+#pragma unroll
+                for (int p = 0; p < kParts<T>; ++p) {
+                    const Vec16 weights = weights_of<T>(x, p);
+                    const Vec16 slopes = weights_of<T>(y, p);
+#pragma unroll
+                    for (int d = 0; d < R::kTiles; ++d) {
+                        Mma<T>::run(grad_v[d], R::across(grads, t * E + 16 * p, d, lane), weights);
+                        Mma<T>::run(grad_k[d], R::across(queries, t * E + 16 * p, d, lane), slopes);
+                    }
+                }
+            }
+        }
+    }
+    if (there) {
+        store_row<T, D>(gradients.grad_k + token * args.k.token + item.head * args.k.head, grad_k, args.scale,
+                        args.head_dim, lane);
+        store_row<T, D>(gradients.grad_v + token * args.v.token + item.head * args.v.head, grad_v, 1.0F, args.head_dim,
+                        lane);
+    }
+}
+
+template <typename T>
+hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& gradients, const PackedArgs& args,
+                  hipStream_t stream) {
+    return with_width(args.head_dim, [&](auto width) -> hipError_t {
+        constexpr int D = decltype(width)::value;
+        constexpr int kTile = Mma<T>::kEdge * kWaves;
+        constexpr std::size_t kLds = 4 * Stage<T, D, kBlockRows<T, D>>::kBytes;
+        constexpr std::size_t kNumbers = 4 * kBlockRows<T, D> * sizeof(float);
+        constexpr auto by_queries = query_gradient_kernel<T, D>;
+        constexpr auto by_keys = key_gradient_kernel<T, D>;
+        const std::int64_t query_tiles = slots(args.tokens, args.group, kTile, args.sequences);
+        const std::int64_t key_tiles = slots(args.kv_tokens, 1, kTile, args.sequences);
+        const std::int64_t query_blocks = items(query_tiles, args.kv_heads);
+        const std::int64_t key_blocks = items(key_tiles, args.kv_heads);
+        if (!launchable(query_blocks, kThreads) || !launchable(key_blocks, kThreads)) {
+            return hipErrorInvalidConfiguration;
+        }
+        hipError_t result = allow_lds<by_queries>(kLds);
+        result = result == hipSuccess ? allow_lds<by_keys>(kLds + kNumbers) : result;
+        if (result != hipSuccess) {
+            return result;
+        }
+        by_queries<<<static_cast<unsigned int>(query_blocks), kThreads, kLds, stream>>>(
+            q, k, v, gradients, args, static_cast<int>(query_tiles));
+        if (result = hipGetLastError(); result != hipSuccess) {
+            return result;
+        }
+        by_keys<<<static_cast<unsigned int>(key_blocks), kThreads, kLds + kNumbers, stream>>>(
+            q, k, v, gradients, args, static_cast<int>(key_tiles));
+        return hipGetLastError();
+    });
+}
+
+} // namespace
+} // namespace packed
+
+hipError_t packed_attention_backward(const float* q, const float* k, const float* v,
+                                     const PackedGradients<float>& gradients, const PackedArgs& args,
+                                     hipStream_t stream) {
+    return packed::launch(q, k, v, gradients, args, stream);
+}
+
+hipError_t packed_attention_backward(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v,
+                                     const PackedGradients<std::uint16_t>& gradients, const PackedArgs& args,
+                                     hipStream_t stream) {
+    return packed::launch(q, k, v, gradients, args, stream);
+}
+
+std::int64_t packed_attention_backward_workspace(const PackedArgs& args) {
+    return static_cast<std::int64_t>(args.tokens) * args.heads * static_cast<std::int64_t>(sizeof(float));
+}
+
+} // namespace cuvit::detail

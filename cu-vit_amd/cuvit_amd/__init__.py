@@ -33,6 +33,8 @@ __all__ = [
     "RotaryProblem", "QkNormProblem", "GatedProblem", "rotary_problem", "qk_norm_problem", "gated_problem",
     "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "qk_norm_rotary_workspace",
     "gated_gemm", "gated_backward",
+    "PackedAttentionProblem", "packed_attention_problem", "packed_attention", "packed_attention_workspace",
+    "packed_attention_backward", "packed_attention_backward_workspace",
     "ROTARY_HALVES", "ROTARY_ADJACENT", "NORM_RMS", "NORM_LAYER",
     "GATE_SILU", "GATE_GELU", "GATE_GELU_TANH",
 ]
@@ -239,6 +241,32 @@ class GatedProblem(ctypes.Structure):
     ]
 
 
+class TokenStrides(ctypes.Structure):
+    """cuvit_token_strides: elements from one token and head to the next; 0
+    selects the packed [tokens, heads, head_dim] one."""
+
+    _fields_ = [("token", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class PackedAttentionProblem(ctypes.Structure):
+    """cuvit_packed_attention_problem."""
+
+    _fields_ = [
+        ("sequences", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("kv_tokens", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_uint8),
+        ("q", TokenStrides),
+        ("k", TokenStrides),
+        ("v", TokenStrides),
+        ("out", TokenStrides),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
@@ -283,6 +311,14 @@ _SIGNATURES = {
     "cuvit_gated_gemm_bf16": (_I, [_P, _P, _P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
     "cuvit_gated_backward_f32": (_I, [_P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
     "cuvit_gated_backward_bf16": (_I, [_P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_packed_attention_problem_init": (None, [ctypes.POINTER(PackedAttentionProblem), _I, _I, _I, _I]),
+    "cuvit_packed_attention_problem_projection": (None, [ctypes.POINTER(PackedAttentionProblem)]),
+    "cuvit_packed_attention_workspace": (_L, [ctypes.POINTER(PackedAttentionProblem)]),
+    "cuvit_packed_attention_f32": (_I, [_P] * 9 + [_L, ctypes.POINTER(PackedAttentionProblem), _P]),
+    "cuvit_packed_attention_bf16": (_I, [_P] * 9 + [_L, ctypes.POINTER(PackedAttentionProblem), _P]),
+    "cuvit_packed_attention_backward_workspace": (_L, [ctypes.POINTER(PackedAttentionProblem)]),
+    "cuvit_packed_attention_backward_f32": (_I, [_P] * 13 + [_L, ctypes.POINTER(PackedAttentionProblem), _P]),
+    "cuvit_packed_attention_backward_bf16": (_I, [_P] * 13 + [_L, ctypes.POINTER(PackedAttentionProblem), _P]),
     "cuvit_weight_writer_create": (_I, [ctypes.POINTER(_P)]),
     "cuvit_weight_writer_add": (_I, [_P, ctypes.c_char_p, _I, ctypes.POINTER(_L), _P]),
     "cuvit_weight_writer_add_bf16": (_I, [_P, ctypes.c_char_p, _I, ctypes.POINTER(_L), _P]),
@@ -348,11 +384,15 @@ _NATIVE_FUNCTIONS = (
     "cuvit_rotary_f32", "cuvit_rotary_bf16", "cuvit_qk_norm_rotary_f32", "cuvit_qk_norm_rotary_bf16",
     "cuvit_qk_norm_rotary_backward_f32", "cuvit_qk_norm_rotary_backward_bf16", "cuvit_qk_norm_rotary_workspace",
     "cuvit_gated_gemm_f32", "cuvit_gated_gemm_bf16", "cuvit_gated_backward_f32", "cuvit_gated_backward_bf16",
+    "cuvit_packed_attention_f32", "cuvit_packed_attention_bf16", "cuvit_packed_attention_workspace",
+    "cuvit_packed_attention_backward_f32", "cuvit_packed_attention_backward_bf16",
+    "cuvit_packed_attention_backward_workspace",
 )
 
 
 _NATIVE_CALLS = ("layer_norm", "softmax", "extract_patches", "gemm", "attention", "preprocess", "vit_forward",
-                 "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "gated_gemm", "gated_backward")
+                 "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "gated_gemm", "gated_backward",
+                 "packed_attention", "packed_attention_backward")
 
 
 def _not_plain(*arguments) -> int:
@@ -402,7 +442,7 @@ class _NativeCalls:
                 if native is not None:
                     lib = library()
                     native.bind(GemmProblem, Preprocessing, RotaryProblem, QkNormProblem, GatedProblem,
-                                *(ctypes.cast(getattr(lib, f), _P).value for f in _NATIVE_FUNCTIONS))
+                                PackedAttentionProblem, *(ctypes.cast(getattr(lib, f), _P).value for f in _NATIVE_FUNCTIONS))
                 for call in _NATIVE_CALLS:
                     setattr(self, call, getattr(native, call) if native is not None else _not_plain)
         return self.__dict__[name]
@@ -904,6 +944,144 @@ def gated_backward(preactivations, grad, grad_preactivations, problem: GatedProb
             grad = _operand(grad, "grad", t, reach[0])
             grad_preactivations = _operand(grad_preactivations, "grad_preactivations", t, reach[1])
     check(fn(_ptr(preactivations), _ptr(grad), _ptr(grad_preactivations), ctypes.byref(problem),
+             stream_handle(stream)))
+
+
+def packed_attention_problem(sequences: int, tokens: int, heads: int, head_dim: int, kv_heads: Optional[int] = None,
+                             kv_tokens: Optional[int] = None, causal: bool = False, scale: float = 0.0,
+                             projection: bool = False) -> PackedAttentionProblem:
+    """Attention over ``sequences`` packed ones: q and out [tokens, heads,
+    head_dim], k and v [kv_tokens, kv_heads, head_dim] (kv_tokens as many as
+    tokens, kv_heads as heads unless given), or with ``projection`` all three
+    within one [tokens, heads + 2 kv_heads, head_dim], as qk_norm_rotary() leaves
+    it. Causal: the last query sees the last key. scale 0 is 1 / sqrt(head_dim)."""
+    problem = PackedAttentionProblem()
+    library().cuvit_packed_attention_problem_init(ctypes.byref(problem), sequences, tokens, heads, head_dim)
+    if kv_heads is not None:
+        problem.kv_heads = kv_heads
+    if kv_tokens is not None:
+        problem.kv_tokens = kv_tokens
+    problem.causal = int(causal)
+    problem.scale = scale
+    if projection:
+        library().cuvit_packed_attention_problem_projection(ctypes.byref(problem))
+    return problem
+
+
+def packed_attention_workspace(problem: PackedAttentionProblem) -> int:
+    """Bytes of the workspace that packed_attention() needs, 0 for none."""
+    return library().cuvit_packed_attention_workspace(ctypes.byref(problem))
+
+
+def packed_attention_backward_workspace(problem: PackedAttentionProblem) -> int:
+    """Bytes of the workspace that packed_attention_backward() needs."""
+    return library().cuvit_packed_attention_backward_workspace(ctypes.byref(problem))
+
+
+def _packed_reach(tokens: int, heads: int, head_dim: int, strides: TokenStrides) -> int:
+    if tokens == 0:
+        return 0
+    return ((tokens - 1) * (strides.token or heads * head_dim) + (heads - 1) * (strides.head or head_dim) + head_dim)
+
+
+def _packed_operands(p: PackedAttentionProblem, names, q, k, v, bf16: bool):
+    """Addresses of q, k and v, or of the projection q where k and v are None."""
+    t, size = _storage(bf16), 2 if bf16 else 4
+    shared = (p.kv_tokens, p.kv_heads, p.head_dim)
+    if k is None and v is None and q is not None and p.kv_tokens > 0:
+        if p.kv_tokens != p.tokens:
+            raise InvalidArgument(ERROR_INVALID_ARGUMENT, f"{names[0]} without {names[1]} and {names[2]} is a "
+                                  "projection, which holds as many keys as queries")
+        to_k, to_v = p.heads * p.head_dim, (p.heads + p.kv_heads) * p.head_dim
+        reach = max(_packed_reach(p.tokens, p.heads, p.head_dim, p.q), to_k + _packed_reach(*shared, p.k),
+                    to_v + _packed_reach(*shared, p.v))
+        slots = (p.heads + 2 * p.kv_heads) * p.head_dim
+        if any(s.token < slots or s.head not in (0, p.head_dim) for s in (p.q, p.k, p.v)):
+            raise InvalidArgument(ERROR_INVALID_ARGUMENT, f"{names[0]} without {names[1]} and {names[2]} is a "
+                                  "projection; the problem's strides are not one's (projection=True)")
+        q = _operand(q, names[0], t, reach)
+        return q, q + to_k * size, q + to_v * size
+    return (_operand(q, names[0], t, _packed_reach(p.tokens, p.heads, p.head_dim, p.q)),
+            _operand(k, names[1], t, _packed_reach(*shared, p.k)),
+            _operand(v, names[2], t, _packed_reach(*shared, p.v)))
+
+
+def _packed_plain(p: PackedAttentionProblem) -> bool:
+    """Whether the operands' sizes follow from the problem; else the library
+    names what is wrong, or has nothing to do."""
+    return (_positive(p.sequences, p.heads, p.kv_heads, p.head_dim) and p.tokens >= 0 and p.kv_tokens >= 0
+            and all(s.token >= 0 and s.head >= 0 for s in (p.q, p.k, p.v, p.out)))
+
+
+def _packed_starts(p: PackedAttentionProblem, starts, kv_starts, kv_lengths):
+    return (_operand(starts, "starts", "int32", p.sequences + 1),
+            _operand(kv_starts, "kv_starts", "int32", p.sequences + 1),
+            _operand(kv_lengths, "kv_lengths", "int32", p.sequences))
+
+
+def packed_attention(q, k, v, starts, out, problem: PackedAttentionProblem, kv_starts=None, kv_lengths=None, lse=None,
+                     workspace=None, stream=None, bf16: Optional[bool] = None) -> None:
+    """out = softmax(scale q.k^T).v within each of the packed sequences: sequence s
+    has the queries starts[s] to starts[s + 1] - 1 and the keys kv_starts[s] to
+    kv_starts[s + 1] - 1 (kv_starts None: starts), of which with kv_lengths the
+    first kv_lengths[s] are filled; all int32 GPU tensors. With k and v None, q is
+    a whole projection [tokens, heads + 2 kv_heads, head_dim]. lse, [tokens, heads]
+    fp32 or None, receives each row's log-sum-exp, which the gradients need.
+    ``workspace``: a uint8 tensor of packed_attention_workspace() bytes (None for
+    0) that one call uses at a time. Rows outside every sequence stay as they
+    were. An extension."""
+    status = _native_calls.packed_attention(q, k, v, starts, out, problem, kv_starts, kv_lengths, lse, workspace,
+                                            stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(q)
+    fn = library().cuvit_packed_attention_bf16 if bf16 else library().cuvit_packed_attention_f32
+    p = problem
+    nbytes = packed_attention_workspace(p)
+    if _packed_plain(p) and p.tokens > 0:
+        _launch_device(stream, q, k, v, starts, out, kv_starts, kv_lengths, lse, workspace)
+        q, k, v = _packed_operands(p, ("q", "k", "v"), q, k, v, bf16)
+        starts, kv_starts, kv_lengths = _packed_starts(p, starts, kv_starts, kv_lengths)
+        out = _operand(out, "out", _storage(bf16), _packed_reach(p.tokens, p.heads, p.head_dim, p.out))
+        lse = _operand(lse, "lse", "float32", p.tokens * p.heads)
+        workspace = _operand(workspace, "workspace", "uint8", nbytes)
+    check(fn(_ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(kv_starts), _ptr(kv_lengths), _ptr(out), _ptr(lse),
+             _ptr(workspace), nbytes, ctypes.byref(problem), stream_handle(stream)))
+
+
+def packed_attention_backward(q, k, v, starts, out, lse, grad_out, grad_q, grad_k, grad_v,
+                              problem: PackedAttentionProblem, kv_starts=None, kv_lengths=None, workspace=None,
+                              stream=None, bf16: Optional[bool] = None) -> None:
+    """The gradients of packed_attention() from its operands, its out and lse and
+    the gradient of out. grad_q, grad_k and grad_v are overwritten within the
+    sequences; with k and v None, grad_q is the whole projection's gradient and
+    grad_k and grad_v are None. ``workspace``: a uint8 tensor of
+    packed_attention_backward_workspace() bytes that one call uses at a time:
+    calls on several streams, and captured graphs that may overlap, take one
+    each. An extension."""
+    status = _native_calls.packed_attention_backward(q, k, v, starts, out, lse, grad_out, grad_q, grad_k, grad_v,
+                                                     problem, kv_starts, kv_lengths, workspace, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(q)
+    fn = library().cuvit_packed_attention_backward_bf16 if bf16 else library().cuvit_packed_attention_backward_f32
+    p = problem
+    nbytes = packed_attention_backward_workspace(p)
+    if _packed_plain(p) and p.tokens + p.kv_tokens > 0:
+        _launch_device(stream, q, k, v, starts, out, lse, grad_out, grad_q, grad_k, grad_v, kv_starts, kv_lengths,
+                       workspace)
+        if (k is None and v is None) != (grad_k is None and grad_v is None):
+            raise InvalidArgument(ERROR_INVALID_ARGUMENT, "a projection's gradient is one tensor, as it is")
+        q, k, v = _packed_operands(p, ("q", "k", "v"), q, k, v, bf16)
+        grad_q, grad_k, grad_v = _packed_operands(p, ("grad_q", "grad_k", "grad_v"), grad_q, grad_k, grad_v, bf16)
+        starts, kv_starts, kv_lengths = _packed_starts(p, starts, kv_starts, kv_lengths)
+        reach = _packed_reach(p.tokens, p.heads, p.head_dim, p.out)
+        out = _operand(out, "out", _storage(bf16), reach)
+        grad_out = _operand(grad_out, "grad_out", _storage(bf16), reach)
+        lse = _operand(lse, "lse", "float32", p.tokens * p.heads)
+        workspace = _operand(workspace, "workspace", "uint8", nbytes)
+    check(fn(_ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(kv_starts), _ptr(kv_lengths), _ptr(out), _ptr(lse),
+             _ptr(grad_out), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v), _ptr(workspace), nbytes, ctypes.byref(problem),
              stream_handle(stream)))
 
 

@@ -322,6 +322,106 @@ int cuvit_gated_backward_bf16(const cuvit_bf16* preactivations, const cuvit_bf16
                               cuvit_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Attention over packed sequences: images and clips of different lengths one
+ * behind the other, each attended within itself; extensions by the same rules.
+ *
+ * Sequence s has queries starts[s] to starts[s + 1] - 1 of q, a token a row, and
+ * keys kv_starts[s] to kv_starts[s + 1] - 1 of k and v; with kv_lengths only the
+ * first kv_lengths[s] of them (a cache with room behind). All three are int32 in
+ * device memory, [sequences + 1], [sequences + 1] and [sequences]; a null
+ * kv_starts is starts (kv_tokens is then tokens), a null kv_lengths all keys.
+ * Starts do not decrease; numbers that leave the operands are cut to them. A
+ * length may be 0. Rows outside every sequence are not read, and their results
+ * and gradients stay as they were.
+ *
+ * Query head h sees key head h / (heads / kv_heads). Causal: the last query sees
+ * the last key, the one before it all keys but that, and so on. A query that sees
+ * no key gets zeros, its log-sum-exp is -infinity; logits that are all -infinity,
+ * or a NaN among them, give NaN.
+ * ------------------------------------------------------------------------- */
+
+/* Elements from one token and head to the next; 0 selects the packed
+ * [tokens, heads, head_dim] one. Whole 16-byte pieces; a token's at least
+ * head_dim and at most 2^23 bytes. */
+typedef struct cuvit_token_strides {
+    int64_t token;
+    int64_t head;
+} cuvit_token_strides;
+
+typedef struct cuvit_packed_attention_problem {
+    int sequences;
+    int tokens;     /* rows of q and out */
+    int kv_tokens;  /* rows of k and v */
+    int heads;      /* a multiple of kv_heads */
+    int kv_heads;
+    int head_dim;   /* a multiple of 8, at most 256 */
+    float scale;    /* of the logits, a positive normal float; 0: 1 / sqrt(head_dim) */
+    uint8_t causal;
+    cuvit_token_strides q;
+    cuvit_token_strides k;
+    cuvit_token_strides v;
+    cuvit_token_strides out;
+} cuvit_packed_attention_problem;
+
+/* kv_tokens = tokens, kv_heads = heads, all tokens seen, packed layouts. */
+void cuvit_packed_attention_problem_init(cuvit_packed_attention_problem* problem, int sequences,
+                                         int tokens, int heads, int head_dim);
+/* The strides of operands within one projection [tokens, heads + 2 kv_heads,
+ * head_dim] (what cuvit_qk_norm_rotary_* leaves), for the problem's heads: q is
+ * its address, k lies heads * head_dim values behind, v kv_heads * head_dim
+ * behind k; out stays packed. */
+void cuvit_packed_attention_problem_projection(cuvit_packed_attention_problem* problem);
+
+/* out = softmax(scale q.k^T).v; lse, [tokens, heads] fp32 or null, receives each
+ * row's log(sum(exp(logits))). Logits, softmax and sums are fp32; the bf16 twin
+ * rounds the weights to bf16 for their product with v. Operands are 16-byte
+ * aligned; out and lse overlap no other operand. The workspace, of
+ * cuvit_packed_attention_workspace() bytes (null where that is 0) and 16-byte
+ * aligned, is used by one call at a time: calls that may overlap, replays of
+ * captured ones among them, take one each. More than 65535 heads, or 2^31 - 1
+ * tokens times heads of either side, or 2^32 threads (2^24 tiles of 64 rows in
+ * fp32, 128 in bf16, a sequence starting a new one) are CUVIT_ERROR_LENGTH. */
+int64_t cuvit_packed_attention_workspace(const cuvit_packed_attention_problem* problem);
+int cuvit_packed_attention_f32(const float* q, const float* k, const float* v,
+                               const int32_t* starts, const int32_t* kv_starts,
+                               const int32_t* kv_lengths, float* out, float* lse, void* workspace,
+                               int64_t workspace_bytes,
+                               const cuvit_packed_attention_problem* problem,
+                               cuvit_stream_t stream);
+int cuvit_packed_attention_bf16(const cuvit_bf16* q, const cuvit_bf16* k, const cuvit_bf16* v,
+                                const int32_t* starts, const int32_t* kv_starts,
+                                const int32_t* kv_lengths, cuvit_bf16* out, float* lse,
+                                void* workspace, int64_t workspace_bytes,
+                                const cuvit_packed_attention_problem* problem,
+                                cuvit_stream_t stream);
+
+/* Its gradients, from the forward's operands, its out and lse (not null) and the
+ * gradient of out (in out's strides); grad_q, grad_k and grad_v, in their
+ * operands' strides, are overwritten within the sequences (zeros for a key that
+ * no query sees) and overlap no operand. A key head's gradients are sums over
+ * its group's heads. Every sum is in fp32, in an order that sizes fix. Infinities
+ * and NaN may spread to all gradients of their sequence. The workspace is
+ * cuvit_packed_attention_backward_workspace() bytes, by the forward's rules. */
+int64_t cuvit_packed_attention_backward_workspace(const cuvit_packed_attention_problem* problem);
+int cuvit_packed_attention_backward_f32(const float* q, const float* k, const float* v,
+                                        const int32_t* starts, const int32_t* kv_starts,
+                                        const int32_t* kv_lengths, const float* out,
+                                        const float* lse, const float* grad_out, float* grad_q,
+                                        float* grad_k, float* grad_v, void* workspace,
+                                        int64_t workspace_bytes,
+                                        const cuvit_packed_attention_problem* problem,
+                                        cuvit_stream_t stream);
+int cuvit_packed_attention_backward_bf16(const cuvit_bf16* q, const cuvit_bf16* k,
+                                         const cuvit_bf16* v, const int32_t* starts,
+                                         const int32_t* kv_starts, const int32_t* kv_lengths,
+                                         const cuvit_bf16* out, const float* lse,
+                                         const cuvit_bf16* grad_out, cuvit_bf16* grad_q,
+                                         cuvit_bf16* grad_k, cuvit_bf16* grad_v, void* workspace,
+                                         int64_t workspace_bytes,
+                                         const cuvit_packed_attention_problem* problem,
+                                         cuvit_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * bfloat16 I/O twins. An extension: the reference has no reduced-precision
  * path (README.md:472-473). Storage is bf16, every reduction and every
  * intermediate is fp32, gamma/beta/bias stay fp32, and each result is rounded
