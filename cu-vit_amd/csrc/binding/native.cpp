@@ -63,6 +63,11 @@ struct Library {
     decltype(&cuvit_packed_attention_backward_f32) packed_attention_backward_f32;
     decltype(&cuvit_packed_attention_backward_bf16) packed_attention_backward_bf16;
     decltype(&cuvit_packed_attention_backward_workspace) packed_attention_backward_workspace;
+    decltype(&cuvit_gated_checkpoint_gemm_f32) gated_checkpoint_gemm_f32;
+    decltype(&cuvit_gated_checkpoint_gemm_bf16) gated_checkpoint_gemm_bf16;
+    decltype(&cuvit_gated_checkpoint_backward_f32) gated_checkpoint_backward_f32;
+    decltype(&cuvit_gated_checkpoint_backward_bf16) gated_checkpoint_backward_bf16;
+    decltype(&cuvit_gated_checkpoint_scales) gated_checkpoint_scales;
 };
 Library library{};
 /// The problem structs' ctypes types.
@@ -682,6 +687,77 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
     });
 }
 
+// (a, b, bias, c, codes, scales, problem, stream, bf16)
+PyObject* gated_checkpoint_gemm(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 9 || !storage(a[8], a[0], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[6], problem_types[kGated], sizeof(cuvit_gated_problem));
+        const auto* const p = static_cast<const cuvit_gated_problem*>(view.get());
+        std::int64_t c_reach, pre_reach;
+        if (!gated_reach(p, &c_reach, &pre_reach) || p->k <= 0) {
+            return kNotPlain;
+        }
+        const std::int64_t lda = p->lda != 0 ? p->lda : p->k;
+        const std::int64_t ldb = p->ldb != 0 ? p->ldb : p->k;
+        if (lda < p->k || ldb < p->k) {
+            return kNotPlain;
+        }
+        Operands operands(a[7]);
+        const void* const left = operands.get(a[0], type, (p->m - 1) * lda + p->k);
+        const void* const right = operands.get(a[1], type, (2 * static_cast<std::int64_t>(p->n) - 1) * ldb + p->k);
+        const float* const bias = operands.floats(a[2], 2 * static_cast<std::int64_t>(p->n));
+        void* const c = operands.get(a[3], type, c_reach);
+        auto* const codes = static_cast<std::uint8_t*>(operands.get(a[4], at::kFloat8_e4m3fn, pre_reach));
+        auto* const scales = static_cast<std::uint8_t*>(
+            operands.get(a[5], at::ScalarType::Float8_e8m0fnu, library.gated_checkpoint_scales(p)));
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat
+                       ? library.gated_checkpoint_gemm_f32(singles(left), singles(right), bias, singles(c), codes,
+                                                           scales, p, operands.stream())
+                       : library.gated_checkpoint_gemm_bf16(bits(left), bits(right), bias, bits(c), codes, scales, p,
+                                                            operands.stream());
+        });
+    });
+}
+
+// (codes, scales, grad, grad_preactivations, problem, hidden, stream, bf16)
+PyObject* gated_checkpoint_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return answer([&]() -> long {
+        at::ScalarType type;
+        if (count != 8 || !storage(a[7], a[2], &type)) {
+            return kNotPlain;
+        }
+        const Struct view(a[4], problem_types[kGated], sizeof(cuvit_gated_problem));
+        const auto* const p = static_cast<const cuvit_gated_problem*>(view.get());
+        std::int64_t c_reach, pre_reach;
+        if (!gated_reach(p, &c_reach, &pre_reach)) {
+            return kNotPlain;
+        }
+        Operands operands(a[6]);
+        const auto* const codes = static_cast<std::uint8_t*>(operands.get(a[0], at::kFloat8_e4m3fn, pre_reach));
+        const auto* const scales = static_cast<std::uint8_t*>(
+            operands.get(a[1], at::ScalarType::Float8_e8m0fnu, library.gated_checkpoint_scales(p)));
+        const void* const grad = operands.get(a[2], type, c_reach);
+        void* const to = operands.get(a[3], type, pre_reach);
+        void* const hidden = operands.maybe(a[5], type, c_reach);
+        if (!operands.plain()) {
+            return kNotPlain;
+        }
+        return unlocked([&]() -> long {
+            return type == at::kFloat ? library.gated_checkpoint_backward_f32(codes, scales, singles(grad), singles(to),
+                                                                              singles(hidden), p, operands.stream())
+                                      : library.gated_checkpoint_backward_bf16(codes, scales, bits(grad), bits(to),
+                                                                               bits(hidden), p, operands.stream());
+        });
+    });
+}
+
 /// What the operands of packed attention reach, in the problem's strides; false for
 /// a problem without tokens, keys or heads, or whose strides no tensor holds.
 struct PackedReach {
@@ -847,7 +923,8 @@ PyMethodDef methods[] = {CUVIT_FAST(bind),           CUVIT_FAST(layer_norm), CUV
                          CUVIT_FAST(preprocess),     CUVIT_FAST(vit_forward), CUVIT_FAST(rotary),
                          CUVIT_FAST(qk_norm_rotary), CUVIT_FAST(qk_norm_rotary_backward), CUVIT_FAST(gated_gemm),
                          CUVIT_FAST(gated_backward), CUVIT_FAST(packed_attention),
-                         CUVIT_FAST(packed_attention_backward), {nullptr, nullptr, 0, nullptr}};
+                         CUVIT_FAST(packed_attention_backward), CUVIT_FAST(gated_checkpoint_gemm),
+                         CUVIT_FAST(gated_checkpoint_backward), {nullptr, nullptr, 0, nullptr}};
 #undef CUVIT_FAST
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "The launchers' plain case.", -1, methods,

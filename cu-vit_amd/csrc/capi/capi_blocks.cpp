@@ -303,12 +303,10 @@ int check_gated_layout(const cuvit_gated_problem& p, detail::GatedArgs* args) {
     return ok();
 }
 
-template <typename T>
-int gated_gemm(const T* a, const T* b, const float* bias, T* c, T* preactivations, const cuvit_gated_problem* problem,
-               cuvit_stream_t stream) {
-    detail::GatedArgs args{};
-    bool empty = false;
-    if (const int s = check_gated_sides(problem, &args, &empty); s != CUVIT_OK || empty) {
+/// The checks of a gated product with its operands, into *args.
+int check_gated_gemm(const void* a, const void* b, const void* c, const cuvit_gated_problem* problem,
+                     detail::GatedArgs* args, bool* empty) {
+    if (const int s = check_gated_sides(problem, args, empty); s != CUVIT_OK || *empty) {
         return s;
     }
     const cuvit_gated_problem& p = *problem;
@@ -318,23 +316,76 @@ int gated_gemm(const T* a, const T* b, const float* bias, T* c, T* preactivation
     if (a == nullptr || b == nullptr || c == nullptr) {
         return fail(CUVIT_ERROR_INVALID_ARGUMENT, "Gated operands cannot be null");
     }
-    if (const int s = check_gated_layout(p, &args); s != CUVIT_OK) {
+    if (const int s = check_gated_layout(p, args); s != CUVIT_OK) {
         return s;
     }
     if (p.k > kMaxDepth) {
         return fail(CUVIT_ERROR_LENGTH, "Gated products take a k of at most 2^31 - 4096");
     }
-    args.k = p.k;
-    args.lda = p.lda != 0 ? p.lda : p.k;
-    args.ldb = p.ldb != 0 ? p.ldb : p.k;
-    if (args.lda < p.k || args.ldb < p.k) {
+    args->k = p.k;
+    args->lda = p.lda != 0 ? p.lda : p.k;
+    args->ldb = p.ldb != 0 ? p.ldb : p.k;
+    if (args->lda < p.k || args->ldb < p.k) {
         return fail(CUVIT_ERROR_INVALID_ARGUMENT, "A gated leading dimension is smaller than its row");
     }
-    const hipError_t launched = detail::gated_gemm(a, b, bias, c, preactivations, args, as_hip(stream));
+    return ok();
+}
+
+int gated_launched(hipError_t launched, const char* what) {
     if (launched == hipErrorInvalidConfiguration) {
         return fail(CUVIT_ERROR_LENGTH, "Gated products take less than 2^32 threads");
     }
-    return from_hip(launched, "gated_gemm launch");
+    return from_hip(launched, what);
+}
+
+template <typename T>
+int gated_gemm(const T* a, const T* b, const float* bias, T* c, T* preactivations, const cuvit_gated_problem* problem,
+               cuvit_stream_t stream) {
+    detail::GatedArgs args{};
+    bool empty = false;
+    if (const int s = check_gated_gemm(a, b, c, problem, &args, &empty); s != CUVIT_OK || empty) {
+        return s;
+    }
+    return gated_launched(detail::gated_gemm(a, b, bias, c, preactivations, args, as_hip(stream)), "gated_gemm launch");
+}
+
+template <typename T>
+int gated_checkpoint_gemm(const T* a, const T* b, const float* bias, T* c, std::uint8_t* codes, std::uint8_t* scales,
+                          const cuvit_gated_problem* problem, cuvit_stream_t stream) {
+    detail::GatedArgs args{};
+    bool empty = false;
+    if (const int s = check_gated_gemm(a, b, codes != nullptr && scales != nullptr ? c : nullptr, problem, &args, &empty);
+        s != CUVIT_OK || empty) {
+        return s;
+    }
+    args.codes = codes;
+    args.scales = scales;
+    return gated_launched(detail::gated_checkpoint_gemm(a, b, bias, c, args, as_hip(stream)),
+                          "gated_checkpoint_gemm launch");
+}
+
+template <typename T>
+int gated_checkpoint_backward(const std::uint8_t* codes, const std::uint8_t* scales, const T* grad,
+                              T* grad_preactivations, T* hidden, const cuvit_gated_problem* problem,
+                              cuvit_stream_t stream) {
+    detail::GatedArgs args{};
+    bool empty = false;
+    if (const int s = check_gated_sides(problem, &args, &empty); s != CUVIT_OK || empty) {
+        return s;
+    }
+    if (codes == nullptr || scales == nullptr || grad == nullptr || grad_preactivations == nullptr) {
+        return fail(CUVIT_ERROR_INVALID_ARGUMENT, "Gated operands cannot be null");
+    }
+    if (grad == grad_preactivations || hidden == grad_preactivations) {
+        return fail(CUVIT_ERROR_INVALID_ARGUMENT, "Gated gradients cannot replace the product's gradient");
+    }
+    if (const int s = check_gated_layout(*problem, &args); s != CUVIT_OK) {
+        return s;
+    }
+    args.codes = const_cast<std::uint8_t*>(codes);
+    args.scales = const_cast<std::uint8_t*>(scales);
+    return from_hip(detail::gated_checkpoint_backward(grad, grad_preactivations, hidden, args, as_hip(stream)),
+                    "gated_checkpoint_backward launch");
 }
 
 template <typename T>
@@ -487,6 +538,35 @@ int cuvit_gated_backward_bf16(const cuvit_bf16* preactivations, const cuvit_bf16
                               cuvit_bf16* grad_preactivations, const cuvit_gated_problem* problem,
                               cuvit_stream_t stream) {
     return capi::gated_backward(preactivations, grad, grad_preactivations, problem, stream);
+}
+
+int64_t cuvit_gated_checkpoint_scales(const cuvit_gated_problem* problem) {
+    return problem != nullptr && problem->m > 0 && problem->n > 0
+               ? 2 * static_cast<std::int64_t>(problem->m) * ((static_cast<std::int64_t>(problem->n) + 31) / 32)
+               : 0;
+}
+
+int cuvit_gated_checkpoint_gemm_f32(const float* a, const float* b, const float* bias, float* c, uint8_t* codes,
+                                    uint8_t* scales, const cuvit_gated_problem* problem, cuvit_stream_t stream) {
+    return capi::gated_checkpoint_gemm(a, b, bias, c, codes, scales, problem, stream);
+}
+
+int cuvit_gated_checkpoint_gemm_bf16(const cuvit_bf16* a, const cuvit_bf16* b, const float* bias, cuvit_bf16* c,
+                                     uint8_t* codes, uint8_t* scales, const cuvit_gated_problem* problem,
+                                     cuvit_stream_t stream) {
+    return capi::gated_checkpoint_gemm(a, b, bias, c, codes, scales, problem, stream);
+}
+
+int cuvit_gated_checkpoint_backward_f32(const uint8_t* codes, const uint8_t* scales, const float* grad,
+                                        float* grad_preactivations, float* hidden, const cuvit_gated_problem* problem,
+                                        cuvit_stream_t stream) {
+    return capi::gated_checkpoint_backward(codes, scales, grad, grad_preactivations, hidden, problem, stream);
+}
+
+int cuvit_gated_checkpoint_backward_bf16(const uint8_t* codes, const uint8_t* scales, const cuvit_bf16* grad,
+                                         cuvit_bf16* grad_preactivations, cuvit_bf16* hidden,
+                                         const cuvit_gated_problem* problem, cuvit_stream_t stream) {
+    return capi::gated_checkpoint_backward(codes, scales, grad, grad_preactivations, hidden, problem, stream);
 }
 
 } // extern "C"

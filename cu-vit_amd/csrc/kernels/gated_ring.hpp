@@ -5,6 +5,7 @@
 // wavefront are the two factors of the same outputs.
 #pragma once
 
+#include "checkpoint.hpp"
 #include "gate.hpp"
 #include "gemm_ring.hpp"
 #include "runs.hpp"
@@ -163,11 +164,206 @@ __device__ __forceinline__ void finish_tiles(const typename Mma<T>::Acc (&acc)[T
         }
 }
 
+/// A lane's part of a group's largest value: @p v's where @p col, the first one's, and
+/// what follows lie before column @p n.
+template <int Count> __device__ __forceinline__ void cut_columns(float (&v)[Count], int col, int n) {
+#pragma unroll
+    for (int e = 0; e < Count; ++e) {
+        v[e] = col + e < n ? v[e] : 0.0F;
+    }
+}
+
+/// The codes of a wavefront's tiles, from registers to memory: 4 bytes of a row a lane.
+/// In bf16 an MFMA tile's 32 outputs are a group, a lane and the one across from it
+/// holding a row of it; in fp32 two tiles of 16 are, of this wavefront or, where it has
+/// only one, of this and the next one of the row, which trade their halves' largest
+/// values through LDS (@p exchange: two for each of @p Rows rows of a half).
+template <typename T, int TM, int TN, int Rows>
+__device__ __forceinline__ void finish_codes(const typename Mma<T>::Acc (&acc)[TM][TN], int lane, int wave_n,
+                                             int tile_row, int row0, int col0, float* exchange,
+                                             const GatedArgs& args) {
+    constexpr int E = Mma<T>::kEdge;
+    constexpr int kTiles = kCodeGroup / E < TN / 2 ? kCodeGroup / E : TN / 2; // of this wavefront's in a group
+    constexpr bool kTraded = kTiles * E < kCodeGroup;
+    constexpr int kValues = E * E / kWave; // a lane's of a tile
+    auto values = [&](int i, int o, int half, float (&v)[kValues]) {
+#pragma unroll
+        for (int q = 0; q < Mma<T>::kRuns; ++q) {
+            float four[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                four[e] = acc[i][2 * o + half][4 * q + e];
+            }
+            cut_columns(four, col0 + o * E + Mma<T>::column(lane, q), args.n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[4 * q + e] = four[e];
+            }
+        }
+    };
+    auto largest_of = [&](int i, int o0, int half) {
+        float largest = 0.0F;
+#pragma unroll
+        for (int o = o0; o < o0 + kTiles; ++o) {
+            float v[kValues];
+            values(i, o, half, v);
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) {
+                largest = fmaxf(largest, finite_size(v[e]));
+            }
+        }
+        if constexpr (sizeof(T) == 4) {
+            largest = attention::combine_rows<16>(largest, Max{});
+        }
+        return attention::combine_rows<32>(largest, Max{});
+    };
+    if constexpr (kTraded) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                exchange[(half * Rows + tile_row + i * E + lane % E) * 2 + (wave_n & 1)] = largest_of(i, 0, half);
+        __syncthreads();
+    }
+    const int groups = (args.n + kCodeGroup - 1) / kCodeGroup;
+#pragma unroll
+    for (int o0 = 0; o0 < TN / 2; o0 += kTiles)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                float largest;
+                if constexpr (kTraded) {
+                    const float* const both = exchange + (half * Rows + tile_row + i * E + lane % E) * 2;
+                    largest = fmaxf(both[0], both[1]);
+                } else {
+                    largest = largest_of(i, o0, half);
+                }
+                const int row = row0 + tile_row + i * E + lane % E;
+                const std::uint32_t scale = code_scale(largest);
+                const float inverse = code_inverse(scale);
+                const int group = (col0 + o0 * E) / kCodeGroup;
+                if (row >= args.m) {
+                    continue;
+                }
+                if (lane < E && group < groups && (!kTraded || (wave_n & 1) == 0)) {
+                    args.scales[static_cast<std::int64_t>(row) * 2 * groups + half * groups + group] =
+                        static_cast<std::uint8_t>(scale);
+                }
+                std::uint8_t* const to = args.codes + static_cast<std::int64_t>(row) * args.ld_pre + half * args.n;
+#pragma unroll
+                for (int o = o0; o < o0 + kTiles; ++o) {
+                    float v[kValues];
+                    values(i, o, half, v);
+#pragma unroll
+                    for (int q = 0; q < Mma<T>::kRuns; ++q) {
+                        const int col = col0 + o * E + Mma<T>::column(lane, q);
+                        store_bytes<1>(to + col, {{four_codes(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inverse)}},
+                                       args.n - col);
+                    }
+                }
+            }
+}
+
+/// Where the codes of a bf16 tile lie in LDS: rows of the gate's, then the value's
+/// codes, 16-byte pieces turned by the row so that the rows that a wavefront writes at
+/// once spread over the banks; behind them a row's scales.
+template <int BO> struct CodeRows {
+    static constexpr int kPitch = 2 * BO;
+    static constexpr int kPieces = kPitch / 16;
+    static constexpr int kGroups = BO / kCodeGroup; // of a half
+    __device__ __forceinline__ static int piece(int row, int at) {
+        return row * kPitch + ((at ^ (row / (128 / BO) & (kPieces - 1))) << 4);
+    }
+    __device__ __forceinline__ static int scale(int rows, int row, int half, int group) {
+        return rows * kPitch + (row * 2 + half) * kGroups + group;
+    }
+};
+
+template <typename S>
+__device__ __forceinline__ void stage_codes(const floatx16 (&acc)[S::kTM][S::kTN], unsigned char* lds, int wave_m,
+                                            int wave_n, int lane, int col0, int n) {
+    constexpr int E = S::kEdge;
+    constexpr int kBO = S::kBN / 2;
+    using Place = CodeRows<kBO>;
+    static_assert(S::kBM * (Place::kPitch + 2 * Place::kGroups) <= S::kSlots * S::kStageBytes, "the ring holds the codes");
+    static_assert(E == kCodeGroup, "a tile's row is a group");
+    const bool whole = col0 + kBO <= n;
+#pragma unroll
+    for (int o = 0; o < S::kTN / 2; ++o)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < S::kTM; ++i) {
+                const int tile = wave_n * (S::kTN / 2) + o;
+                const int row = (wave_m * S::kTM + i) * E + lane % E;
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    v[e] = acc[i][2 * o + half][e];
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        v[e] = col0 + tile * E + Mma<std::uint16_t>::column(lane, e / 4) + e % 4 < n ? v[e] : 0.0F;
+                    }
+                }
+                float largest = 0.0F;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    largest = fmaxf(largest, finite_size(v[e]));
+                }
+                const std::uint32_t scale = code_scale(attention::combine_rows<32>(largest, Max{}));
+                const float inverse = code_inverse(scale);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int at = half * kBO + tile * E + Mma<std::uint16_t>::column(lane, q);
+                    *reinterpret_cast<std::uint32_t*>(lds + Place::piece(row, at / 16) + at % 16) =
+                        four_codes(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inverse);
+                }
+                if (lane < E) {
+                    lds[Place::scale(S::kBM, row, half, tile)] = static_cast<std::uint8_t>(scale);
+                }
+            }
+}
+
+template <int BM, int BO, int Threads>
+__device__ __forceinline__ void store_codes(const unsigned char* lds, int row0, int col0, const GatedArgs& args) {
+    using Place = CodeRows<BO>;
+    constexpr int kOfHalf = Place::kPieces / 2;
+    for (int i = static_cast<int>(threadIdx.x); i < BM * Place::kPieces; i += Threads) {
+        const int row = i / Place::kPieces;
+        const int at = i % Place::kPieces;
+        const int half = at / kOfHalf;
+        const int col = col0 + at % kOfHalf * 16;
+        if (row0 + row < args.m && col < args.n) {
+            const Vec16 v = load16(lds + Place::piece(row, at));
+            store_bytes<4>(args.codes + static_cast<std::int64_t>(row0 + row) * args.ld_pre + half * args.n + col,
+                           {{v.w[0], v.w[1], v.w[2], v.w[3]}}, args.n - col);
+        }
+    }
+    const int groups = (args.n + kCodeGroup - 1) / kCodeGroup;
+    for (int i = static_cast<int>(threadIdx.x); i < BM * 2; i += Threads) {
+        const int row = i / 2;
+        const int half = i % 2;
+        if (row0 + row < args.m) {
+            std::uint8_t* const to =
+                args.scales + static_cast<std::int64_t>(row0 + row) * 2 * groups + half * groups + col0 / kCodeGroup;
+#pragma unroll
+            for (int g = 0; g < Place::kGroups; ++g) {
+                if (col0 / kCodeGroup + g < groups) {
+                    to[g] = lds[Place::scale(BM, row, half, g)];
+                }
+            }
+        }
+    }
+}
+
 /// finish_tiles for bf16, through the drained ring: the MFMA layout gives a lane 8
 /// bytes of a row, 32 rows a store; from LDS the workgroup's rows go out as 16-byte
 /// pieces, side by side (12608 x 2048 x 768: 105 -> 99 us when it came). @p Streaming:
-/// C past the caches.
-template <typename S, Gate G, bool Streaming>
+/// C past the caches. @p Codes: the preactivations' codes, too.
+template <typename S, Gate G, bool Streaming, bool Codes>
 __device__ __forceinline__ void finish_staged(const floatx16 (&acc)[S::kTM][S::kTN], unsigned char* lds, bool loading,
                                               int wave_m, int wave_n, int lane, int row0, int col0, std::uint16_t* c,
                                               std::uint16_t* pre, const GatedArgs& args) {
@@ -221,7 +417,14 @@ __device__ __forceinline__ void finish_staged(const floatx16 (&acc)[S::kTM][S::k
         }
     };
     pass(std::integral_constant<int, 0>{}, c, args.ldc);
-    if (pre != nullptr) {
+    if constexpr (Codes) {
+        __syncthreads();
+        if (!loading) {
+            stage_codes<S>(acc, lds, wave_m, wave_n, lane, col0, args.n);
+        }
+        __syncthreads();
+        store_codes<S::kBM, kBO, S::kThreads>(lds, row0, col0, args);
+    } else if (pre != nullptr) {
         __syncthreads();
         pass(std::integral_constant<int, 1>{}, pre, args.ld_pre);
         __syncthreads();
@@ -299,7 +502,7 @@ __device__ __forceinline__ void gated_multiply(const Loads& loads, const unsigne
     stage_barrier(true);
 }
 
-template <typename T, typename S, Gate G, bool Streaming>
+template <typename T, typename S, Gate G, bool Streaming, bool Codes>
 __global__ __launch_bounds__(S::kThreads) void gated_ring_kernel(const T* __restrict__ a, const T* __restrict__ b,
                                                                  const float* __restrict__ bias, T* c, T* pre,
                                                                  GatedArgs args, TileMap map) {
@@ -339,10 +542,16 @@ __global__ __launch_bounds__(S::kThreads) void gated_ring_kernel(const T* __rest
         gated_multiply<S>(loads, lds, wave_m, wave_n, lane, stages, acc, start);
     }
     if constexpr (sizeof(T) == 2) {
-        finish_staged<S, G, Streaming>(acc, lds, loading, wave_m, wave_n, lane, row0, col0, c, pre, args);
+        finish_staged<S, G, Streaming, Codes>(acc, lds, loading, wave_m, wave_n, lane, row0, col0, c, pre, args);
     } else if (!loading) { // 16 bytes a lane, 64 a row: no slower than through LDS
         finish_tiles<T, G, S::kTM, S::kTN>(acc, lane, row0 + wave_m * S::kEdge * S::kTM,
                                            col0 + wave_n * S::kEdge * S::kTN / 2, c, pre, args);
+        if constexpr (Codes) {
+            static_assert(!S::kLoaders, "every wavefront passes the barrier");
+            finish_codes<T, S::kTM, S::kTN, S::kBM>(acc, lane, wave_n, wave_m * S::kEdge * S::kTM, row0,
+                                                    col0 + wave_n * S::kEdge * S::kTN / 2,
+                                                    reinterpret_cast<float*>(lds), args);
+        }
     }
 }
 

@@ -242,6 +242,10 @@ struct GatedArgs {
     int ldb;
     int ldc;
     int ld_pre;
+    /// The preactivations in 8 bits (checkpoint.hpp), rows ld_pre apart, and the packed
+    /// scales of their groups.
+    std::uint8_t* codes = nullptr;
+    std::uint8_t* scales = nullptr;
 };
 hipError_t gated_gemm(const float* a, const float* b, const float* bias, float* c, float* preactivations,
                       const GatedArgs& args, hipStream_t stream);
@@ -251,6 +255,17 @@ hipError_t gated_backward(const float* preactivations, const float* grad, float*
                           const GatedArgs& args, hipStream_t stream);
 hipError_t gated_backward(const std::uint16_t* preactivations, const std::uint16_t* grad,
                           std::uint16_t* grad_preactivations, const GatedArgs& args, hipStream_t stream);
+
+// gated_checkpoint.hip: the product that keeps codes, and the gradient from them (and
+// the product again, where @p hidden is not null).
+hipError_t gated_checkpoint_gemm(const float* a, const float* b, const float* bias, float* c, const GatedArgs& args,
+                                 hipStream_t stream);
+hipError_t gated_checkpoint_gemm(const std::uint16_t* a, const std::uint16_t* b, const float* bias, std::uint16_t* c,
+                                 const GatedArgs& args, hipStream_t stream);
+hipError_t gated_checkpoint_backward(const float* grad, float* grad_preactivations, float* hidden,
+                                     const GatedArgs& args, hipStream_t stream);
+hipError_t gated_checkpoint_backward(const std::uint16_t* grad, std::uint16_t* grad_preactivations,
+                                     std::uint16_t* hidden, const GatedArgs& args, hipStream_t stream);
 
 // packed_attention.hip and packed_backward.hip. Strides are resolved and checked:
 // whole 16-byte pieces, a token's at least a head's values.

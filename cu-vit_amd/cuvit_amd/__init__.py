@@ -33,6 +33,7 @@ __all__ = [
     "RotaryProblem", "QkNormProblem", "GatedProblem", "rotary_problem", "qk_norm_problem", "gated_problem",
     "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "qk_norm_rotary_workspace",
     "gated_gemm", "gated_backward",
+    "gated_checkpoint_gemm", "gated_checkpoint_backward", "gated_checkpoint_scales",
     "PackedAttentionProblem", "packed_attention_problem", "packed_attention", "packed_attention_workspace",
     "packed_attention_backward", "packed_attention_backward_workspace",
     "ROTARY_HALVES", "ROTARY_ADJACENT", "NORM_RMS", "NORM_LAYER",
@@ -311,6 +312,11 @@ _SIGNATURES = {
     "cuvit_gated_gemm_bf16": (_I, [_P, _P, _P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
     "cuvit_gated_backward_f32": (_I, [_P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
     "cuvit_gated_backward_bf16": (_I, [_P, _P, _P, ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_checkpoint_scales": (_L, [ctypes.POINTER(GatedProblem)]),
+    "cuvit_gated_checkpoint_gemm_f32": (_I, [_P] * 6 + [ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_checkpoint_gemm_bf16": (_I, [_P] * 6 + [ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_checkpoint_backward_f32": (_I, [_P] * 5 + [ctypes.POINTER(GatedProblem), _P]),
+    "cuvit_gated_checkpoint_backward_bf16": (_I, [_P] * 5 + [ctypes.POINTER(GatedProblem), _P]),
     "cuvit_packed_attention_problem_init": (None, [ctypes.POINTER(PackedAttentionProblem), _I, _I, _I, _I]),
     "cuvit_packed_attention_problem_projection": (None, [ctypes.POINTER(PackedAttentionProblem)]),
     "cuvit_packed_attention_workspace": (_L, [ctypes.POINTER(PackedAttentionProblem)]),
@@ -386,13 +392,16 @@ _NATIVE_FUNCTIONS = (
     "cuvit_gated_gemm_f32", "cuvit_gated_gemm_bf16", "cuvit_gated_backward_f32", "cuvit_gated_backward_bf16",
     "cuvit_packed_attention_f32", "cuvit_packed_attention_bf16", "cuvit_packed_attention_workspace",
     "cuvit_packed_attention_backward_f32", "cuvit_packed_attention_backward_bf16",
-    "cuvit_packed_attention_backward_workspace",
+    "cuvit_packed_attention_backward_workspace", "cuvit_gated_checkpoint_gemm_f32",
+    "cuvit_gated_checkpoint_gemm_bf16", "cuvit_gated_checkpoint_backward_f32",
+    "cuvit_gated_checkpoint_backward_bf16", "cuvit_gated_checkpoint_scales",
 )
 
 
 _NATIVE_CALLS = ("layer_norm", "softmax", "extract_patches", "gemm", "attention", "preprocess", "vit_forward",
                  "rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "gated_gemm", "gated_backward",
-                 "packed_attention", "packed_attention_backward")
+                 "packed_attention", "packed_attention_backward", "gated_checkpoint_gemm",
+                 "gated_checkpoint_backward")
 
 
 def _not_plain(*arguments) -> int:
@@ -480,7 +489,7 @@ def _ptr(x) -> Optional[int]:
 def _operand(x, name: str, dtype: str, elements: int) -> Optional[int]:
     """The address of operand @p x after checking that the kernel may touch
     @p elements of it: a torch tensor must live on the GPU, hold @p dtype
-    ("float32", "bfloat16" or "uint8"), be contiguous and have at least that
+    ("float32", "bfloat16", "uint8" and the like), be contiguous and have at least that
     many elements; anything else would be a device access outside the
     tensor or a host address read by the GPU. Raw int addresses and None go
     through unchecked, as in the C API (None becomes NULL, which the library
@@ -944,6 +953,67 @@ def gated_backward(preactivations, grad, grad_preactivations, problem: GatedProb
             grad = _operand(grad, "grad", t, reach[0])
             grad_preactivations = _operand(grad_preactivations, "grad_preactivations", t, reach[1])
     check(fn(_ptr(preactivations), _ptr(grad), _ptr(grad_preactivations), ctypes.byref(problem),
+             stream_handle(stream)))
+
+
+def gated_checkpoint_scales(problem: GatedProblem) -> int:
+    """How many scales a gated product's codes have: 2 ceil(n / 32) a row."""
+    return library().cuvit_gated_checkpoint_scales(ctypes.byref(problem))
+
+
+def gated_checkpoint_gemm(a, b, bias, c, codes, scales, problem: GatedProblem, stream=None,
+                          bf16: Optional[bool] = None) -> None:
+    """gated_gemm() that keeps [gate, value] in 8 bits, for
+    gated_checkpoint_backward(): ``codes`` [m, 2 n] float8_e4m3fn and ``scales``
+    [m, 2 ceil(n / 32)] float8_e8m0fnu, a power of two for every 32 columns of a
+    half. Values are rounded once, from their fp32 sums; infinities and NaN become
+    NaN. An extension."""
+    status = _native_calls.gated_checkpoint_gemm(a, b, bias, c, codes, scales, problem, stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(a)
+    fn = library().cuvit_gated_checkpoint_gemm_bf16 if bf16 else library().cuvit_gated_checkpoint_gemm_f32
+    p = problem
+    if _positive(p.m, p.n) and p.k >= 0:
+        _launch_device(stream, a, b, bias, c, codes, scales)
+        reach = _gated_reach(p)
+        lda, ldb = p.lda or p.k, p.ldb or p.k
+        if reach is not None and lda >= p.k and ldb >= p.k:
+            t = _storage(bf16)
+            a = _operand(a, "A", t, (p.m - 1) * lda + p.k)
+            b = _operand(b, "B", t, (2 * p.n - 1) * ldb + p.k)
+            bias = _operand(bias, "bias", "float32", 2 * p.n)
+            c = _operand(c, "C", t, reach[0])
+            codes = _operand(codes, "codes", "float8_e4m3fn", reach[1])
+            scales = _operand(scales, "scales", "float8_e8m0fnu", gated_checkpoint_scales(p))
+    check(fn(_ptr(a), _ptr(b), _ptr(bias), _ptr(c), _ptr(codes), _ptr(scales), ctypes.byref(problem),
+             stream_handle(stream)))
+
+
+def gated_checkpoint_backward(codes, scales, grad, grad_preactivations, problem: GatedProblem, hidden=None,
+                              stream=None, bf16: Optional[bool] = None) -> None:
+    """gated_backward() from the codes and scales that gated_checkpoint_gemm()
+    kept. A ``hidden`` tensor [m, n] receives activation(gate) * value again, as
+    the codes have them, for the gradient of the weight behind the product; it may
+    be ``grad``. An extension."""
+    status = _native_calls.gated_checkpoint_backward(codes, scales, grad, grad_preactivations, problem, hidden,
+                                                     stream, bf16)
+    if status >= 0:
+        return check(status)
+    bf16 = bf16 if bf16 is not None else _bf16(grad)
+    fn = library().cuvit_gated_checkpoint_backward_bf16 if bf16 else library().cuvit_gated_checkpoint_backward_f32
+    p = problem
+    if _positive(p.m, p.n):
+        _launch_device(stream, codes, scales, grad, grad_preactivations, hidden)
+        reach = _gated_reach(p)
+        if reach is not None:
+            t = _storage(bf16)
+            codes = _operand(codes, "codes", "float8_e4m3fn", reach[1])
+            scales = _operand(scales, "scales", "float8_e8m0fnu", gated_checkpoint_scales(p))
+            grad = _operand(grad, "grad", t, reach[0])
+            grad_preactivations = _operand(grad_preactivations, "grad_preactivations", t, reach[1])
+            hidden = _operand(hidden, "hidden", t, reach[0])
+    check(fn(_ptr(codes), _ptr(scales), _ptr(grad), _ptr(grad_preactivations), _ptr(hidden), ctypes.byref(problem),
              stream_handle(stream)))
 
 

@@ -321,6 +321,36 @@ int cuvit_gated_backward_bf16(const cuvit_bf16* preactivations, const cuvit_bf16
                               cuvit_bf16* grad_preactivations, const cuvit_gated_problem* problem,
                               cuvit_stream_t stream);
 
+/* The same with preactivations kept in 8 bits: codes [m, 2 n] in e4m3, rows
+ * ld_preactivations apart, and for every 32 columns of a half (from its first on,
+ * the last group of a half may be short) a scale in e8m0, the power of two
+ * 2^(scale - 127): scales is packed [m, 2 ceil(n / 32)], the gate's groups first,
+ * cuvit_gated_checkpoint_scales() bytes. A scale is the least from 2^-117 on that
+ * keeps its group's largest finite value within 448 of it; values are rounded once,
+ * to nearest-even, from their fp32 sums (by at most 2^-4 of them, or 2^-10 of the
+ * scale); infinities and NaN become NaN. C is the other product's, but for up to 64
+ * rows, where it may be summed in another order. */
+int64_t cuvit_gated_checkpoint_scales(const cuvit_gated_problem* problem);
+int cuvit_gated_checkpoint_gemm_f32(const float* a, const float* b, const float* bias, float* c,
+                                    uint8_t* codes, uint8_t* scales,
+                                    const cuvit_gated_problem* problem, cuvit_stream_t stream);
+int cuvit_gated_checkpoint_gemm_bf16(const cuvit_bf16* a, const cuvit_bf16* b, const float* bias,
+                                     cuvit_bf16* c, uint8_t* codes, uint8_t* scales,
+                                     const cuvit_gated_problem* problem, cuvit_stream_t stream);
+
+/* The gate's gradient from codes and scales: grad [m, n] and grad_preactivations as
+ * in cuvit_gated_backward_*. With hidden [m, n] (rows ldc apart) not null, the
+ * product that the codes stand for is stored too, for the gradient of the weight
+ * behind it; hidden == grad is allowed. */
+int cuvit_gated_checkpoint_backward_f32(const uint8_t* codes, const uint8_t* scales,
+                                        const float* grad, float* grad_preactivations,
+                                        float* hidden, const cuvit_gated_problem* problem,
+                                        cuvit_stream_t stream);
+int cuvit_gated_checkpoint_backward_bf16(const uint8_t* codes, const uint8_t* scales,
+                                         const cuvit_bf16* grad, cuvit_bf16* grad_preactivations,
+                                         cuvit_bf16* hidden, const cuvit_gated_problem* problem,
+                                         cuvit_stream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Attention over packed sequences: images and clips of different lengths one
  * behind the other, each attended within itself; extensions by the same rules.
