@@ -119,39 +119,83 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
     }
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void packed_attention_kernel(const T* __restrict__ q, const T* __restrict__ k,
-                                                                    const T* __restrict__ v, T* __restrict__ out,
-                                                                    float* __restrict__ lse, PackedArgs args,
-                                                                    int slots) {
+/// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
+/// the registers that the VALU reads, instead of moving logits and weights over.
+template <int D> constexpr int kShare = D <= 64 ? 3 : D <= 128 ? 2 : 1;
+
+/// How a workgroup's wavefronts divide its work: Shared of them take the same rows, each
+/// its own keys of every block, and add up at the end. One for tiles that fill the
+/// chip; four (two for the widest heads, whose blocks would not fit) for few rows.
+template <typename T, int D, bool Few> struct Division {
+    using R = Rows<T, D>;
+    static constexpr int kShared = !Few ? 1 : R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : 2;
+    static constexpr int kRows = R::kE * kWaves / kShared;                    // of a workgroup
+    static constexpr int kKeys = Few ? R::kE * kShared : kBlockRows<T, D>;    // of a block
+    static constexpr int kTiles = kKeys / R::kE / kShared;                    // of keys, a wavefront's
+    using Loads = Stage<T, D, kKeys>;
+    static constexpr int kLds = 4 * Loads::kBytes;
+    static_assert(kLds <= 128 * 1024, "two blocks of keys and values");
+    // The sums of the wavefronts that add up: accumulators, shift and sum of each lane.
+    static constexpr int kSums = R::kTiles * kRegisters<T> + 2;
+    static_assert(kWaves / kShared * (kShared - 1) * kSums * kWave * 4 <= kLds, "the blocks' LDS holds them");
+};
+
+/// A row's partial sums in the workspace: head_dim floats and the shift and the sum.
+__device__ __forceinline__ std::int64_t partial_at(const PackedArgs& args, std::int64_t row, int parts, int part) {
+    return (row * parts + part) * (args.head_dim + 2);
+}
+
+/// The result and log-sum-exp of a row from its sums, or false where they are of no use
+/// (see the top). @p largest is the largest size among the accumulators.
+__device__ __forceinline__ bool usable(int seen, float largest, float total) {
+    return seen == 0 || (largest < INFINITY && total > 0.F && total < INFINITY);
+}
+__device__ __forceinline__ float log_sum_exp(int seen, float total, float shift) {
+    return seen > 0 ? (__builtin_amdgcn_logf(total) - shift) * kLn2 : -INFINITY;
+}
+
+/// With @p Parts several workgroups take a tile, each its part of the keys, and leave
+/// partial sums for join_kernel.
+template <typename T, int D, bool Few, bool Parts>
+__global__ __launch_bounds__(kThreads, kShare<D>) void packed_attention_kernel(const T* __restrict__ q,
+                                                                               const T* __restrict__ k,
+                                                                               const T* __restrict__ v,
+                                                                               T* __restrict__ out,
+                                                                               float* __restrict__ lse,
+                                                                               float* __restrict__ partial,
+                                                                               PackedArgs args, int slots, int parts) {
     using R = Rows<T, D>;
     using Acc = typename Mma<T>::Acc;
+    using S = Division<T, D, Few>;
+    using Loads = typename S::Loads;
     constexpr int E = R::kE;
-    constexpr int K = kBlockRows<T, D>;
-    constexpr int kTile = E * kWaves; // rows of a workgroup
-    using Loads = Stage<T, D, K>;
+    constexpr int K = S::kKeys;
     extern __shared__ Vec16 lds_vectors[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
-    const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
+    const int part = Parts ? static_cast<int>(blockIdx.x % static_cast<unsigned int>(parts)) : 0;
+    const Item item = item_of(Parts ? blockIdx.x / static_cast<unsigned int>(parts) : blockIdx.x, slots, args.kv_heads,
+                              args.causal);
     if (item.head < 0) {
         return; // the whole workgroup, before any barrier (so below)
     }
-    const Spot spot = find(args.starts, args.sequences, args.tokens, args.group, kTile, item.slot);
+    const Spot spot = find(args.starts, args.sequences, args.tokens, args.group, S::kRows, item.slot);
     if (spot.sequence < 0) {
         return;
     }
     const Span span = span_of(args, spot.sequence);
     const int rows = span.queries * args.group;
-    const int first_row = spot.tile * kTile;
-    if (first_row >= rows) {
+    const int tile_row = spot.tile * S::kRows;
+    if (tile_row >= rows) {
         return;
     }
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int share = wave % S::kShared; // which keys of a block are this wavefront's
+    const int first_row = tile_row + wave / S::kShared * E;
     const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
 
     // The lane's row, and the keys that it, its wavefront and the workgroup see.
-    const int row = first_row + wave * E + lane % E;
+    const int row = first_row + lane % E;
     const bool there = row < rows;
     const int query = row / args.group;
     const int head = item.head * args.group + row % args.group;
@@ -160,14 +204,20 @@ __global__ __launch_bounds__(kThreads) void packed_attention_kernel(const T* __r
         return args.causal ? min(max(min(r, rows - 1) / args.group + 1 + behind, 0), span.keys) : span.keys;
     };
     const int seen = there ? sees(row) : 0;
-    const int wave_least = __builtin_amdgcn_readfirstlane(sees(first_row + wave * E));
-    const int wave_most = first_row + wave * E < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + wave * E + E - 1)) : 0;
-    const int most = __builtin_amdgcn_readfirstlane(sees(first_row + kTile - 1));
+    const int wave_least = __builtin_amdgcn_readfirstlane(sees(first_row));
+    const int wave_most = first_row < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + E - 1)) : 0;
+    int most = __builtin_amdgcn_readfirstlane(sees(tile_row + S::kRows - 1));
+    int start = 0;
+    if constexpr (Parts) {
+        const int blocks = (most + K - 1) / K;
+        const int of_part = (blocks + parts - 1) / parts;
+        start = min(part * of_part * K, most);
+        most = min(start + of_part * K, most);
+    }
 
     const T* const k_head = k + span.first_key * args.k.token + item.head * args.k.head;
     const T* const v_head = v + span.first_key * args.v.token + item.head * args.v.head;
-    const T* const q_row = there ? q + (static_cast<std::int64_t>(span.first_query) + query) * args.q.token + head * args.q.head
-                                 : nullptr;
+    const std::int64_t token = static_cast<std::int64_t>(span.first_query) + query;
     const Loads k_loads(k_head, args.k.token, args.head_dim, wave, lane);
     const Loads v_loads(v_head, args.v.token, args.head_dim, wave, lane);
     auto issue = [&](int first, int buffer) {
@@ -175,11 +225,11 @@ __global__ __launch_bounds__(kThreads) void packed_attention_kernel(const T* __r
         k_loads.issue(first, span.keys - first, to, wave);
         v_loads.issue(first, span.keys - first, to + Loads::kBytes, wave);
     };
-    if (most > 0) {
-        issue(0, 0);
+    if (start < most) {
+        issue(start, 0);
     }
     Vec16 qf[R::kBlocks];
-    load_rows<T, D>(q_row, args.head_dim, lane, qf);
+    load_rows<T, D>(there ? q + token * args.q.token + head * args.q.head : nullptr, args.head_dim, lane, qf);
 
     Running running{args.scale * kLog2e};
     Acc acc[R::kTiles];
@@ -188,46 +238,81 @@ __global__ __launch_bounds__(kThreads) void packed_attention_kernel(const T* __r
         acc[t] = Acc{};
     }
     int buffer = 0;
-    for (int first = 0; first < most; first += K) {
+    for (int block = start; block < most; block += K) {
         landed(); // and every wavefront is done with the other buffer
-        if (first + K < most) {
-            issue(first + K, buffer ^ 1);
+        if (block + K < most) {
+            issue(block + K, buffer ^ 1);
         }
-        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes;
+        const int first = block + share * E; // this wavefront's first key
+        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes + share * E * R::kPitch;
         const unsigned char* const values = keys + Loads::kBytes;
         buffer ^= 1;
         if (first >= wave_most) {
             continue;
         }
-        Acc x[K / E];
-#pragma unroll
-        for (int t = 0; t < K / E; ++t) {
-            x[t] = Acc{};
+        // Fragments are read a tile ahead of their MFMAs, the first values' behind the
+        // last keys', so that their latency lies under the softmax; where the registers
+        // do not hold them, as they are needed.
+        constexpr bool kAhead = D <= 96 || (D == 128 && sizeof(T) == 2 && !Parts);
+        Vec16 kf[kAhead ? 2 : 1][R::kBlocks], vf[kAhead ? 2 : 1][kParts<T>][R::kTiles];
+        auto read_keys = [&](int t) {
 #pragma unroll
             for (int b = 0; b < R::kBlocks; ++b) {
-                Mma<T>::run(x[t], R::along(keys, t * E + lane % E, b, lane), qf[b]);
+                kf[t % 2][b] = R::along(keys, t * E + lane % E, b, lane);
+            }
+        };
+        auto read_values = [&](int t) {
+#pragma unroll
+            for (int p = 0; p < kParts<T>; ++p) {
+#pragma unroll
+                for (int d = 0; d < R::kTiles; ++d) {
+                    vf[t % 2][p][d] = R::across(values, t * E + 16 * p, d, lane);
+                }
+            }
+        };
+        Acc x[S::kTiles];
+        if constexpr (kAhead) {
+            read_keys(0);
+        }
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t) {
+            x[t] = Acc{};
+            if constexpr (kAhead) {
+                if (t + 1 < S::kTiles) {
+                    read_keys(t + 1);
+                } else {
+                    read_values(0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int b = 0; b < R::kBlocks; ++b) {
+                Mma<T>::run(x[t], kAhead ? kf[t % 2][b] : R::along(keys, t * E + lane % E, b, lane), qf[b]);
+            }
+            if constexpr (kAhead) {
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (first + K > wave_least) {
+        if (block + K > wave_least) {
 #pragma unroll
-            for (int t = 0; t < K / E; ++t) {
+            for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
                 for (int i = 0; i < kRegisters<T>; ++i) {
                     x[t][i] = first + t * E + row_of<T>(lane, i) < seen ? x[t][i] : -INFINITY;
                 }
             }
         }
-        float block = -INFINITY;
+        float largest = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < K / E; ++t) {
+        for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
             for (int i = 0; i < kRegisters<T>; ++i) {
-                block = fmaxf(block, x[t][i]);
+                largest = fmaxf(largest, x[t][i]);
             }
         }
-        block = combine_column<T>(block, Max{});
+        largest = combine_column<T>(largest, Max{});
         float factor = 1.0F;
-        if (running.raise(block, factor)) {
+        if (running.raise(largest, factor)) {
 #pragma unroll
             for (int t = 0; t < R::kTiles; ++t) {
 #pragma unroll
@@ -236,28 +321,101 @@ __global__ __launch_bounds__(kThreads) void packed_attention_kernel(const T* __r
                 }
             }
         }
+        float sums[4] = {0.F, 0.F, 0.F, 0.F};
 #pragma unroll
-        for (int t = 0; t < K / E; ++t) {
+        for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
             for (int i = 0; i < kRegisters<T>; ++i) {
                 x[t][i] = running.weight(x[t][i]);
-                running.sum += x[t][i];
+                sums[i % 4] += x[t][i];
             }
         }
+        running.sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
-        for (int t = 0; t < K / E; ++t) {
+        for (int t = 0; t < S::kTiles; ++t) {
+            if constexpr (kAhead) {
+                if (t + 1 < S::kTiles) {
+                    read_values(t + 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int p = 0; p < kParts<T>; ++p) {
                 const Vec16 weights = weights_of<T>(x[t], p);
 #pragma unroll
                 for (int d = 0; d < R::kTiles; ++d) {
-                    Mma<T>::run(acc[d], R::across(values, t * E + 16 * p, d, lane), weights);
+                    Mma<T>::run(acc[d], kAhead ? vf[t % 2][p][d] : R::across(values, t * E + 16 * p, d, lane), weights);
                 }
+            }
+            if constexpr (kAhead) {
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
 
-    const float total = combine_column<T>(running.sum, Sum{});
+    float total = combine_column<T>(running.sum, Sum{});
+    if constexpr (S::kShared > 1) {
+        // The others' sums through LDS, each scaled to the larger maximum, in turn.
+        __syncthreads();
+        float* const sums = reinterpret_cast<float*>(lds) + wave / S::kShared * (S::kShared - 1) * S::kSums * kWave + lane;
+        if (share > 0) {
+            float* const to = sums + (share - 1) * S::kSums * kWave;
+#pragma unroll
+            for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    to[(t * kRegisters<T> + i) * kWave] = acc[t][i];
+                }
+            }
+            to[(S::kSums - 2) * kWave] = running.maximum == -INFINITY ? INFINITY : running.shift;
+            to[(S::kSums - 1) * kWave] = total;
+        }
+        __syncthreads();
+        if (share > 0) {
+            return;
+        }
+        float shift = running.maximum == -INFINITY ? INFINITY : running.shift;
+#pragma unroll
+        for (int o = 0; o < S::kShared - 1; ++o) {
+            const float* const from = sums + o * S::kSums * kWave;
+            const float other = from[(S::kSums - 2) * kWave];
+            const float common = fminf(shift, other);
+            // (No logit above -infinity yet: the shift is infinity, its sums 0.)
+            const float mine = shift == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - shift);
+            const float theirs = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - other);
+            total = total * mine + from[(S::kSums - 1) * kWave] * theirs;
+#pragma unroll
+            for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    acc[t][i] = acc[t][i] * mine + from[(t * kRegisters<T> + i) * kWave] * theirs;
+                }
+            }
+            shift = common;
+        }
+        running.shift = shift;
+        running.maximum = shift == INFINITY ? -INFINITY : 0.F;
+    }
+    if constexpr (Parts) {
+        if (there) {
+            float* const to = partial + partial_at(args, token * args.heads + head, parts, part);
+#pragma unroll
+            for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    const int dim = t * E + row_of<T>(lane, i);
+                    if (dim < args.head_dim) {
+                        to[dim] = acc[t][i];
+                    }
+                }
+            }
+            if (lane < E) {
+                to[args.head_dim] = running.maximum == -INFINITY ? INFINITY : running.shift;
+                to[args.head_dim + 1] = total;
+            }
+        }
+        return;
+    }
     float largest = 0.F;
 #pragma unroll
     for (int t = 0; t < R::kTiles; ++t) {
@@ -266,66 +424,193 @@ __global__ __launch_bounds__(kThreads) void packed_attention_kernel(const T* __r
             largest = __builtin_elementwise_maximum(largest, fabsf(acc[t][i]));
         }
     }
-    const bool usable = seen == 0 || (largest < INFINITY && total > 0.F && total < INFINITY);
-    std::uint64_t bad = __ballot(there && !usable);
-    T* const to = out + (static_cast<std::int64_t>(span.first_query) + query) * args.out.token + head * args.out.head;
-    float* const lse_to =
-        lse != nullptr ? lse + (static_cast<std::int64_t>(span.first_query) + query) * args.heads + head : nullptr;
+    std::uint64_t bad = __ballot(there && !usable(seen, largest, total));
     for (int half = 32; half >= E; half /= 2) { // any of a row's lanes
         bad |= bad >> half;
     }
     if (there && (bad >> (lane % E) & 1U) == 0) {
-        store_row<T, D>(to, acc, seen > 0 ? 1.0F / total : 0.F, args.head_dim, lane);
-        if (lse_to != nullptr && lane < E) {
-            *lse_to = seen > 0 ? (__builtin_amdgcn_logf(total) - running.shift) * kLn2 : -INFINITY;
+        store_row<T, D>(out + token * args.out.token + head * args.out.head, acc, seen > 0 ? 1.0F / total : 0.F,
+                        args.head_dim, lane);
+        if (lse != nullptr && lane < E) {
+            lse[token * args.heads + head] = log_sum_exp(seen, total, running.shift);
         }
     }
     bad &= E == 32 ? 0xFFFFFFFFU : 0xFFFFU;
     for (; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
-        const int r = first_row + wave * E + __builtin_ctzll(bad);
+        const int r = first_row + __builtin_ctzll(bad);
         const int h = item.head * args.group + r % args.group;
-        const std::int64_t token = static_cast<std::int64_t>(span.first_query) + r / args.group;
-        attend_alone<T>(q + token * args.q.token + h * args.q.head, k_head, v_head,
-                        out + token * args.out.token + h * args.out.head,
-                        lse != nullptr ? lse + token * args.heads + h : nullptr, sees(r), args.k.token, args.v.token,
-                        args.head_dim, running.c);
+        const std::int64_t at = static_cast<std::int64_t>(span.first_query) + r / args.group;
+        attend_alone<T>(q + at * args.q.token + h * args.q.head, k_head, v_head,
+                        out + at * args.out.token + h * args.out.head, lse != nullptr ? lse + at * args.heads + h : nullptr,
+                        sees(r), args.k.token, args.v.token, args.head_dim, running.c);
     }
 }
 
+/// Adds up a row's parts in their order, a wavefront a row at a time.
+template <typename T, int Tile>
+__global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                        const T* __restrict__ v, T* __restrict__ out,
+                                                        float* __restrict__ lse, const float* __restrict__ partial,
+                                                        PackedArgs args, int slots, int parts) {
+    const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
+    if (item.head < 0) {
+        return;
+    }
+    const Spot spot = find(args.starts, args.sequences, args.tokens, args.group, Tile, item.slot);
+    if (spot.sequence < 0) {
+        return;
+    }
+    const Span span = span_of(args, spot.sequence);
+    const int rows = span.queries * args.group;
+    const int lane = lane_id();
+    const int last = min(rows, spot.tile * Tile + Tile);
+    const float c = args.scale * kLog2e;
+    for (int row = spot.tile * Tile + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave); row < last;
+         row += kWaves) {
+        const int query = row / args.group;
+        const int head = item.head * args.group + row % args.group;
+        const std::int64_t token = static_cast<std::int64_t>(span.first_query) + query;
+        const int seen = args.causal ? min(max(query + 1 + span.keys - span.queries, 0), span.keys) : span.keys;
+        const float* const from = partial + partial_at(args, token * args.heads + head, parts, 0);
+        const int step = args.head_dim + 2;
+        float shift = INFINITY;
+        for (int p = lane; p < parts; p += kWave) {
+            shift = fminf(shift, from[p * step + args.head_dim]);
+        }
+        shift = -wave_allreduce(-shift, Max{});
+        float total = 0.F;
+        float value[4] = {0.F, 0.F, 0.F, 0.F};
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            const float* const at = from + p * step;
+            const float other = at[args.head_dim];
+            const float factor = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(shift - other);
+            total += at[args.head_dim + 1] * factor;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (lane + kWave * i < args.head_dim) {
+                    value[i] += at[lane + kWave * i] * factor;
+                }
+            }
+        }
+        float largest = 0.F;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            largest = __builtin_elementwise_maximum(largest, fabsf(value[i]));
+        }
+        T* const to = out + token * args.out.token + head * args.out.head;
+        float* const lse_to = lse != nullptr ? lse + token * args.heads + head : nullptr;
+        if (__builtin_expect(__any(!usable(seen, largest, total)), 0)) {
+            attend_alone<T>(q + token * args.q.token + head * args.q.head,
+                            k + span.first_key * args.k.token + item.head * args.k.head,
+                            v + span.first_key * args.v.token + item.head * args.v.head, to, lse_to, seen, args.k.token,
+                            args.v.token, args.head_dim, c);
+            continue;
+        }
+        const float inverse = seen > 0 ? 1.0F / total : 0.F;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (lane + kWave * i < args.head_dim) {
+                Elem<T>::store(to + lane + kWave * i, value[i] * inverse);
+            }
+        }
+        if (lse_to != nullptr && lane == 0) {
+            *lse_to = log_sum_exp(seen, total, shift);
+        }
+    }
+}
+
+/// How a call is divided, by its sizes alone: whole tiles of 128 (64) rows to a
+/// workgroup, or of 32 (16) where those would leave CUs without one, and then as many
+/// parts of the keys as fill the chip twice, of two blocks or more on average.
+struct Plan {
+    bool few;
+    int parts;
+};
+
+template <typename T, int D> Plan plan(const PackedArgs& args) {
+    using Few = Division<T, D, true>;
+    const std::int64_t units = compute_units();
+    const std::int64_t whole = slots(args.tokens, args.group, Division<T, D, false>::kRows, args.sequences) * args.kv_heads;
+    if (whole >= units) {
+        return {false, 1};
+    }
+    const std::int64_t tiles = slots(args.tokens, args.group, Few::kRows, args.sequences) * args.kv_heads;
+    const std::int64_t blocks = args.kv_tokens / args.sequences / (2 * Few::kKeys);
+    const std::int64_t wanted = 2 * units / tiles;
+    const std::int64_t parts = wanted < blocks ? wanted : blocks;
+    return {true, static_cast<int>(parts > 1 ? parts : 1)};
+}
+
 template <typename T>
-hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, const PackedArgs& args, hipStream_t stream) {
+hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, float* workspace, const PackedArgs& args,
+                  hipStream_t stream) {
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
-        constexpr int kTile = Mma<T>::kEdge * kWaves;
-        constexpr std::size_t kLds = 4 * Stage<T, D, kBlockRows<T, D>>::kBytes;
-        constexpr auto kernel = packed_attention_kernel<T, D>;
-        const std::int64_t tiles = slots(args.tokens, args.group, kTile, args.sequences);
-        const std::int64_t blocks = items(tiles, args.kv_heads);
-        if (!launchable(blocks, kThreads)) {
-            return hipErrorInvalidConfiguration;
+        const Plan chosen = plan<T, D>(args);
+        auto run = [&](auto kernel_constant, int rows, std::size_t lds) -> hipError_t {
+            constexpr auto kernel = decltype(kernel_constant)::kValue;
+            const std::int64_t tiles = slots(args.tokens, args.group, rows, args.sequences);
+            const std::int64_t blocks = items(tiles, args.kv_heads) * chosen.parts;
+            if (!launchable(blocks, kThreads)) {
+                return hipErrorInvalidConfiguration;
+            }
+            if (const hipError_t opted = allow_lds<kernel>(lds); opted != hipSuccess) {
+                return opted;
+            }
+            kernel<<<static_cast<unsigned int>(blocks), kThreads, lds, stream>>>(
+                q, k, v, out, lse, workspace, args, static_cast<int>(tiles), chosen.parts);
+            return hipGetLastError();
+        };
+        using Whole = Division<T, D, false>;
+        using Few = Division<T, D, true>;
+        if (!chosen.few) {
+            return run(KernelConstant<packed_attention_kernel<T, D, false, false>>{}, Whole::kRows, Whole::kLds);
         }
-        if (const hipError_t opted = allow_lds<kernel>(kLds); opted != hipSuccess) {
-            return opted;
+        if (chosen.parts == 1) {
+            return run(KernelConstant<packed_attention_kernel<T, D, true, false>>{}, Few::kRows, Few::kLds);
         }
-        kernel<<<static_cast<unsigned int>(blocks), kThreads, kLds, stream>>>(q, k, v, out, lse, args,
-                                                                             static_cast<int>(tiles));
+        if (const hipError_t result = run(KernelConstant<packed_attention_kernel<T, D, true, true>>{}, Few::kRows, Few::kLds);
+            result != hipSuccess) {
+            return result;
+        }
+        const std::int64_t tiles = slots(args.tokens, args.group, Few::kRows, args.sequences);
+        join_kernel<T, Few::kRows><<<static_cast<unsigned int>(items(tiles, args.kv_heads)), kThreads, 0, stream>>>(
+            q, k, v, out, lse, workspace, args, static_cast<int>(tiles), chosen.parts);
         return hipGetLastError();
     });
+}
+
+template <typename T> std::int64_t workspace_of(const PackedArgs& args) {
+    std::int64_t bytes = 0;
+    (void)with_width(args.head_dim, [&](auto width) -> hipError_t {
+        const Plan chosen = plan<T, decltype(width)::value>(args);
+        if (chosen.parts > 1) {
+            bytes = static_cast<std::int64_t>(args.tokens) * args.heads * chosen.parts * (args.head_dim + 2) *
+                    static_cast<std::int64_t>(sizeof(float));
+        }
+        return hipSuccess;
+    });
+    return bytes;
 }
 
 } // namespace
 } // namespace packed
 
-hipError_t packed_attention(const float* q, const float* k, const float* v, float* out, float* lse, void*,
+hipError_t packed_attention(const float* q, const float* k, const float* v, float* out, float* lse, void* workspace,
                             const PackedArgs& args, hipStream_t stream) {
-    return packed::launch(q, k, v, out, lse, args, stream);
+    return packed::launch(q, k, v, out, lse, static_cast<float*>(workspace), args, stream);
 }
 
 hipError_t packed_attention(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v, std::uint16_t* out,
-                            float* lse, void*, const PackedArgs& args, hipStream_t stream) {
-    return packed::launch(q, k, v, out, lse, args, stream);
+                            float* lse, void* workspace, const PackedArgs& args, hipStream_t stream) {
+    return packed::launch(q, k, v, out, lse, static_cast<float*>(workspace), args, stream);
 }
 
-std::int64_t packed_attention_workspace(const PackedArgs&) { return 0; }
+std::int64_t packed_attention_workspace(const PackedArgs& args) {
+    const std::int64_t single = packed::workspace_of<float>(args);
+    const std::int64_t half = packed::workspace_of<std::uint16_t>(args);
+    return single > half ? single : half;
+}
 
 } // namespace cuvit::detail

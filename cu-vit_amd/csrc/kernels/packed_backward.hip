@@ -15,8 +15,12 @@ namespace cuvit::detail {
 namespace packed {
 namespace {
 
+/// Wavefronts that share a SIMD (packed_attention.hip).
+template <int D> constexpr int kShareQueries = D <= 128 ? 2 : 1;
+template <int D> constexpr int kShareKeys = D <= 64 ? 2 : 1;
+
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void query_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
+__global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                   const T* __restrict__ v,
                                                                   PackedGradients<T> gradients, PackedArgs args,
                                                                   int slots) {
@@ -148,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void query_gradient_kernel(const T* __res
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void key_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
+__global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                 const T* __restrict__ v, PackedGradients<T> gradients,
                                                                 PackedArgs args, int slots) {
     using R = Rows<T, D>;
