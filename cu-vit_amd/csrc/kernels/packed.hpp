@@ -111,19 +111,13 @@ struct Item {
     int slot;
 };
 
-__device__ __forceinline__ Item item_of(std::int64_t block, int slots, int heads, bool uneven) {
-    const std::uint32_t total = static_cast<std::uint32_t>(slots) * static_cast<std::uint32_t>(heads);
-    const std::uint32_t share = (total + 7) / 8;
-    const std::uint32_t at = static_cast<std::uint32_t>(block % 8) * share + static_cast<std::uint32_t>(block / 8);
-    if (static_cast<std::uint32_t>(block / 8) >= share || at >= total) {
+__device__ __forceinline__ Item item_of(std::uint32_t block, int slots, int heads, bool uneven) {
+    const int slot = static_cast<int>(block / static_cast<std::uint32_t>(heads));
+    const int head = static_cast<int>(block) - slot * heads;
+    if (slot >= slots) {
         return {-1, 0};
     }
-    const int head = static_cast<int>(at / static_cast<std::uint32_t>(slots));
-    int slot = static_cast<int>(at) - head * slots;
-    if (uneven) {
-        slot = (slot & 1) != 0 ? slot / 2 : slots - 1 - slot / 2;
-    }
-    return {head, slot};
+    return {head, uneven ? slots - 1 - slot : slot};
 }
 
 /// Workgroups that item_of() needs.
@@ -227,14 +221,14 @@ template <typename T, typename Op> __device__ __forceinline__ float combine_colu
 }
 
 /// Loads of @p Count consecutive rows (a token's stride apart) of one head into a
-/// tile, by all wavefronts of the workgroup: each brings Count * kPitch / 4096 pieces of
-/// 1024 bytes. Rows past the last and values past head_dim read as zeros.
-template <typename T, int D, int Count> struct Stage {
+/// tile, by all @p Waves wavefronts of the workgroup, 1024 bytes a load. Rows past the
+/// last and values past head_dim read as zeros.
+template <typename T, int D, int Count, int Waves = kWaves> struct Stage {
     using R = Rows<T, D>;
     static constexpr int kBytes = Count * R::kPitch;
     static constexpr int kRowsOfPiece = 1024 / R::kPitch;
-    static constexpr int kLoads = kBytes / 1024 / kWaves;
-    static_assert(kBytes % (1024 * kWaves) == 0, "whole pieces for every wavefront");
+    static constexpr int kLoads = kBytes / 1024 / Waves;
+    static_assert(kBytes % (1024 * Waves) == 0, "whole pieces for every wavefront");
 
     const T* base; // of the head, at the sequence's first row
     std::int64_t token;
@@ -245,7 +239,7 @@ template <typename T, int D, int Count> struct Stage {
         : base(base_), token(token_), head_dim(head_dim_) {
 #pragma unroll
         for (int p = 0; p < kLoads; ++p) {
-            const int row = (p * kWaves + wave) * kRowsOfPiece + lane / R::kSlots;
+            const int row = (p * Waves + wave) * kRowsOfPiece + lane / R::kSlots;
             const int piece = lane % R::kSlots ^ R::turned(row);
             offset[p] = piece * R::kV < head_dim
                             ? static_cast<unsigned int>(row * static_cast<int>(token) * static_cast<int>(sizeof(T)) + piece * 16)
@@ -261,7 +255,7 @@ template <typename T, int D, int Count> struct Stage {
                                                                           static_cast<int>(sizeof(T))));
 #pragma unroll
         for (int p = 0; p < kLoads; ++p) {
-            load_to_lds(lds + static_cast<unsigned int>((p * kWaves + wave) * 1024), offset[p], resource);
+            load_to_lds(lds + static_cast<unsigned int>((p * Waves + wave) * 1024), offset[p], resource);
         }
     }
 };

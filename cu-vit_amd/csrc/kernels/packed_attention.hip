@@ -26,7 +26,7 @@ constexpr float kHeadroom = 8.0F;
 
 /// The running maximum and sum of a lane's row; shift is -(maximum c).
 struct Running {
-    float c;
+    float c = 0.F;
     float maximum = -INFINITY;
     float shift = 0.F;
     float sum = 0.F;
@@ -119,25 +119,32 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
     }
 }
 
-/// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
-/// the registers that the VALU reads, instead of moving logits and weights over.
-template <int D> constexpr int kShare = D <= 64 ? 3 : D <= 128 ? 2 : 1;
+/// How a workgroup's four wavefronts divide its work: kShared of them take the same
+/// rows, each its own keys of every block, and add up at the end, which shortens a
+/// tile's walk (a call's time where tiles are few or uneven). kLarge: 128 rows in bf16,
+/// two tiles of them a wavefront, whose MFMAs share each fragment read from LDS; kMiddle
+/// half as many; kFew one tile for all four (for two of the widest heads, whose blocks
+/// would not fit otherwise).
+enum class Kind { kFew, kMiddle, kLarge };
 
-/// How a workgroup's wavefronts divide its work: Shared of them take the same rows, each
-/// its own keys of every block, and add up at the end. One for tiles that fill the
-/// chip; four (two for the widest heads, whose blocks would not fit) for few rows.
-template <typename T, int D, bool Few> struct Division {
+template <typename T, int D, Kind Way> struct Division {
     using R = Rows<T, D>;
-    static constexpr int kShared = !Few ? 1 : R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : 2;
-    static constexpr int kRows = R::kE * kWaves / kShared;                    // of a workgroup
-    static constexpr int kKeys = Few ? R::kE * kShared : kBlockRows<T, D>;    // of a block
-    static constexpr int kTiles = kKeys / R::kE / kShared;                    // of keys, a wavefront's
+    static constexpr bool kFew = Way == Kind::kFew;
+    static constexpr int kShared = kFew && R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : (Way == Kind::kLarge && R::kTiles * R::kE > 128 ? 1 : 2);
+    static constexpr int kM = Way == Kind::kLarge && sizeof(T) == 2 && D <= 96 ? 2 : 1; // tiles of rows, a wavefront's
+    static constexpr int kRows = R::kE * kM * kWaves / kShared;                 // of a workgroup
+    static constexpr int kKeys = !kFew && kBlockRows<T, D> > R::kE * kShared ? kBlockRows<T, D> : R::kE * kShared; // of a block
+    static constexpr int kTiles = kKeys / R::kE / kShared;                     // of keys, a wavefront's
+    static constexpr int kStep = kM > 1 && D > 64 ? 1 : kTiles;                // of them to a softmax
+    /// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
+    /// the registers that the VALU reads, instead of moving logits and weights over.
+    static constexpr int kShare = D > 128 ? 1 : D > 64 || kM > 1 ? 2 : 3;
     using Loads = Stage<T, D, kKeys>;
-    static constexpr int kLds = 4 * Loads::kBytes;
-    static_assert(kLds <= 128 * 1024, "two blocks of keys and values");
     // The sums of the wavefronts that add up: accumulators, shift and sum of each lane.
-    static constexpr int kSums = R::kTiles * kRegisters<T> + 2;
-    static_assert(kWaves / kShared * (kShared - 1) * kSums * kWave * 4 <= kLds, "the blocks' LDS holds them");
+    static constexpr int kSums = kM * (R::kTiles * kRegisters<T> + 2);
+    static constexpr int kExchange = kWaves / kShared * (kShared - 1) * kSums * kWave * 4;
+    static constexpr int kLds = 4 * Loads::kBytes > kExchange ? 4 * Loads::kBytes : kExchange;
+    static_assert(kLds <= 128 * 1024, "two blocks of keys and values, or the sums");
 };
 
 /// A row's partial sums in the workspace: head_dim floats and the shift and the sum.
@@ -156,20 +163,21 @@ __device__ __forceinline__ float log_sum_exp(int seen, float total, float shift)
 
 /// With @p Parts several workgroups take a tile, each its part of the keys, and leave
 /// partial sums for join_kernel.
-template <typename T, int D, bool Few, bool Parts>
-__global__ __launch_bounds__(kThreads, kShare<D>) void packed_attention_kernel(const T* __restrict__ q,
-                                                                               const T* __restrict__ k,
-                                                                               const T* __restrict__ v,
-                                                                               T* __restrict__ out,
-                                                                               float* __restrict__ lse,
-                                                                               float* __restrict__ partial,
-                                                                               PackedArgs args, int slots, int parts) {
+template <typename T, int D, typename S, bool Parts>
+__global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(const T* __restrict__ q,
+                                                                                  const T* __restrict__ k,
+                                                                                  const T* __restrict__ v,
+                                                                                  T* __restrict__ out,
+                                                                                  float* __restrict__ lse,
+                                                                                  float* __restrict__ partial,
+                                                                                  PackedArgs args, int slots,
+                                                                                  int parts) {
     using R = Rows<T, D>;
     using Acc = typename Mma<T>::Acc;
-    using S = Division<T, D, Few>;
     using Loads = typename S::Loads;
     constexpr int E = R::kE;
     constexpr int K = S::kKeys;
+    constexpr int M = S::kM;
     extern __shared__ Vec16 lds_vectors[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
     const int part = Parts ? static_cast<int>(blockIdx.x % static_cast<unsigned int>(parts)) : 0;
@@ -191,21 +199,22 @@ __global__ __launch_bounds__(kThreads, kShare<D>) void packed_attention_kernel(c
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int share = wave % S::kShared; // which keys of a block are this wavefront's
-    const int first_row = tile_row + wave / S::kShared * E;
+    const int first_row = tile_row + wave / S::kShared * E * M;
     const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
 
-    // The lane's row, and the keys that it, its wavefront and the workgroup see.
-    const int row = first_row + lane % E;
-    const bool there = row < rows;
-    const int query = row / args.group;
-    const int head = item.head * args.group + row % args.group;
+    // The keys that the lane's rows (one of each tile), the wavefront and the workgroup see.
     const int behind = span.keys - span.queries;
     const auto sees = [&](int r) {
         return args.causal ? min(max(min(r, rows - 1) / args.group + 1 + behind, 0), span.keys) : span.keys;
     };
-    const int seen = there ? sees(row) : 0;
+    int seen[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        const int row = first_row + m * E + lane % E;
+        seen[m] = row < rows ? sees(row) : 0;
+    }
     const int wave_least = __builtin_amdgcn_readfirstlane(sees(first_row));
-    const int wave_most = first_row < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + E - 1)) : 0;
+    const int wave_most = first_row < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + E * M - 1)) : 0;
     int most = __builtin_amdgcn_readfirstlane(sees(tile_row + S::kRows - 1));
     int start = 0;
     if constexpr (Parts) {
@@ -217,7 +226,6 @@ __global__ __launch_bounds__(kThreads, kShare<D>) void packed_attention_kernel(c
 
     const T* const k_head = k + span.first_key * args.k.token + item.head * args.k.head;
     const T* const v_head = v + span.first_key * args.v.token + item.head * args.v.head;
-    const std::int64_t token = static_cast<std::int64_t>(span.first_query) + query;
     const Loads k_loads(k_head, args.k.token, args.head_dim, wave, lane);
     const Loads v_loads(v_head, args.v.token, args.head_dim, wave, lane);
     auto issue = [&](int first, int buffer) {
@@ -228,14 +236,35 @@ __global__ __launch_bounds__(kThreads, kShare<D>) void packed_attention_kernel(c
     if (start < most) {
         issue(start, 0);
     }
-    Vec16 qf[R::kBlocks];
-    load_rows<T, D>(there ? q + token * args.q.token + head * args.q.head : nullptr, args.head_dim, lane, qf);
-
-    Running running{args.scale * kLog2e};
-    Acc acc[R::kTiles];
+    /// A row's token and query head.
+    struct Place {
+        std::int64_t token;
+        int head;
+    };
+    const auto place_of = [&](int row) {
+        const int query = row / args.group;
+        return Place{static_cast<std::int64_t>(span.first_query) + query,
+                     item.head * args.group + row - query * args.group};
+    };
+    Vec16 qf[M][R::kBlocks];
 #pragma unroll
-    for (int t = 0; t < R::kTiles; ++t) {
-        acc[t] = Acc{};
+    for (int m = 0; m < M; ++m) {
+        const int row = first_row + m * E + lane % E;
+        const Place at = place_of(row);
+        load_rows<T, D>(row < rows ? q + at.token * args.q.token + at.head * args.q.head : nullptr, args.head_dim, lane,
+                        qf[m]);
+    }
+
+    const float c = args.scale * kLog2e;
+    Running running[M];
+    Acc acc[M][R::kTiles];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        running[m].c = c;
+#pragma unroll
+        for (int t = 0; t < R::kTiles; ++t) {
+            acc[m][t] = Acc{};
+        }
     }
     int buffer = 0;
     for (int block = start; block < most; block += K) {
@@ -243,206 +272,251 @@ __global__ __launch_bounds__(kThreads, kShare<D>) void packed_attention_kernel(c
         if (block + K < most) {
             issue(block + K, buffer ^ 1);
         }
-        const int first = block + share * E; // this wavefront's first key
-        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes + share * E * R::kPitch;
+        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes + share * S::kTiles * E * R::kPitch;
         const unsigned char* const values = keys + Loads::kBytes;
         buffer ^= 1;
-        if (first >= wave_most) {
-            continue;
-        }
-        // Fragments are read a tile ahead of their MFMAs, the first values' behind the
-        // last keys', so that their latency lies under the softmax; where the registers
-        // do not hold them, as they are needed.
-        constexpr bool kAhead = D <= 96 || (D == 128 && sizeof(T) == 2 && !Parts);
-        Vec16 kf[kAhead ? 2 : 1][R::kBlocks], vf[kAhead ? 2 : 1][kParts<T>][R::kTiles];
-        auto read_keys = [&](int t) {
 #pragma unroll
-            for (int b = 0; b < R::kBlocks; ++b) {
-                kf[t % 2][b] = R::along(keys, t * E + lane % E, b, lane);
+        for (int t0 = 0; t0 < S::kTiles; t0 += S::kStep) {
+            const int first = block + (share * S::kTiles + t0) * E; // the first key of the step
+            if (first >= wave_most) {
+                break;
             }
-        };
-        auto read_values = [&](int t) {
+            // Fragments are read a tile ahead of their MFMAs, the first values' behind the
+            // last keys', so that their latency lies under the softmax; where the registers
+            // do not hold them, as they are needed.
+            constexpr bool kAhead = D <= 64 || (M == 1 && (D <= 96 || (D == 128 && sizeof(T) == 2 && !Parts)));
+            constexpr int kSets = S::kStep > 1 ? 2 : 1;
+            Vec16 kf[kSets][R::kBlocks], vf[kSets][kParts<T>][R::kTiles];
+            auto read_keys = [&](int t) {
 #pragma unroll
-            for (int p = 0; p < kParts<T>; ++p) {
-#pragma unroll
-                for (int d = 0; d < R::kTiles; ++d) {
-                    vf[t % 2][p][d] = R::across(values, t * E + 16 * p, d, lane);
+                for (int b = 0; b < R::kBlocks; ++b) {
+                    kf[t % kSets][b] = R::along(keys, (t0 + t) * E + lane % E, b, lane);
                 }
-            }
-        };
-        Acc x[S::kTiles];
-        if constexpr (kAhead) {
-            read_keys(0);
-        }
+            };
+            auto read_values = [&](int t) {
 #pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) {
-            x[t] = Acc{};
+                for (int p = 0; p < kParts<T>; ++p) {
+#pragma unroll
+                    for (int d = 0; d < R::kTiles; ++d) {
+                        vf[t % kSets][p][d] = R::across(values, (t0 + t) * E + 16 * p, d, lane);
+                    }
+                }
+            };
+            Acc x[S::kStep][M];
             if constexpr (kAhead) {
-                if (t + 1 < S::kTiles) {
-                    read_keys(t + 1);
-                } else {
-                    read_values(0);
+                read_keys(0);
+            }
+#pragma unroll
+            for (int t = 0; t < S::kStep; ++t) {
+                if constexpr (kAhead) {
+                    if (t + 1 < S::kStep) {
+                        read_keys(t + 1);
+                    } else {
+                        read_values(0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            }
 #pragma unroll
-            for (int b = 0; b < R::kBlocks; ++b) {
-                Mma<T>::run(x[t], kAhead ? kf[t % 2][b] : R::along(keys, t * E + lane % E, b, lane), qf[b]);
-            }
-            if constexpr (kAhead) {
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        if (block + K > wave_least) {
+                for (int b = 0; b < R::kBlocks; ++b) {
+                    const Vec16 fragment = kAhead ? kf[t % kSets][b] : R::along(keys, (t0 + t) * E + lane % E, b, lane);
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) {
-#pragma unroll
-                for (int i = 0; i < kRegisters<T>; ++i) {
-                    x[t][i] = first + t * E + row_of<T>(lane, i) < seen ? x[t][i] : -INFINITY;
+                    for (int m = 0; m < M; ++m) {
+                        if (b == 0) {
+                            x[t][m] = Acc{};
+                        }
+                        Mma<T>::run(x[t][m], fragment, qf[m][b]);
+                    }
                 }
-            }
-        }
-        float largest = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) {
-#pragma unroll
-            for (int i = 0; i < kRegisters<T>; ++i) {
-                largest = fmaxf(largest, x[t][i]);
-            }
-        }
-        largest = combine_column<T>(largest, Max{});
-        float factor = 1.0F;
-        if (running.raise(largest, factor)) {
-#pragma unroll
-            for (int t = 0; t < R::kTiles; ++t) {
-#pragma unroll
-                for (int i = 0; i < kRegisters<T>; ++i) {
-                    acc[t][i] *= factor;
+                if constexpr (kAhead) {
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-        }
-        float sums[4] = {0.F, 0.F, 0.F, 0.F};
+            if (first + S::kStep * E > wave_least) {
 #pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) {
+                for (int t = 0; t < S::kStep; ++t) {
 #pragma unroll
-            for (int i = 0; i < kRegisters<T>; ++i) {
-                x[t][i] = running.weight(x[t][i]);
-                sums[i % 4] += x[t][i];
-            }
-        }
-        running.sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        const int key = first + t * E + row_of<T>(lane, i);
 #pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) {
-            if constexpr (kAhead) {
-                if (t + 1 < S::kTiles) {
-                    read_values(t + 1);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int p = 0; p < kParts<T>; ++p) {
-                const Vec16 weights = weights_of<T>(x[t], p);
-#pragma unroll
-                for (int d = 0; d < R::kTiles; ++d) {
-                    Mma<T>::run(acc[d], kAhead ? vf[t % 2][p][d] : R::across(values, t * E + 16 * p, d, lane), weights);
+                        for (int m = 0; m < M; ++m) {
+                            x[t][m][i] = key < seen[m] ? x[t][m][i] : -INFINITY;
+                        }
+                    }
                 }
             }
-            if constexpr (kAhead) {
-                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                float largest = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < S::kStep; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        largest = fmaxf(largest, x[t][m][i]);
+                    }
+                }
+                largest = combine_column<T>(largest, Max{});
+                float factor = 1.0F;
+                if (running[m].raise(largest, factor)) {
+#pragma unroll
+                    for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                        for (int i = 0; i < kRegisters<T>; ++i) {
+                            acc[m][t][i] *= factor;
+                        }
+                    }
+                }
+                float sums[4] = {0.F, 0.F, 0.F, 0.F};
+#pragma unroll
+                for (int t = 0; t < S::kStep; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        x[t][m][i] = running[m].weight(x[t][m][i]);
+                        sums[i % 4] += x[t][m][i];
+                    }
+                }
+                running[m].sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < S::kStep; ++t) {
+                if constexpr (kAhead) {
+                    if (t + 1 < S::kStep) {
+                        read_values(t + 1);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int p = 0; p < kParts<T>; ++p) {
+                    Vec16 weights[M];
+#pragma unroll
+                    for (int m = 0; m < M; ++m) {
+                        weights[m] = weights_of<T>(x[t][m], p);
+                    }
+#pragma unroll
+                    for (int d = 0; d < R::kTiles; ++d) {
+                        const Vec16 fragment =
+                            kAhead ? vf[t % kSets][p][d] : R::across(values, (t0 + t) * E + 16 * p, d, lane);
+#pragma unroll
+                        for (int m = 0; m < M; ++m) {
+                            Mma<T>::run(acc[m][d], fragment, weights[m]);
+                        }
+                    }
+                }
+                if constexpr (kAhead) {
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
     }
 
-    float total = combine_column<T>(running.sum, Sum{});
+    float total[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        total[m] = combine_column<T>(running[m].sum, Sum{});
+    }
     if constexpr (S::kShared > 1) {
         // The others' sums through LDS, each scaled to the larger maximum, in turn.
+        constexpr int kOfTile = S::kSums / M; // a lane's of one tile of rows
         __syncthreads();
         float* const sums = reinterpret_cast<float*>(lds) + wave / S::kShared * (S::kShared - 1) * S::kSums * kWave + lane;
         if (share > 0) {
-            float* const to = sums + (share - 1) * S::kSums * kWave;
 #pragma unroll
-            for (int t = 0; t < R::kTiles; ++t) {
+            for (int m = 0; m < M; ++m) {
+                float* const to = sums + ((share - 1) * S::kSums + m * kOfTile) * kWave;
 #pragma unroll
-                for (int i = 0; i < kRegisters<T>; ++i) {
-                    to[(t * kRegisters<T> + i) * kWave] = acc[t][i];
+                for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        to[(t * kRegisters<T> + i) * kWave] = acc[m][t][i];
+                    }
                 }
+                to[(kOfTile - 2) * kWave] = running[m].maximum == -INFINITY ? INFINITY : running[m].shift;
+                to[(kOfTile - 1) * kWave] = total[m];
             }
-            to[(S::kSums - 2) * kWave] = running.maximum == -INFINITY ? INFINITY : running.shift;
-            to[(S::kSums - 1) * kWave] = total;
         }
         __syncthreads();
         if (share > 0) {
             return;
         }
-        float shift = running.maximum == -INFINITY ? INFINITY : running.shift;
 #pragma unroll
-        for (int o = 0; o < S::kShared - 1; ++o) {
-            const float* const from = sums + o * S::kSums * kWave;
-            const float other = from[(S::kSums - 2) * kWave];
-            const float common = fminf(shift, other);
-            // (No logit above -infinity yet: the shift is infinity, its sums 0.)
-            const float mine = shift == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - shift);
-            const float theirs = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - other);
-            total = total * mine + from[(S::kSums - 1) * kWave] * theirs;
+        for (int m = 0; m < M; ++m) {
+            float shift = running[m].maximum == -INFINITY ? INFINITY : running[m].shift;
 #pragma unroll
-            for (int t = 0; t < R::kTiles; ++t) {
+            for (int o = 0; o < S::kShared - 1; ++o) {
+                const float* const from = sums + (o * S::kSums + m * kOfTile) * kWave;
+                const float other = from[(kOfTile - 2) * kWave];
+                const float common = fminf(shift, other);
+                // (No logit above -infinity yet: the shift is infinity, its sums 0.)
+                const float mine = shift == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - shift);
+                const float theirs = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - other);
+                total[m] = total[m] * mine + from[(kOfTile - 1) * kWave] * theirs;
 #pragma unroll
-                for (int i = 0; i < kRegisters<T>; ++i) {
-                    acc[t][i] = acc[t][i] * mine + from[(t * kRegisters<T> + i) * kWave] * theirs;
+                for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        acc[m][t][i] = acc[m][t][i] * mine + from[(t * kRegisters<T> + i) * kWave] * theirs;
+                    }
                 }
+                shift = common;
             }
-            shift = common;
+            running[m].shift = shift;
+            running[m].maximum = shift == INFINITY ? -INFINITY : 0.F;
         }
-        running.shift = shift;
-        running.maximum = shift == INFINITY ? -INFINITY : 0.F;
     }
     if constexpr (Parts) {
-        if (there) {
-            float* const to = partial + partial_at(args, token * args.heads + head, parts, part);
+        const int row = first_row + lane % E;
+        if (row < rows) {
+            const Place at = place_of(row);
+            float* const to = partial + partial_at(args, at.token * args.heads + at.head, parts, part);
 #pragma unroll
             for (int t = 0; t < R::kTiles; ++t) {
 #pragma unroll
                 for (int i = 0; i < kRegisters<T>; ++i) {
                     const int dim = t * E + row_of<T>(lane, i);
                     if (dim < args.head_dim) {
-                        to[dim] = acc[t][i];
+                        to[dim] = acc[0][t][i];
                     }
                 }
             }
             if (lane < E) {
-                to[args.head_dim] = running.maximum == -INFINITY ? INFINITY : running.shift;
-                to[args.head_dim + 1] = total;
+                to[args.head_dim] = running[0].maximum == -INFINITY ? INFINITY : running[0].shift;
+                to[args.head_dim + 1] = total[0];
             }
         }
         return;
     }
-    float largest = 0.F;
 #pragma unroll
-    for (int t = 0; t < R::kTiles; ++t) {
+    for (int m = 0; m < M; ++m) {
+        const int row = first_row + m * E + lane % E;
+        const bool there = row < rows;
+        float largest = 0.F;
 #pragma unroll
-        for (int i = 0; i < kRegisters<T>; ++i) { // (a NaN stays)
-            largest = __builtin_elementwise_maximum(largest, fabsf(acc[t][i]));
+        for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+            for (int i = 0; i < kRegisters<T>; ++i) { // (a NaN stays)
+                largest = __builtin_elementwise_maximum(largest, fabsf(acc[m][t][i]));
+            }
         }
-    }
-    std::uint64_t bad = __ballot(there && !usable(seen, largest, total));
-    for (int half = 32; half >= E; half /= 2) { // any of a row's lanes
-        bad |= bad >> half;
-    }
-    if (there && (bad >> (lane % E) & 1U) == 0) {
-        store_row<T, D>(out + token * args.out.token + head * args.out.head, acc, seen > 0 ? 1.0F / total : 0.F,
-                        args.head_dim, lane);
-        if (lse != nullptr && lane < E) {
-            lse[token * args.heads + head] = log_sum_exp(seen, total, running.shift);
+        std::uint64_t bad = __ballot(there && !usable(seen[m], largest, total[m]));
+        for (int half = 32; half >= E; half /= 2) { // any of a row's lanes
+            bad |= bad >> half;
         }
-    }
-    bad &= E == 32 ? 0xFFFFFFFFU : 0xFFFFU;
-    for (; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
-        const int r = first_row + __builtin_ctzll(bad);
-        const int h = item.head * args.group + r % args.group;
-        const std::int64_t at = static_cast<std::int64_t>(span.first_query) + r / args.group;
-        attend_alone<T>(q + at * args.q.token + h * args.q.head, k_head, v_head,
-                        out + at * args.out.token + h * args.out.head, lse != nullptr ? lse + at * args.heads + h : nullptr,
-                        sees(r), args.k.token, args.v.token, args.head_dim, running.c);
+        if (there && (bad >> (lane % E) & 1U) == 0) {
+            const Place at = place_of(row);
+            store_row<T, D>(out + at.token * args.out.token + at.head * args.out.head, acc[m],
+                            seen[m] > 0 ? 1.0F / total[m] : 0.F, args.head_dim, lane);
+            if (lse != nullptr && lane < E) {
+                lse[at.token * args.heads + at.head] = log_sum_exp(seen[m], total[m], running[m].shift);
+            }
+        }
+        bad &= E == 32 ? 0xFFFFFFFFU : 0xFFFFU;
+        for (; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
+            const int r = first_row + m * E + __builtin_ctzll(bad);
+            const Place at = place_of(r);
+            attend_alone<T>(q + at.token * args.q.token + at.head * args.q.head, k_head, v_head,
+                            out + at.token * args.out.token + at.head * args.out.head,
+                            lse != nullptr ? lse + at.token * args.heads + at.head : nullptr, sees(r), args.k.token,
+                            args.v.token, args.head_dim, c);
+        }
     }
 }
 
@@ -520,26 +594,28 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q,
     }
 }
 
-/// How a call is divided, by its sizes alone: whole tiles of 128 (64) rows to a
-/// workgroup, or of 32 (16) where those would leave CUs without one, and then as many
-/// parts of the keys as fill the chip twice, of two blocks or more on average.
+/// How a call is divided, by its sizes alone: into the largest tiles of rows that still
+/// give every CU work, and for few rows into as many parts of the keys as fill the chip
+/// twice, of two blocks or more on average.
 struct Plan {
-    bool few;
+    Kind kind;
     int parts;
 };
 
 template <typename T, int D> Plan plan(const PackedArgs& args) {
-    using Few = Division<T, D, true>;
+    using Few = Division<T, D, Kind::kFew>;
     const std::int64_t units = compute_units();
-    const std::int64_t whole = slots(args.tokens, args.group, Division<T, D, false>::kRows, args.sequences) * args.kv_heads;
-    if (whole >= units) {
-        return {false, 1};
+    const auto tiles = [&](int rows) { return slots(args.tokens, args.group, rows, args.sequences) * args.kv_heads; };
+    if (tiles(Division<T, D, Kind::kLarge>::kRows) >= 2 * units) {
+        return {Kind::kLarge, 1};
     }
-    const std::int64_t tiles = slots(args.tokens, args.group, Few::kRows, args.sequences) * args.kv_heads;
+    if (tiles(Division<T, D, Kind::kMiddle>::kRows) >= units) {
+        return {Kind::kMiddle, 1};
+    }
     const std::int64_t blocks = args.kv_tokens / args.sequences / (2 * Few::kKeys);
-    const std::int64_t wanted = 2 * units / tiles;
+    const std::int64_t wanted = 2 * units / tiles(Few::kRows);
     const std::int64_t parts = wanted < blocks ? wanted : blocks;
-    return {true, static_cast<int>(parts > 1 ? parts : 1)};
+    return {Kind::kFew, static_cast<int>(parts > 1 ? parts : 1)};
 }
 
 template <typename T>
@@ -547,31 +623,37 @@ hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, float*
                   hipStream_t stream) {
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
+        using Few = Division<T, D, Kind::kFew>;
         const Plan chosen = plan<T, D>(args);
-        auto run = [&](auto kernel_constant, int rows, std::size_t lds) -> hipError_t {
-            constexpr auto kernel = decltype(kernel_constant)::kValue;
-            const std::int64_t tiles = slots(args.tokens, args.group, rows, args.sequences);
+        auto run = [&](auto division, auto in_parts) -> hipError_t {
+            using S = decltype(division);
+            constexpr auto kernel = packed_attention_kernel<T, D, S, decltype(in_parts)::value>;
+            const std::int64_t tiles = slots(args.tokens, args.group, S::kRows, args.sequences);
             const std::int64_t blocks = items(tiles, args.kv_heads) * chosen.parts;
             if (!launchable(blocks, kThreads)) {
                 return hipErrorInvalidConfiguration;
             }
-            if (const hipError_t opted = allow_lds<kernel>(lds); opted != hipSuccess) {
+            if (const hipError_t opted = allow_lds<kernel>(S::kLds); opted != hipSuccess) {
                 return opted;
             }
-            kernel<<<static_cast<unsigned int>(blocks), kThreads, lds, stream>>>(
+            kernel<<<static_cast<unsigned int>(blocks), kThreads, S::kLds, stream>>>(
                 q, k, v, out, lse, workspace, args, static_cast<int>(tiles), chosen.parts);
             return hipGetLastError();
         };
-        using Whole = Division<T, D, false>;
-        using Few = Division<T, D, true>;
-        if (!chosen.few) {
-            return run(KernelConstant<packed_attention_kernel<T, D, false, false>>{}, Whole::kRows, Whole::kLds);
+        if (chosen.kind == Kind::kLarge) {
+            return run(Division<T, D, Kind::kLarge>{}, std::false_type{});
+        }
+        if constexpr (Division<T, D, Kind::kMiddle>::kRows < Division<T, D, Kind::kLarge>::kRows) {
+            if (chosen.kind == Kind::kMiddle) {
+                return run(Division<T, D, Kind::kMiddle>{}, std::false_type{});
+            }
+        } else if (chosen.kind == Kind::kMiddle) {
+            return run(Division<T, D, Kind::kLarge>{}, std::false_type{});
         }
         if (chosen.parts == 1) {
-            return run(KernelConstant<packed_attention_kernel<T, D, true, false>>{}, Few::kRows, Few::kLds);
+            return run(Few{}, std::false_type{});
         }
-        if (const hipError_t result = run(KernelConstant<packed_attention_kernel<T, D, true, true>>{}, Few::kRows, Few::kLds);
-            result != hipSuccess) {
+        if (const hipError_t result = run(Few{}, std::true_type{}); result != hipSuccess) {
             return result;
         }
         const std::int64_t tiles = slots(args.tokens, args.group, Few::kRows, args.sequences);
