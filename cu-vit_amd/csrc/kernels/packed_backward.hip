@@ -15,11 +15,63 @@ namespace cuvit::detail {
 namespace packed {
 namespace {
 
+/// How a workgroup's wavefronts divide its work: Shared of them take the same rows (or
+/// keys), each its own part of every block, and add up at the end, so that tiles are
+/// smaller and more where they would not fill the chip.
+template <typename T, int D, int Shared> struct Division {
+    using R = Rows<T, D>;
+    static constexpr int kShared = Shared;
+    static constexpr int kTile = R::kE * kWaves / Shared;
+    static constexpr int kCount = kBlockRows<T, D> > R::kE * Shared ? kBlockRows<T, D> : R::kE * Shared; // of a block
+    static constexpr int kTiles = kCount / R::kE / Shared; // of a block, a wavefront's
+    using Loads = Stage<T, D, kCount>;
+    static constexpr int kBlocks = 4 * Loads::kBytes; // two operands, two buffers
+    static_assert(kBlocks <= 128 * 1024, "two blocks of two operands");
+};
+template <typename T, int D> constexpr int kMostShared = Rows<T, D>::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : 2;
+
+/// Adds the accumulators of the wavefronts that share a tile, in their order, in the
+/// first one of them; false for the others, which are done.
+template <typename T, int D, int Shared>
+__device__ __forceinline__ bool add_up(float* lds, int wave, int lane,
+                                       typename Mma<T>::Acc (&acc)[Rows<T, D>::kTiles]) {
+    if constexpr (Shared > 1) {
+        constexpr int kSums = Rows<T, D>::kTiles * kRegisters<T>;
+        float* const sums = lds + wave / Shared * (Shared - 1) * kSums * kWave + lane;
+        const int share = wave % Shared;
+        __syncthreads();
+        if (share > 0) {
+#pragma unroll
+            for (int t = 0; t < Rows<T, D>::kTiles; ++t) {
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    sums[((share - 1) * kSums + t * kRegisters<T> + i) * kWave] = acc[t][i];
+                }
+            }
+        }
+        __syncthreads();
+        if (share == 0) {
+#pragma unroll
+            for (int o = 0; o < Shared - 1; ++o) {
+#pragma unroll
+                for (int t = 0; t < Rows<T, D>::kTiles; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kRegisters<T>; ++i) {
+                        acc[t][i] += sums[(o * kSums + t * kRegisters<T> + i) * kWave];
+                    }
+                }
+            }
+        }
+        return share == 0;
+    }
+    return true;
+}
+
 /// Wavefronts that share a SIMD (packed_attention.hip).
 template <int D> constexpr int kShareQueries = D <= 128 ? 2 : 1;
 template <int D> constexpr int kShareKeys = D <= 64 ? 2 : 1;
 
-template <typename T, int D>
+template <typename T, int D, typename S>
 __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                   const T* __restrict__ v,
                                                                   PackedGradients<T> gradients, PackedArgs args,
@@ -27,9 +79,9 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
     using R = Rows<T, D>;
     using Acc = typename Mma<T>::Acc;
     constexpr int E = R::kE;
-    constexpr int K = kBlockRows<T, D>;
-    constexpr int kTile = E * kWaves;
-    using Loads = Stage<T, D, K>;
+    constexpr int K = S::kCount;
+    constexpr int kTile = S::kTile;
+    using Loads = typename S::Loads;
     extern __shared__ Vec16 lds_vectors[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
     const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
@@ -49,7 +101,9 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    const int row = first_row + wave * E + lane % E;
+    const int share = wave % S::kShared; // which keys of a block are this wavefront's
+    const int wave_row = first_row + wave / S::kShared * E;
+    const int row = wave_row + lane % E;
     const bool there = row < rows;
     const int query = row / args.group;
     const int head = item.head * args.group + row % args.group;
@@ -58,8 +112,8 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
         return args.causal ? min(max(min(r, rows - 1) / args.group + 1 + behind, 0), span.keys) : span.keys;
     };
     const int seen = there ? sees(row) : 0;
-    const int wave_least = __builtin_amdgcn_readfirstlane(sees(first_row + wave * E));
-    const int wave_most = first_row + wave * E < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + wave * E + E - 1)) : 0;
+    const int wave_least = __builtin_amdgcn_readfirstlane(sees(wave_row));
+    const int wave_most = wave_row < rows ? __builtin_amdgcn_readfirstlane(sees(wave_row + E - 1)) : 0;
     const int most = __builtin_amdgcn_readfirstlane(sees(first_row + kTile - 1));
 
     const Loads k_loads(k + span.first_key * args.k.token + item.head * args.k.head, args.k.token, args.head_dim, wave,
@@ -95,7 +149,7 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
     float shift = 0.F;
     if (there) {
         shift = -gradients.lse[token * args.heads + head] * kLog2e;
-        if (lane < E) {
+        if (lane < E && share == 0) {
             static_cast<float*>(gradients.workspace)[token * args.heads + head] = delta;
         }
     }
@@ -106,19 +160,20 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
         acc[t] = Acc{};
     }
     int buffer = 0;
-    for (int first = 0; first < most; first += K) {
+    for (int block = 0; block < most; block += K) {
         landed(); // and every wavefront is done with the other buffer
-        if (first + K < most) {
-            issue(first + K, buffer ^ 1);
+        if (block + K < most) {
+            issue(block + K, buffer ^ 1);
         }
-        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes;
+        const int first = block + share * S::kTiles * E; // this wavefront's first key
+        const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes + share * S::kTiles * E * R::kPitch;
         const unsigned char* const values = keys + Loads::kBytes;
         buffer ^= 1;
         if (first >= wave_most) {
             continue;
         }
 #pragma unroll
-        for (int t = 0; t < K / E; ++t) {
+        for (int t = 0; t < S::kTiles; ++t) {
             Acc x{}, y{};
 #pragma unroll
             for (int b = 0; b < R::kBlocks; ++b) {
@@ -129,7 +184,7 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
             for (int i = 0; i < kRegisters<T>; ++i) {
                 x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, shift)) * (y[i] - delta);
             }
-            if (first + K > wave_least) {
+            if (first + S::kTiles * E > wave_least) {
 #pragma unroll
                 for (int i = 0; i < kRegisters<T>; ++i) {
                     x[i] = first + t * E + row_of<T>(lane, i) < seen ? x[i] : 0.F;
@@ -145,27 +200,27 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
             }
         }
     }
-    if (there) {
+    if (add_up<T, D, S::kShared>(reinterpret_cast<float*>(lds), wave, lane, acc) && there) {
         store_row<T, D>(gradients.grad_q + token * args.q.token + head * args.q.head, acc, args.scale, args.head_dim,
                         lane);
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, typename S>
 __global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                 const T* __restrict__ v, PackedGradients<T> gradients,
                                                                 PackedArgs args, int slots) {
     using R = Rows<T, D>;
     using Acc = typename Mma<T>::Acc;
     constexpr int E = R::kE;
-    constexpr int Q = kBlockRows<T, D>; // queries of a block
-    constexpr int kTile = E * kWaves;
-    using Loads = Stage<T, D, Q>;
+    constexpr int Q = S::kCount; // queries of a block
+    constexpr int kTile = S::kTile;
+    using Loads = typename S::Loads;
     extern __shared__ Vec16 lds_vectors[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
     // Behind the tiles: the block's log-sum-exps (times -log2 e) and deltas, two buffers.
     float* const numbers = reinterpret_cast<float*>(lds + 4 * Loads::kBytes);
-    const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
+    const Item item = item_of(blockIdx.x, slots, args.kv_heads, false);
     if (item.head < 0) {
         return; // the whole workgroup, before any barrier (so below)
     }
@@ -182,13 +237,15 @@ __global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(c
     const int thread = static_cast<int>(threadIdx.x);
     const int wave = __builtin_amdgcn_readfirstlane(thread / kWave);
     const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    const int key = first_key + wave * E + lane % E;
+    const int share = wave % S::kShared; // which queries of a block are this wavefront's
+    const int wave_key = first_key + wave / S::kShared * E;
+    const int key = wave_key + lane % E;
     const bool there = key < span.keys;
     // Query i sees key j from i = j - (keys - queries) on.
     const int behind = span.keys - span.queries;
     const int from = args.causal ? max(key - behind, 0) : 0; // the first query that sees the lane's key
-    const int wave_most = __builtin_amdgcn_readfirstlane(args.causal ? max(first_key + wave * E + E - 1 - behind, 0) : 0);
-    const int wave_least = __builtin_amdgcn_readfirstlane(args.causal ? max(first_key + wave * E - behind, 0) : 0);
+    const int wave_most = __builtin_amdgcn_readfirstlane(args.causal ? max(wave_key + E - 1 - behind, 0) : 0);
+    const int wave_least = __builtin_amdgcn_readfirstlane(args.causal ? max(wave_key - behind, 0) : 0);
     const int start = __builtin_amdgcn_readfirstlane(args.causal ? max(first_key - behind, 0) / Q * Q : 0);
 
     const std::int64_t token = static_cast<std::int64_t>(span.first_key) + key;
@@ -239,16 +296,17 @@ __global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(c
                 issue(first + Q, buffer ^ 1);
                 held = fetch(first + Q);
             }
-            const unsigned char* const queries = lds + buffer * 2 * Loads::kBytes;
+            const int mine = share * S::kTiles * E; // the block's queries from here on
+            const unsigned char* const queries = lds + buffer * 2 * Loads::kBytes + mine * R::kPitch;
             const unsigned char* const grads = queries + Loads::kBytes;
-            const float* const shifts = numbers + buffer * 2 * Q;
+            const float* const shifts = numbers + buffer * 2 * Q + mine;
             const float* const deltas = shifts + Q;
             buffer ^= 1;
-            if (first + Q <= wave_least) {
+            if (first + mine + S::kTiles * E <= wave_least) {
                 continue;
             }
 #pragma unroll
-            for (int t = 0; t < Q / E; ++t) {
+            for (int t = 0; t < S::kTiles; ++t) {
                 Acc x{}, y{};
 #pragma unroll
                 for (int b = 0; b < R::kBlocks; ++b) {
@@ -267,10 +325,10 @@ __global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(c
                         y[i] -= __uint_as_float(d.w[e]);
                     }
                 }
-                if (first < wave_most) {
+                if (first + mine < wave_most) {
 #pragma unroll
                     for (int i = 0; i < kRegisters<T>; ++i) {
-                        x[i] = first + t * E + row_of<T>(lane, i) >= from ? x[i] : 0.F;
+                        x[i] = first + mine + t * E + row_of<T>(lane, i) >= from ? x[i] : 0.F;
                     }
                 }
 #pragma unroll
@@ -290,7 +348,9 @@ __global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(c
             }
         }
     }
-    if (there) {
+    float* const sums = reinterpret_cast<float*>(lds);
+    add_up<T, D, S::kShared>(sums, wave, lane, grad_k);
+    if (add_up<T, D, S::kShared>(sums, wave, lane, grad_v) && there) {
         store_row<T, D>(gradients.grad_k + token * args.k.token + item.head * args.k.head, grad_k, args.scale,
                         args.head_dim, lane);
         store_row<T, D>(gradients.grad_v + token * args.v.token + item.head * args.v.head, grad_v, 1.0F, args.head_dim,
@@ -303,31 +363,50 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
                   hipStream_t stream) {
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
-        constexpr int kTile = Mma<T>::kEdge * kWaves;
-        constexpr std::size_t kLds = 4 * Stage<T, D, kBlockRows<T, D>>::kBytes;
-        constexpr std::size_t kNumbers = 4 * kBlockRows<T, D> * sizeof(float);
-        constexpr auto by_queries = query_gradient_kernel<T, D>;
-        constexpr auto by_keys = key_gradient_kernel<T, D>;
-        const std::int64_t query_tiles = slots(args.tokens, args.group, kTile, args.sequences);
-        const std::int64_t key_tiles = slots(args.kv_tokens, 1, kTile, args.sequences);
-        const std::int64_t query_blocks = items(query_tiles, args.kv_heads);
-        const std::int64_t key_blocks = items(key_tiles, args.kv_heads);
-        if (!launchable(query_blocks, kThreads) || !launchable(key_blocks, kThreads)) {
-            return hipErrorInvalidConfiguration;
+        const std::int64_t units = compute_units();
+        /// @p run with the largest tiles that give the CUs two workgroups each, or the
+        /// smallest ones.
+        auto divided = [&](int tokens, int times, auto&& run) -> hipError_t {
+            const auto enough = [&](int rows) {
+                return slots(tokens, times, rows, args.sequences) * args.kv_heads >= 2 * units;
+            };
+            if (enough(Division<T, D, 1>::kTile)) {
+                return run(Division<T, D, 1>{});
+            }
+            if constexpr (kMostShared<T, D> > 2) {
+                if (!enough(Division<T, D, 2>::kTile)) {
+                    return run(Division<T, D, kMostShared<T, D>>{});
+                }
+            }
+            return run(Division<T, D, 2>{});
+        };
+        auto start = [&](auto kernel_constant, std::int64_t tiles, std::size_t lds) -> hipError_t {
+            constexpr auto kernel = decltype(kernel_constant)::kValue;
+            const std::int64_t blocks = items(tiles, args.kv_heads);
+            if (!launchable(blocks, kThreads)) {
+                return hipErrorInvalidConfiguration;
+            }
+            if (const hipError_t opted = allow_lds<kernel>(lds); opted != hipSuccess) {
+                return opted;
+            }
+            kernel<<<static_cast<unsigned int>(blocks), kThreads, lds, stream>>>(q, k, v, gradients, args,
+                                                                                static_cast<int>(tiles));
+            return hipGetLastError();
+        };
+        const hipError_t first = divided(args.tokens, args.group, [&](auto division) -> hipError_t {
+            using S = decltype(division);
+            return start(KernelConstant<query_gradient_kernel<T, D, S>>{},
+                         slots(args.tokens, args.group, S::kTile, args.sequences), S::kBlocks);
+        });
+        if (first != hipSuccess) {
+            return first;
         }
-        hipError_t result = allow_lds<by_queries>(kLds);
-        result = result == hipSuccess ? allow_lds<by_keys>(kLds + kNumbers) : result;
-        if (result != hipSuccess) {
-            return result;
-        }
-        by_queries<<<static_cast<unsigned int>(query_blocks), kThreads, kLds, stream>>>(
-            q, k, v, gradients, args, static_cast<int>(query_tiles));
-        if (result = hipGetLastError(); result != hipSuccess) {
-            return result;
-        }
-        by_keys<<<static_cast<unsigned int>(key_blocks), kThreads, kLds + kNumbers, stream>>>(
-            q, k, v, gradients, args, static_cast<int>(key_tiles));
-        return hipGetLastError();
+        return divided(args.kv_tokens, 1, [&](auto division) -> hipError_t {
+            using S = decltype(division);
+            return start(KernelConstant<key_gradient_kernel<T, D, S>>{},
+                         slots(args.kv_tokens, 1, S::kTile, args.sequences),
+                         S::kBlocks + 4 * S::kCount * sizeof(float));
+        });
     });
 }
 
