@@ -121,27 +121,33 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
 
 /// How a workgroup's four wavefronts divide its work: kShared of them take the same
 /// rows, each its own keys of every block, and add up at the end, which shortens a
-/// tile's walk (a call's time where tiles are few or uneven). kLarge: 128 rows in bf16,
-/// two tiles of them a wavefront, whose MFMAs share each fragment read from LDS; kMiddle
-/// half as many; kFew one tile for all four (for two of the widest heads, whose blocks
-/// would not fit otherwise).
+/// tile's walk where tiles are few. In bf16 none share where there are rows enough
+/// (kLarge, 128 of them), pairs do for fewer (kMiddle), all four for the fewest (kFew;
+/// pairs of the widest heads, whose blocks would not fit otherwise); in fp32, whose
+/// MFMAs leave nothing to overlap with in one wavefront, pairs do however many rows there are.
+/// us, kFew / kMiddle / kLarge: bf16 64 x 577 tokens, 12 heads of 64 250 / 135 / 123,
+/// 1 x 3136 72 / 65 / 84, 4 x 577 with 6 heads 10.1 / 10.9 / 15, 8192 tokens, 16 heads of
+/// 128 1555 / 652 / 537; fp32 (kFew, pairs, none) 4 x 577 with 6 heads 34.6 / 29.2 / 33.9,
+/// 4096 tokens, 16 heads 713 / 588 / 611. (Two tiles of rows a wavefront, whose MFMAs
+/// share fragments, halve what LDS is read for, but leave two wavefronts a SIMD: 146 for
+/// 123 at 64 x 577, 335 for 357 at 8192 tokens and 16 heads of 64.)
 enum class Kind { kFew, kMiddle, kLarge };
 
 template <typename T, int D, Kind Way> struct Division {
     using R = Rows<T, D>;
-    static constexpr bool kFew = Way == Kind::kFew;
-    static constexpr int kShared = kFew && R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : (Way == Kind::kLarge && R::kTiles * R::kE > 128 ? 1 : 2);
-    static constexpr int kM = Way == Kind::kLarge && sizeof(T) == 2 && D <= 96 ? 2 : 1; // tiles of rows, a wavefront's
-    static constexpr int kRows = R::kE * kM * kWaves / kShared;                 // of a workgroup
-    static constexpr int kKeys = !kFew && kBlockRows<T, D> > R::kE * kShared ? kBlockRows<T, D> : R::kE * kShared; // of a block
-    static constexpr int kTiles = kKeys / R::kE / kShared;                     // of keys, a wavefront's
-    static constexpr int kStep = kM > 1 && D > 64 ? 1 : kTiles;                // of them to a softmax
+    static constexpr int kPairs = Way == Kind::kLarge && sizeof(T) == 2 ? 1 : 2;
+    static constexpr int kShared =
+        Way == Kind::kFew && R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : kPairs;
+    static constexpr int kRows = R::kE * kWaves / kShared; // of a workgroup
+    static constexpr int kKeys = Way != Kind::kFew && kBlockRows<T, D> > R::kE * kShared ? kBlockRows<T, D>
+                                                                                        : R::kE * kShared; // of a block
+    static constexpr int kTiles = kKeys / R::kE / kShared; // of keys, a wavefront's
     /// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
     /// the registers that the VALU reads, instead of moving logits and weights over.
-    static constexpr int kShare = D > 128 ? 1 : D > 64 || kM > 1 ? 2 : 3;
+    static constexpr int kShare = D > 128 ? 1 : D > 64 ? 2 : 3;
     using Loads = Stage<T, D, kKeys>;
     // The sums of the wavefronts that add up: accumulators, shift and sum of each lane.
-    static constexpr int kSums = kM * (R::kTiles * kRegisters<T> + 2);
+    static constexpr int kSums = R::kTiles * kRegisters<T> + 2;
     static constexpr int kExchange = kWaves / kShared * (kShared - 1) * kSums * kWave * 4;
     static constexpr int kLds = 4 * Loads::kBytes > kExchange ? 4 * Loads::kBytes : kExchange;
     static_assert(kLds <= 128 * 1024, "two blocks of keys and values, or the sums");
@@ -177,7 +183,6 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
     using Loads = typename S::Loads;
     constexpr int E = R::kE;
     constexpr int K = S::kKeys;
-    constexpr int M = S::kM;
     extern __shared__ Vec16 lds_vectors[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
     const int part = Parts ? static_cast<int>(blockIdx.x % static_cast<unsigned int>(parts)) : 0;
@@ -199,22 +204,19 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int share = wave % S::kShared; // which keys of a block are this wavefront's
-    const int first_row = tile_row + wave / S::kShared * E * M;
+    const int first_row = tile_row + wave / S::kShared * E;
     const unsigned int lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
 
-    // The keys that the lane's rows (one of each tile), the wavefront and the workgroup see.
+    // The keys that the lane's row, the wavefront and the workgroup see.
     const int behind = span.keys - span.queries;
     const auto sees = [&](int r) {
         return args.causal ? min(max(min(r, rows - 1) / args.group + 1 + behind, 0), span.keys) : span.keys;
     };
-    int seen[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        const int row = first_row + m * E + lane % E;
-        seen[m] = row < rows ? sees(row) : 0;
-    }
+    const int row = first_row + lane % E;
+    const bool there = row < rows;
+    const int seen = there ? sees(row) : 0;
     const int wave_least = __builtin_amdgcn_readfirstlane(sees(first_row));
-    const int wave_most = first_row < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + E * M - 1)) : 0;
+    const int wave_most = first_row < rows ? __builtin_amdgcn_readfirstlane(sees(first_row + E - 1)) : 0;
     int most = __builtin_amdgcn_readfirstlane(sees(tile_row + S::kRows - 1));
     int start = 0;
     if constexpr (Parts) {
@@ -246,25 +248,16 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
         return Place{static_cast<std::int64_t>(span.first_query) + query,
                      item.head * args.group + row - query * args.group};
     };
-    Vec16 qf[M][R::kBlocks];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        const int row = first_row + m * E + lane % E;
-        const Place at = place_of(row);
-        load_rows<T, D>(row < rows ? q + at.token * args.q.token + at.head * args.q.head : nullptr, args.head_dim, lane,
-                        qf[m]);
-    }
+    const Place at = place_of(row);
+    Vec16 qf[R::kBlocks];
+    load_rows<T, D>(there ? q + at.token * args.q.token + at.head * args.q.head : nullptr, args.head_dim, lane, qf);
 
     const float c = args.scale * kLog2e;
-    Running running[M];
-    Acc acc[M][R::kTiles];
+    Running running{c};
+    Acc acc[R::kTiles];
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-        running[m].c = c;
-#pragma unroll
-        for (int t = 0; t < R::kTiles; ++t) {
-            acc[m][t] = Acc{};
-        }
+    for (int t = 0; t < R::kTiles; ++t) {
+        acc[t] = Acc{};
     }
     int buffer = 0;
     for (int block = start; block < most; block += K) {
@@ -275,197 +268,159 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
         const unsigned char* const keys = lds + buffer * 2 * Loads::kBytes + share * S::kTiles * E * R::kPitch;
         const unsigned char* const values = keys + Loads::kBytes;
         buffer ^= 1;
+        const int first = block + share * S::kTiles * E; // this wavefront's first key
+        if (first >= wave_most) {
+            continue;
+        }
+        // Fragments are read a tile ahead of their MFMAs, the first values' behind the
+        // last keys', so that their latency lies under the softmax; where the registers
+        // do not hold them, as they are needed.
+        constexpr bool kAhead = D <= 96 || (D == 128 && sizeof(T) == 2 && !Parts);
+        constexpr int kSets = S::kTiles > 1 ? 2 : 1;
+        Vec16 kf[kSets][R::kBlocks], vf[kSets][kParts<T>][R::kTiles];
+        auto read_keys = [&](int t) {
 #pragma unroll
-        for (int t0 = 0; t0 < S::kTiles; t0 += S::kStep) {
-            const int first = block + (share * S::kTiles + t0) * E; // the first key of the step
-            if (first >= wave_most) {
-                break;
+            for (int b = 0; b < R::kBlocks; ++b) {
+                kf[t % kSets][b] = R::along(keys, t * E + lane % E, b, lane);
             }
-            // Fragments are read a tile ahead of their MFMAs, the first values' behind the
-            // last keys', so that their latency lies under the softmax; where the registers
-            // do not hold them, as they are needed.
-            constexpr bool kAhead = D <= 64 || (M == 1 && (D <= 96 || (D == 128 && sizeof(T) == 2 && !Parts)));
-            constexpr int kSets = S::kStep > 1 ? 2 : 1;
-            Vec16 kf[kSets][R::kBlocks], vf[kSets][kParts<T>][R::kTiles];
-            auto read_keys = [&](int t) {
+        };
+        auto read_values = [&](int t) {
 #pragma unroll
-                for (int b = 0; b < R::kBlocks; ++b) {
-                    kf[t % kSets][b] = R::along(keys, (t0 + t) * E + lane % E, b, lane);
+            for (int p = 0; p < kParts<T>; ++p) {
+#pragma unroll
+                for (int d = 0; d < R::kTiles; ++d) {
+                    vf[t % kSets][p][d] = R::across(values, t * E + 16 * p, d, lane);
                 }
-            };
-            auto read_values = [&](int t) {
+            }
+        };
+        Acc x[S::kTiles];
+        if constexpr (kAhead) {
+            read_keys(0);
+        }
 #pragma unroll
-                for (int p = 0; p < kParts<T>; ++p) {
-#pragma unroll
-                    for (int d = 0; d < R::kTiles; ++d) {
-                        vf[t % kSets][p][d] = R::across(values, (t0 + t) * E + 16 * p, d, lane);
-                    }
-                }
-            };
-            Acc x[S::kStep][M];
+        for (int t = 0; t < S::kTiles; ++t) {
+            x[t] = Acc{};
             if constexpr (kAhead) {
-                read_keys(0);
+                if (t + 1 < S::kTiles) {
+                    read_keys(t + 1);
+                } else {
+                    read_values(0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int t = 0; t < S::kStep; ++t) {
-                if constexpr (kAhead) {
-                    if (t + 1 < S::kStep) {
-                        read_keys(t + 1);
-                    } else {
-                        read_values(0);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            for (int b = 0; b < R::kBlocks; ++b) {
+                Mma<T>::run(x[t], kAhead ? kf[t % kSets][b] : R::along(keys, t * E + lane % E, b, lane), qf[b]);
+            }
+            if constexpr (kAhead) {
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (first + S::kTiles * E > wave_least) {
 #pragma unroll
-                for (int b = 0; b < R::kBlocks; ++b) {
-                    const Vec16 fragment = kAhead ? kf[t % kSets][b] : R::along(keys, (t0 + t) * E + lane % E, b, lane);
+            for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
-                    for (int m = 0; m < M; ++m) {
-                        if (b == 0) {
-                            x[t][m] = Acc{};
-                        }
-                        Mma<T>::run(x[t][m], fragment, qf[m][b]);
-                    }
-                }
-                if constexpr (kAhead) {
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    x[t][i] = first + t * E + row_of<T>(lane, i) < seen ? x[t][i] : -INFINITY;
                 }
             }
-            if (first + S::kStep * E > wave_least) {
+        }
+        float largest = -INFINITY;
 #pragma unroll
-                for (int t = 0; t < S::kStep; ++t) {
+        for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
-                    for (int i = 0; i < kRegisters<T>; ++i) {
-                        const int key = first + t * E + row_of<T>(lane, i);
+            for (int i = 0; i < kRegisters<T>; ++i) {
+                largest = fmaxf(largest, x[t][i]);
+            }
+        }
+        largest = combine_column<T>(largest, Max{});
+        float factor = 1.0F;
+        if (running.raise(largest, factor)) {
 #pragma unroll
-                        for (int m = 0; m < M; ++m) {
-                            x[t][m][i] = key < seen[m] ? x[t][m][i] : -INFINITY;
-                        }
-                    }
+            for (int t = 0; t < R::kTiles; ++t) {
+#pragma unroll
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    acc[t][i] *= factor;
                 }
             }
+        }
+        float sums[4] = {0.F, 0.F, 0.F, 0.F};
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                float largest = -INFINITY;
+        for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
-                for (int t = 0; t < S::kStep; ++t) {
+            for (int i = 0; i < kRegisters<T>; ++i) {
+                x[t][i] = running.weight(x[t][i]);
+                sums[i % 4] += x[t][i];
+            }
+        }
+        running.sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
-                    for (int i = 0; i < kRegisters<T>; ++i) {
-                        largest = fmaxf(largest, x[t][m][i]);
-                    }
+        for (int t = 0; t < S::kTiles; ++t) {
+            if constexpr (kAhead) {
+                if (t + 1 < S::kTiles) {
+                    read_values(t + 1);
                 }
-                largest = combine_column<T>(largest, Max{});
-                float factor = 1.0F;
-                if (running[m].raise(largest, factor)) {
-#pragma unroll
-                    for (int t = 0; t < R::kTiles; ++t) {
-#pragma unroll
-                        for (int i = 0; i < kRegisters<T>; ++i) {
-                            acc[m][t][i] *= factor;
-                        }
-                    }
-                }
-                float sums[4] = {0.F, 0.F, 0.F, 0.F};
-#pragma unroll
-                for (int t = 0; t < S::kStep; ++t) {
-#pragma unroll
-                    for (int i = 0; i < kRegisters<T>; ++i) {
-                        x[t][m][i] = running[m].weight(x[t][m][i]);
-                        sums[i % 4] += x[t][m][i];
-                    }
-                }
-                running[m].sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int t = 0; t < S::kStep; ++t) {
-                if constexpr (kAhead) {
-                    if (t + 1 < S::kStep) {
-                        read_values(t + 1);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+            for (int p = 0; p < kParts<T>; ++p) {
+                const Vec16 weights = weights_of<T>(x[t], p);
+#pragma unroll
+                for (int d = 0; d < R::kTiles; ++d) {
+                    Mma<T>::run(acc[d], kAhead ? vf[t % kSets][p][d] : R::across(values, t * E + 16 * p, d, lane), weights);
                 }
-#pragma unroll
-                for (int p = 0; p < kParts<T>; ++p) {
-                    Vec16 weights[M];
-#pragma unroll
-                    for (int m = 0; m < M; ++m) {
-                        weights[m] = weights_of<T>(x[t][m], p);
-                    }
-#pragma unroll
-                    for (int d = 0; d < R::kTiles; ++d) {
-                        const Vec16 fragment =
-                            kAhead ? vf[t % kSets][p][d] : R::across(values, (t0 + t) * E + 16 * p, d, lane);
-#pragma unroll
-                        for (int m = 0; m < M; ++m) {
-                            Mma<T>::run(acc[m][d], fragment, weights[m]);
-                        }
-                    }
-                }
-                if constexpr (kAhead) {
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            }
+            if constexpr (kAhead) {
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
 
-    float total[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        total[m] = combine_column<T>(running[m].sum, Sum{});
-    }
+    float total = combine_column<T>(running.sum, Sum{});
     if constexpr (S::kShared > 1) {
         // The others' sums through LDS, each scaled to the larger maximum, in turn.
-        constexpr int kOfTile = S::kSums / M; // a lane's of one tile of rows
         __syncthreads();
         float* const sums = reinterpret_cast<float*>(lds) + wave / S::kShared * (S::kShared - 1) * S::kSums * kWave + lane;
         if (share > 0) {
+            float* const to = sums + (share - 1) * S::kSums * kWave;
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                float* const to = sums + ((share - 1) * S::kSums + m * kOfTile) * kWave;
+            for (int t = 0; t < R::kTiles; ++t) {
 #pragma unroll
-                for (int t = 0; t < R::kTiles; ++t) {
-#pragma unroll
-                    for (int i = 0; i < kRegisters<T>; ++i) {
-                        to[(t * kRegisters<T> + i) * kWave] = acc[m][t][i];
-                    }
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    to[(t * kRegisters<T> + i) * kWave] = acc[t][i];
                 }
-                to[(kOfTile - 2) * kWave] = running[m].maximum == -INFINITY ? INFINITY : running[m].shift;
-                to[(kOfTile - 1) * kWave] = total[m];
             }
+            to[(S::kSums - 2) * kWave] = running.maximum == -INFINITY ? INFINITY : running.shift;
+            to[(S::kSums - 1) * kWave] = total;
         }
         __syncthreads();
         if (share > 0) {
             return;
         }
+        float shift = running.maximum == -INFINITY ? INFINITY : running.shift;
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            float shift = running[m].maximum == -INFINITY ? INFINITY : running[m].shift;
+        for (int o = 0; o < S::kShared - 1; ++o) {
+            const float* const from = sums + o * S::kSums * kWave;
+            const float other = from[(S::kSums - 2) * kWave];
+            const float common = fminf(shift, other);
+            // (No logit above -infinity yet: the shift is infinity, its sums 0.)
+            const float mine = shift == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - shift);
+            const float theirs = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - other);
+            total = total * mine + from[(S::kSums - 1) * kWave] * theirs;
 #pragma unroll
-            for (int o = 0; o < S::kShared - 1; ++o) {
-                const float* const from = sums + (o * S::kSums + m * kOfTile) * kWave;
-                const float other = from[(kOfTile - 2) * kWave];
-                const float common = fminf(shift, other);
-                // (No logit above -infinity yet: the shift is infinity, its sums 0.)
-                const float mine = shift == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - shift);
-                const float theirs = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - other);
-                total[m] = total[m] * mine + from[(kOfTile - 1) * kWave] * theirs;
+            for (int t = 0; t < R::kTiles; ++t) {
 #pragma unroll
-                for (int t = 0; t < R::kTiles; ++t) {
-#pragma unroll
-                    for (int i = 0; i < kRegisters<T>; ++i) {
-                        acc[m][t][i] = acc[m][t][i] * mine + from[(t * kRegisters<T> + i) * kWave] * theirs;
-                    }
+                for (int i = 0; i < kRegisters<T>; ++i) {
+                    acc[t][i] = acc[t][i] * mine + from[(t * kRegisters<T> + i) * kWave] * theirs;
                 }
-                shift = common;
             }
-            running[m].shift = shift;
-            running[m].maximum = shift == INFINITY ? -INFINITY : 0.F;
+            shift = common;
         }
+        running.shift = shift;
+        running.maximum = shift == INFINITY ? -INFINITY : 0.F;
     }
     if constexpr (Parts) {
-        const int row = first_row + lane % E;
-        if (row < rows) {
-            const Place at = place_of(row);
+        if (there) {
             float* const to = partial + partial_at(args, at.token * args.heads + at.head, parts, part);
 #pragma unroll
             for (int t = 0; t < R::kTiles; ++t) {
@@ -473,50 +428,44 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
                 for (int i = 0; i < kRegisters<T>; ++i) {
                     const int dim = t * E + row_of<T>(lane, i);
                     if (dim < args.head_dim) {
-                        to[dim] = acc[0][t][i];
+                        to[dim] = acc[t][i];
                     }
                 }
             }
             if (lane < E) {
-                to[args.head_dim] = running[0].maximum == -INFINITY ? INFINITY : running[0].shift;
-                to[args.head_dim + 1] = total[0];
+                to[args.head_dim] = running.maximum == -INFINITY ? INFINITY : running.shift;
+                to[args.head_dim + 1] = total;
             }
         }
         return;
     }
+    float largest = 0.F;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-        const int row = first_row + m * E + lane % E;
-        const bool there = row < rows;
-        float largest = 0.F;
+    for (int t = 0; t < R::kTiles; ++t) {
 #pragma unroll
-        for (int t = 0; t < R::kTiles; ++t) {
-#pragma unroll
-            for (int i = 0; i < kRegisters<T>; ++i) { // (a NaN stays)
-                largest = __builtin_elementwise_maximum(largest, fabsf(acc[m][t][i]));
-            }
+        for (int i = 0; i < kRegisters<T>; ++i) { // (a NaN stays)
+            largest = __builtin_elementwise_maximum(largest, fabsf(acc[t][i]));
         }
-        std::uint64_t bad = __ballot(there && !usable(seen[m], largest, total[m]));
-        for (int half = 32; half >= E; half /= 2) { // any of a row's lanes
-            bad |= bad >> half;
+    }
+    std::uint64_t bad = __ballot(there && !usable(seen, largest, total));
+    for (int half = 32; half >= E; half /= 2) { // any of a row's lanes
+        bad |= bad >> half;
+    }
+    if (there && (bad >> (lane % E) & 1U) == 0) {
+        store_row<T, D>(out + at.token * args.out.token + at.head * args.out.head, acc, seen > 0 ? 1.0F / total : 0.F,
+                        args.head_dim, lane);
+        if (lse != nullptr && lane < E) {
+            lse[at.token * args.heads + at.head] = log_sum_exp(seen, total, running.shift);
         }
-        if (there && (bad >> (lane % E) & 1U) == 0) {
-            const Place at = place_of(row);
-            store_row<T, D>(out + at.token * args.out.token + at.head * args.out.head, acc[m],
-                            seen[m] > 0 ? 1.0F / total[m] : 0.F, args.head_dim, lane);
-            if (lse != nullptr && lane < E) {
-                lse[at.token * args.heads + at.head] = log_sum_exp(seen[m], total[m], running[m].shift);
-            }
-        }
-        bad &= E == 32 ? 0xFFFFFFFFU : 0xFFFFU;
-        for (; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
-            const int r = first_row + m * E + __builtin_ctzll(bad);
-            const Place at = place_of(r);
-            attend_alone<T>(q + at.token * args.q.token + at.head * args.q.head, k_head, v_head,
-                            out + at.token * args.out.token + at.head * args.out.head,
-                            lse != nullptr ? lse + at.token * args.heads + at.head : nullptr, sees(r), args.k.token,
-                            args.v.token, args.head_dim, c);
-        }
+    }
+    bad &= E == 32 ? 0xFFFFFFFFU : 0xFFFFU;
+    for (; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
+        const int r = first_row + __builtin_ctzll(bad);
+        const Place again = place_of(r);
+        attend_alone<T>(q + again.token * args.q.token + again.head * args.q.head, k_head, v_head,
+                        out + again.token * args.out.token + again.head * args.out.head,
+                        lse != nullptr ? lse + again.token * args.heads + again.head : nullptr, sees(r), args.k.token,
+                        args.v.token, args.head_dim, c);
     }
 }
 
