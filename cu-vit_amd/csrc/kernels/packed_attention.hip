@@ -131,21 +131,26 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
 /// 4096 tokens, 16 heads 713 / 588 / 611. (Two tiles of rows a wavefront, whose MFMAs
 /// share fragments, halve what LDS is read for, but leave two wavefronts a SIMD: 146 for
 /// 123 at 64 x 577, 335 for 357 at 8192 tokens and 16 heads of 64.)
-enum class Kind { kFew, kMiddle, kLarge };
+enum class Kind { kParts, kFew, kMiddle, kLarge };
 
 template <typename T, int D, Kind Way> struct Division {
     using R = Rows<T, D>;
-    static constexpr int kPairs = Way == Kind::kLarge && sizeof(T) == 2 ? 1 : 2;
+    static constexpr bool kInParts = Way == Kind::kParts;
+    static constexpr int kWaves = kInParts ? 1 : packed::kWaves;
+    static constexpr int kThreads = kWaves * kWave;
+    static constexpr int kPairs = kInParts || (Way == Kind::kLarge && sizeof(T) == 2) ? 1 : 2;
     static constexpr int kShared =
         Way == Kind::kFew && R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : kPairs;
     static constexpr int kRows = R::kE * kWaves / kShared; // of a workgroup
-    static constexpr int kKeys = Way != Kind::kFew && kBlockRows<T, D> > R::kE * kShared ? kBlockRows<T, D>
-                                                                                        : R::kE * kShared; // of a block
+    static constexpr int kLeast = kInParts ? 32 : R::kE * kShared;
+    static constexpr int kKeys = (Way == Kind::kMiddle || Way == Kind::kLarge) && kBlockRows<T, D> > kLeast
+                                     ? kBlockRows<T, D>
+                                     : kLeast; // of a block
     static constexpr int kTiles = kKeys / R::kE / kShared; // of keys, a wavefront's
     /// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
     /// the registers that the VALU reads, instead of moving logits and weights over.
     static constexpr int kShare = D > 128 ? 1 : D > 64 ? 2 : 3;
-    using Loads = Stage<T, D, kKeys>;
+    using Loads = Stage<T, D, kKeys, kWaves>;
     // The sums of the wavefronts that add up: accumulators, shift and sum of each lane.
     static constexpr int kSums = R::kTiles * kRegisters<T> + 2;
     static constexpr int kExchange = kWaves / kShared * (kShared - 1) * kSums * kWave * 4;
@@ -167,10 +172,10 @@ __device__ __forceinline__ float log_sum_exp(int seen, float total, float shift)
     return seen > 0 ? (__builtin_amdgcn_logf(total) - shift) * kLn2 : -INFINITY;
 }
 
-/// With @p Parts several workgroups take a tile, each its part of the keys, and leave
+/// In parts (Kind::kParts) several workgroups take a tile, each its part of the keys, and leave
 /// partial sums for join_kernel.
-template <typename T, int D, typename S, bool Parts>
-__global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(const T* __restrict__ q,
+template <typename T, int D, typename S>
+__global__ __launch_bounds__(S::kThreads, S::kShare) void packed_attention_kernel(const T* __restrict__ q,
                                                                                   const T* __restrict__ k,
                                                                                   const T* __restrict__ v,
                                                                                   T* __restrict__ out,
@@ -183,6 +188,7 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
     using Loads = typename S::Loads;
     constexpr int E = R::kE;
     constexpr int K = S::kKeys;
+    constexpr bool Parts = S::kInParts;
     extern __shared__ Vec16 lds_vectors[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_vectors);
     const int part = Parts ? static_cast<int>(blockIdx.x % static_cast<unsigned int>(parts)) : 0;
@@ -469,15 +475,24 @@ __global__ __launch_bounds__(kThreads, S::kShare) void packed_attention_kernel(c
     }
 }
 
-/// Adds up a row's parts in their order, a wavefront a row at a time.
+/// Workgroups to a tile's rows in the join.
+constexpr int kJoiners = 8;
+
+/// Adds up the parts of a row, wavefront w those of number w, w + 4, ..., then the four
+/// wavefronts' sums in turn. Bound by the latency of its loads: all of a wavefront's are
+/// in flight at once (32 parts of heads of 128: 22 us with a wavefront a row and a part after
+/// the other).
 template <typename T, int Tile>
 __global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                         const T* __restrict__ v, T* __restrict__ out,
                                                         float* __restrict__ lse, const float* __restrict__ partial,
                                                         PackedArgs args, int slots, int parts) {
+    __shared__ float sums[kWaves][4 * kWave];
+    __shared__ float totals[kWaves];
+    __shared__ float shifts[kWaves];
     const Item item = item_of(blockIdx.x, slots, args.kv_heads, args.causal);
     if (item.head < 0) {
-        return;
+        return; // the whole workgroup, before any barrier (so below)
     }
     const Spot spot = find(args.starts, args.sequences, args.tokens, args.group, Tile, item.slot);
     if (spot.sequence < 0) {
@@ -486,39 +501,88 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q,
     const Span span = span_of(args, spot.sequence);
     const int rows = span.queries * args.group;
     const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int last = min(rows, spot.tile * Tile + Tile);
     const float c = args.scale * kLog2e;
-    for (int row = spot.tile * Tile + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave); row < last;
-         row += kWaves) {
+    for (int row = spot.tile * Tile + static_cast<int>(blockIdx.y); row < last; row += kJoiners) {
         const int query = row / args.group;
         const int head = item.head * args.group + row % args.group;
         const std::int64_t token = static_cast<std::int64_t>(span.first_query) + query;
         const int seen = args.causal ? min(max(query + 1 + span.keys - span.queries, 0), span.keys) : span.keys;
         const float* const from = partial + partial_at(args, token * args.heads + head, parts, 0);
         const int step = args.head_dim + 2;
-        float shift = INFINITY;
-        for (int p = lane; p < parts; p += kWave) {
-            shift = fminf(shift, from[p * step + args.head_dim]);
-        }
-        shift = -wave_allreduce(-shift, Max{});
+        float shift = INFINITY; // no logit above -infinity yet
         float total = 0.F;
         float value[4] = {0.F, 0.F, 0.F, 0.F};
-#pragma unroll 4
-        for (int p = 0; p < parts; ++p) {
-            const float* const at = from + p * step;
-            const float other = at[args.head_dim];
-            const float factor = other == INFINITY ? 0.F : __builtin_amdgcn_exp2f(shift - other);
-            total += at[args.head_dim + 1] * factor;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (lane + kWave * i < args.head_dim) {
-                    value[i] += at[lane + kWave * i] * factor;
-                }
-            }
-        }
-        float largest = 0.F;
+        int dim[4]; // (behind the last one the last one again, without a branch)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            dim[i] = min(lane + kWave * i, args.head_dim - 1);
+        }
+        for (int p0 = wave; p0 < parts; p0 += 8 * kWaves) {
+            float there[8][4], others[8], totals_there[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int p = p0 + u * kWaves;
+                const float* const at = from + min(p, parts - 1) * step;
+                others[u] = p < parts ? at[args.head_dim] : INFINITY;
+                totals_there[u] = at[args.head_dim + 1];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    there[u][i] = at[dim[i]];
+                }
+            }
+            float common = shift;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                common = fminf(common, others[u]);
+            }
+            const float mine = shift == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - shift);
+            total *= mine;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                value[i] *= mine;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float theirs = others[u] == INFINITY ? 0.F : __builtin_amdgcn_exp2f(common - others[u]);
+                total += totals_there[u] * theirs;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    value[i] += there[u][i] * theirs;
+                }
+            }
+            shift = common;
+        }
+        __syncthreads(); // the last row's sums are read
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sums[wave][lane + kWave * i] = value[i];
+        }
+        if (lane == 0) {
+            totals[wave] = total;
+            shifts[wave] = shift;
+        }
+        __syncthreads();
+        if (wave != 0) {
+            continue;
+        }
+        shift = fminf(fminf(shifts[0], shifts[1]), fminf(shifts[2], shifts[3]));
+        float largest = 0.F;
+        float factor[kWaves];
+        total = 0.F;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            factor[w] = shifts[w] == INFINITY ? 0.F : __builtin_amdgcn_exp2f(shift - shifts[w]);
+            total += totals[w] * factor[w];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            value[i] = 0.F;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                value[i] += sums[w][lane + kWave * i] * factor[w];
+            }
             largest = __builtin_elementwise_maximum(largest, fabsf(value[i]));
         }
         T* const to = out + token * args.out.token + head * args.out.head;
@@ -552,7 +616,6 @@ struct Plan {
 };
 
 template <typename T, int D> Plan plan(const PackedArgs& args) {
-    using Few = Division<T, D, Kind::kFew>;
     const std::int64_t units = compute_units();
     const auto tiles = [&](int rows) { return slots(args.tokens, args.group, rows, args.sequences) * args.kv_heads; };
     if (tiles(Division<T, D, Kind::kLarge>::kRows) >= 2 * units) {
@@ -561,10 +624,11 @@ template <typename T, int D> Plan plan(const PackedArgs& args) {
     if (tiles(Division<T, D, Kind::kMiddle>::kRows) >= units) {
         return {Kind::kMiddle, 1};
     }
-    const std::int64_t blocks = args.kv_tokens / args.sequences / (2 * Few::kKeys);
-    const std::int64_t wanted = 2 * units / tiles(Few::kRows);
-    const std::int64_t parts = wanted < blocks ? wanted : blocks;
-    return {Kind::kFew, static_cast<int>(parts > 1 ? parts : 1)};
+    const std::int64_t lengths = args.kv_tokens / args.sequences; // on average
+    const std::int64_t most = lengths / (4 * Division<T, D, Kind::kParts>::kKeys);
+    const std::int64_t wanted = 8 * units / tiles(Division<T, D, Kind::kParts>::kRows);
+    const std::int64_t parts = wanted < most ? wanted : most;
+    return parts >= 4 ? Plan{Kind::kParts, static_cast<int>(parts)} : Plan{Kind::kFew, 1};
 }
 
 template <typename T>
@@ -572,41 +636,35 @@ hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, float*
                   hipStream_t stream) {
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
-        using Few = Division<T, D, Kind::kFew>;
         const Plan chosen = plan<T, D>(args);
-        auto run = [&](auto division, auto in_parts) -> hipError_t {
+        auto run = [&](auto division) -> hipError_t {
             using S = decltype(division);
-            constexpr auto kernel = packed_attention_kernel<T, D, S, decltype(in_parts)::value>;
+            constexpr auto kernel = packed_attention_kernel<T, D, S>;
             const std::int64_t tiles = slots(args.tokens, args.group, S::kRows, args.sequences);
             const std::int64_t blocks = items(tiles, args.kv_heads) * chosen.parts;
-            if (!launchable(blocks, kThreads)) {
+            if (!launchable(blocks, S::kThreads)) {
                 return hipErrorInvalidConfiguration;
             }
             if (const hipError_t opted = allow_lds<kernel>(S::kLds); opted != hipSuccess) {
                 return opted;
             }
-            kernel<<<static_cast<unsigned int>(blocks), kThreads, S::kLds, stream>>>(
+            kernel<<<static_cast<unsigned int>(blocks), S::kThreads, S::kLds, stream>>>(
                 q, k, v, out, lse, workspace, args, static_cast<int>(tiles), chosen.parts);
             return hipGetLastError();
         };
-        if (chosen.kind == Kind::kLarge) {
-            return run(Division<T, D, Kind::kLarge>{}, std::false_type{});
+        switch (chosen.kind) {
+        case Kind::kLarge: return run(Division<T, D, Kind::kLarge>{});
+        case Kind::kMiddle: return run(Division<T, D, Kind::kMiddle>{});
+        case Kind::kFew: return run(Division<T, D, Kind::kFew>{});
+        default: break;
         }
-        if constexpr (Division<T, D, Kind::kMiddle>::kRows < Division<T, D, Kind::kLarge>::kRows) {
-            if (chosen.kind == Kind::kMiddle) {
-                return run(Division<T, D, Kind::kMiddle>{}, std::false_type{});
-            }
-        } else if (chosen.kind == Kind::kMiddle) {
-            return run(Division<T, D, Kind::kLarge>{}, std::false_type{});
-        }
-        if (chosen.parts == 1) {
-            return run(Few{}, std::false_type{});
-        }
-        if (const hipError_t result = run(Few{}, std::true_type{}); result != hipSuccess) {
+        using Parts = Division<T, D, Kind::kParts>;
+        if (const hipError_t result = run(Parts{}); result != hipSuccess) {
             return result;
         }
-        const std::int64_t tiles = slots(args.tokens, args.group, Few::kRows, args.sequences);
-        join_kernel<T, Few::kRows><<<static_cast<unsigned int>(items(tiles, args.kv_heads)), kThreads, 0, stream>>>(
+        const std::int64_t tiles = slots(args.tokens, args.group, Parts::kRows, args.sequences);
+        const dim3 grid(static_cast<unsigned int>(items(tiles, args.kv_heads)), kJoiners);
+        join_kernel<T, Parts::kRows><<<grid, kThreads, 0, stream>>>(
             q, k, v, out, lse, workspace, args, static_cast<int>(tiles), chosen.parts);
         return hipGetLastError();
     });
