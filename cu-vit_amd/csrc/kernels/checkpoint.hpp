@@ -17,10 +17,22 @@ constexpr int kCodeGroup = 32;
 /// float.
 constexpr int kLeastScale = 127 - 117;
 
-/// A value's size where it is finite, else 0.
-__device__ __forceinline__ float finite_size(float v) {
-    const float size = fabsf(v);
-    return size < INFINITY ? size : 0.0F;
+/// The largest size of a lane's finite values, 0 without one. (The maximum passes over
+/// NaN by itself; only where an infinity is about are values looked at one by one.)
+template <int Count> __device__ __forceinline__ float largest_finite(const float (&v)[Count]) {
+    float largest = 0.0F;
+#pragma unroll
+    for (int e = 0; e < Count; ++e) {
+        largest = fmaxf(largest, fabsf(v[e]));
+    }
+    if (__builtin_expect(__any(largest == INFINITY), 0)) {
+        largest = 0.0F;
+#pragma unroll
+        for (int e = 0; e < Count; ++e) {
+            largest = fmaxf(largest, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0F);
+        }
+    }
+    return largest;
 }
 
 /// The scale (its exponent plus 127) of a group whose largest size is @p largest:
@@ -55,13 +67,18 @@ template <int Words> struct Bytes {
     std::uint32_t w[Words];
 };
 
-/// Four bytes a word to any address, or the first @p count of them.
-template <int Words>
+/// Four bytes a word to any address, or the first @p count of them; whole ones with
+/// @p Streaming past the caches.
+template <int Words, bool Streaming = false>
 __device__ __forceinline__ void store_bytes(std::uint8_t* to, const Bytes<Words>& bytes, int count) {
     typedef std::uint32_t words __attribute__((ext_vector_type(Words)));
     typedef words loose __attribute__((aligned(1)));
     if (count >= 4 * Words) {
-        *reinterpret_cast<loose*>(to) = __builtin_bit_cast(words, bytes);
+        if constexpr (Streaming) {
+            __builtin_nontemporal_store(__builtin_bit_cast(words, bytes), reinterpret_cast<loose*>(to));
+        } else {
+            *reinterpret_cast<loose*>(to) = __builtin_bit_cast(words, bytes);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4 * Words; ++i) {

@@ -207,10 +207,7 @@ __device__ __forceinline__ void finish_codes(const typename Mma<T>::Acc (&acc)[T
         for (int o = o0; o < o0 + kTiles; ++o) {
             float v[kValues];
             values(i, o, half, v);
-#pragma unroll
-            for (int e = 0; e < kValues; ++e) {
-                largest = fmaxf(largest, finite_size(v[e]));
-            }
+            largest = fmaxf(largest, largest_finite(v));
         }
         if constexpr (sizeof(T) == 4) {
             largest = attention::combine_rows<16>(largest, Max{});
@@ -308,12 +305,7 @@ __device__ __forceinline__ void stage_codes(const floatx16 (&acc)[S::kTM][S::kTN
                         v[e] = col0 + tile * E + Mma<std::uint16_t>::column(lane, e / 4) + e % 4 < n ? v[e] : 0.0F;
                     }
                 }
-                float largest = 0.0F;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    largest = fmaxf(largest, finite_size(v[e]));
-                }
-                const std::uint32_t scale = code_scale(attention::combine_rows<32>(largest, Max{}));
+                const std::uint32_t scale = code_scale(attention::combine_rows<32>(largest_finite(v), Max{}));
                 const float inverse = code_inverse(scale);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -327,7 +319,7 @@ __device__ __forceinline__ void stage_codes(const floatx16 (&acc)[S::kTM][S::kTN
             }
 }
 
-template <int BM, int BO, int Threads>
+template <int BM, int BO, int Threads, bool Streaming>
 __device__ __forceinline__ void store_codes(const unsigned char* lds, int row0, int col0, const GatedArgs& args) {
     using Place = CodeRows<BO>;
     constexpr int kOfHalf = Place::kPieces / 2;
@@ -338,7 +330,7 @@ __device__ __forceinline__ void store_codes(const unsigned char* lds, int row0, 
         const int col = col0 + at % kOfHalf * 16;
         if (row0 + row < args.m && col < args.n) {
             const Vec16 v = load16(lds + Place::piece(row, at));
-            store_bytes<4>(args.codes + static_cast<std::int64_t>(row0 + row) * args.ld_pre + half * args.n + col,
+            store_bytes<4, Streaming>(args.codes + static_cast<std::int64_t>(row0 + row) * args.ld_pre + half * args.n + col,
                            {{v.w[0], v.w[1], v.w[2], v.w[3]}}, args.n - col);
         }
     }
@@ -418,12 +410,12 @@ __device__ __forceinline__ void finish_staged(const floatx16 (&acc)[S::kTM][S::k
     };
     pass(std::integral_constant<int, 0>{}, c, args.ldc);
     if constexpr (Codes) {
-        __syncthreads();
+        stage_barrier(false); // (C is in registers on its way, not in LDS any more)
         if (!loading) {
             stage_codes<S>(acc, lds, wave_m, wave_n, lane, col0, args.n);
         }
-        __syncthreads();
-        store_codes<S::kBM, kBO, S::kThreads>(lds, row0, col0, args);
+        stage_barrier(false);
+        store_codes<S::kBM, kBO, S::kThreads, Streaming>(lds, row0, col0, args);
     } else if (pre != nullptr) {
         __syncthreads();
         pass(std::integral_constant<int, 1>{}, pre, args.ld_pre);
