@@ -323,11 +323,12 @@ __global__ __launch_bounds__(S::kThreads, S::kShare) void packed_attention_kerne
             }
         }
         if (first + S::kTiles * E > wave_least) {
+            const int left = seen - first - row_of<T>(lane, 0); // compared with constants
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
                 for (int i = 0; i < kRegisters<T>; ++i) {
-                    x[t][i] = first + t * E + row_of<T>(lane, i) < seen ? x[t][i] : -INFINITY;
+                    x[t][i] = t * E + row_of<T>(0, i) < left ? x[t][i] : -INFINITY;
                 }
             }
         }

@@ -185,9 +185,10 @@ __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_ker
                 x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, shift)) * (y[i] - delta);
             }
             if (first + S::kTiles * E > wave_least) {
+                const int left = seen - first - row_of<T>(lane, 0); // compared with constants
 #pragma unroll
                 for (int i = 0; i < kRegisters<T>; ++i) {
-                    x[i] = first + t * E + row_of<T>(lane, i) < seen ? x[i] : 0.F;
+                    x[i] = t * E + row_of<T>(0, i) < left ? x[i] : 0.F;
                 }
             }
 #pragma unroll
@@ -326,9 +327,10 @@ __global__ __launch_bounds__(kThreads, kShareKeys<D>) void key_gradient_kernel(c
                     }
                 }
                 if (first + mine < wave_most) {
+                    const int until = from - first - mine - row_of<T>(lane, 0); // compared with constants
 #pragma unroll
                     for (int i = 0; i < kRegisters<T>; ++i) {
-                        x[i] = first + mine + t * E + row_of<T>(lane, i) >= from ? x[i] : 0.F;
+                        x[i] = t * E + row_of<T>(0, i) >= until ? x[i] : 0.F;
                     }
                 }
 #pragma unroll
