@@ -149,7 +149,7 @@ template <typename T, int D, Kind Way> struct Division {
     static constexpr int kTiles = kKeys / R::kE / kShared; // of keys, a wavefront's
     /// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
     /// the registers that the VALU reads, instead of moving logits and weights over.
-    static constexpr int kShare = D > 128 ? 1 : D > 64 ? 2 : 3;
+    static constexpr int kShare = D > 128 ? 1 : D > 64 ? 2 : sizeof(T) == 2 && Way == Kind::kLarge ? 4 : 3;
     using Loads = Stage<T, D, kKeys, kWaves>;
     // The sums of the wavefronts that add up: accumulators, shift and sum of each lane.
     static constexpr int kSums = R::kTiles * kRegisters<T> + 2;
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(S::kThreads, S::kShare) void packed_attention_kerne
         // Fragments are read a tile ahead of their MFMAs, the first values' behind the
         // last keys', so that their latency lies under the softmax; where the registers
         // do not hold them, as they are needed.
-        constexpr bool kAhead = D <= 96 || (D == 128 && sizeof(T) == 2 && !Parts);
+        constexpr bool kAhead = (D <= 96 && S::kShare < 4) || (D == 128 && sizeof(T) == 2 && !Parts);
         constexpr int kSets = S::kTiles > 1 ? 2 : 1;
         Vec16 kf[kSets][R::kBlocks], vf[kSets][kParts<T>][R::kTiles];
         auto read_keys = [&](int t) {
