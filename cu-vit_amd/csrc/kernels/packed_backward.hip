@@ -69,7 +69,7 @@ __device__ __forceinline__ bool add_up(float* lds, int wave, int lane,
 
 /// Wavefronts that share a SIMD (packed_attention.hip).
 template <int D> constexpr int kShareQueries = D <= 128 ? 2 : 1;
-template <int D> constexpr int kShareKeys = D <= 64 ? 2 : 1;
+template <int D> constexpr int kShareKeys = D <= 96 ? 2 : 1;
 
 template <typename T, int D, typename S>
 __global__ __launch_bounds__(kThreads, kShareQueries<D>) void query_gradient_kernel(const T* __restrict__ q, const T* __restrict__ k,
@@ -408,14 +408,20 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
         const std::int64_t units = compute_units();
-        /// @p run with the largest tiles that give the CUs two workgroups each, or the
-        /// smallest ones.
-        auto divided = [&](int tokens, int times, auto&& run) -> hipError_t {
+        /// @p run with the largest tiles of rows (keys) that give the CUs two workgroups
+        /// each, or the smallest ones. Where a tile's walk, @p walk rows of the other side
+        /// on average, is short, splitting it gains less than it costs, and in fp32 pairs
+        /// of wavefronts share whatever the size (packed_attention.hip). us for 1 / 2 / 4
+        /// wavefronts to the same keys: 32 x 197 tokens, 3 heads of 64 21.7 / 22.6 / 28.9;
+        /// 1 x 3136, causal, 12 heads on 4 of 80 385 / 240 / 186, 4 of them of 128 663 /
+        /// 655 / 686; fp32 4 x 577, 6 heads 104.7 / 95.5 / 103.6.
+        auto divided = [&](int tokens, int times, std::int64_t walk, auto&& run) -> hipError_t {
             const auto enough = [&](int rows) {
                 return slots(tokens, times, rows, args.sequences) * args.kv_heads >= 2 * units;
             };
-            if (enough(Division<T, D, 1>::kTile)) {
-                return run(Division<T, D, 1>{});
+            constexpr int kLeast = sizeof(T) == 2 ? 1 : 2;
+            if (walk < 512 * args.sequences || enough(Division<T, D, kLeast>::kTile)) {
+                return run(Division<T, D, kLeast>{});
             }
             if constexpr (kMostShared<T, D> > 2) {
                 if (!enough(Division<T, D, 2>::kTile)) {
@@ -437,7 +443,7 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
                                                                                 static_cast<int>(tiles));
             return hipGetLastError();
         };
-        const hipError_t first = divided(args.tokens, args.group, [&](auto division) -> hipError_t {
+        const hipError_t first = divided(args.tokens, args.group, args.kv_tokens, [&](auto division) -> hipError_t {
             using S = decltype(division);
             return start(KernelConstant<query_gradient_kernel<T, D, S>>{},
                          slots(args.tokens, args.group, S::kTile, args.sequences), S::kBlocks);
@@ -445,7 +451,7 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
         if (first != hipSuccess) {
             return first;
         }
-        return divided(args.kv_tokens, 1, [&](auto division) -> hipError_t {
+        return divided(args.kv_tokens, 1, static_cast<std::int64_t>(args.tokens) * args.group, [&](auto division) -> hipError_t {
             using S = decltype(division);
             return start(KernelConstant<key_gradient_kernel<T, D, S>>{},
                          slots(args.kv_tokens, 1, S::kTile, args.sequences),
