@@ -409,7 +409,7 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
         constexpr int D = decltype(width)::value;
         const std::int64_t units = compute_units();
         /// @p run with the largest tiles of rows (keys) that give the CUs two workgroups
-        /// each, or the smallest ones. Where a tile's walk, @p walk rows of the other side
+        /// each (one in fp32), or the smallest ones. Where a tile's walk, @p walk rows of the other side
         /// on average, is short, splitting it gains less than it costs, and in fp32 pairs
         /// of wavefronts share whatever the size (packed_attention.hip). us for 1 / 2 / 4
         /// wavefronts to the same keys: 32 x 197 tokens, 3 heads of 64 21.7 / 22.6 / 28.9;
@@ -417,7 +417,7 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
         /// 655 / 686; fp32 4 x 577, 6 heads 104.7 / 95.5 / 103.6.
         auto divided = [&](int tokens, int times, std::int64_t walk, auto&& run) -> hipError_t {
             const auto enough = [&](int rows) {
-                return slots(tokens, times, rows, args.sequences) * args.kv_heads >= 2 * units;
+                return slots(tokens, times, rows, args.sequences) * args.kv_heads >= (sizeof(T) == 2 ? 2 : 1) * units;
             };
             constexpr int kLeast = sizeof(T) == 2 ? 1 : 2;
             if (walk < 512 * args.sequences || enough(Division<T, D, kLeast>::kTile)) {
