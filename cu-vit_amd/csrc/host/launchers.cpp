@@ -190,4 +190,60 @@ void launch_gated_backward(const std::uint16_t* preactivations, const std::uint1
     throw_on_error(cuvit_gated_backward_bf16(preactivations, grad, grad_preactivations, &problem, as_c(stream)));
 }
 
+void launch_gated_checkpoint_gemm(const float* a, const float* b, const float* bias, float* c, std::uint8_t* codes,
+                                  std::uint8_t* scales, const GatedProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_gated_checkpoint_gemm_f32(a, b, bias, c, codes, scales, &problem, as_c(stream)));
+}
+
+void launch_gated_checkpoint_backward(const std::uint8_t* codes, const std::uint8_t* scales, const float* grad,
+                                      float* grad_preactivations, float* hidden, const GatedProblem& problem,
+                                      hipStream_t stream) {
+    throw_on_error(cuvit_gated_checkpoint_backward_f32(codes, scales, grad, grad_preactivations, hidden, &problem,
+                                                        as_c(stream)));
+}
+
+void launch_packed_attention(const float* q, const float* k, const float* v, const PackedSequences& sequences, float* out,
+                             float* lse, const PackedAttentionProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_packed_attention_f32(q, k, v, sequences.starts, sequences.kv_starts, sequences.kv_lengths,
+                                               out, lse, sequences.workspace, sequences.workspace_bytes, &problem,
+                                               as_c(stream)));
+}
+
+void launch_packed_attention_backward(const float* q, const float* k, const float* v, const PackedSequences& sequences,
+                                      const float* out, const float* lse, const float* grad_out, float* grad_q, float* grad_k,
+                                      float* grad_v, const PackedAttentionProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_packed_attention_backward_f32(q, k, v, sequences.starts, sequences.kv_starts,
+                                                        sequences.kv_lengths, out, lse, grad_out, grad_q, grad_k,
+                                                        grad_v, sequences.workspace, sequences.workspace_bytes,
+                                                        &problem, as_c(stream)));
+}
+
+void launch_gated_checkpoint_gemm(const std::uint16_t* a, const std::uint16_t* b, const float* bias, std::uint16_t* c, std::uint8_t* codes,
+                                  std::uint8_t* scales, const GatedProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_gated_checkpoint_gemm_bf16(a, b, bias, c, codes, scales, &problem, as_c(stream)));
+}
+
+void launch_gated_checkpoint_backward(const std::uint8_t* codes, const std::uint8_t* scales, const std::uint16_t* grad,
+                                      std::uint16_t* grad_preactivations, std::uint16_t* hidden, const GatedProblem& problem,
+                                      hipStream_t stream) {
+    throw_on_error(cuvit_gated_checkpoint_backward_bf16(codes, scales, grad, grad_preactivations, hidden, &problem,
+                                                        as_c(stream)));
+}
+
+void launch_packed_attention(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v, const PackedSequences& sequences, std::uint16_t* out,
+                             float* lse, const PackedAttentionProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_packed_attention_bf16(q, k, v, sequences.starts, sequences.kv_starts, sequences.kv_lengths,
+                                               out, lse, sequences.workspace, sequences.workspace_bytes, &problem,
+                                               as_c(stream)));
+}
+
+void launch_packed_attention_backward(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v, const PackedSequences& sequences,
+                                      const std::uint16_t* out, const float* lse, const std::uint16_t* grad_out, std::uint16_t* grad_q, std::uint16_t* grad_k,
+                                      std::uint16_t* grad_v, const PackedAttentionProblem& problem, hipStream_t stream) {
+    throw_on_error(cuvit_packed_attention_backward_bf16(q, k, v, sequences.starts, sequences.kv_starts,
+                                                        sequences.kv_lengths, out, lse, grad_out, grad_q, grad_k,
+                                                        grad_v, sequences.workspace, sequences.workspace_bytes,
+                                                        &problem, as_c(stream)));
+}
+
 } // namespace cuvit

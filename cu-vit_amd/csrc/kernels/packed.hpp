@@ -17,7 +17,7 @@
 
 #include "attention_common.hpp"
 #include "gemm_dma.hpp"
-#include "launch.hpp"
+#include "packed_places.hpp"
 
 namespace cuvit::detail::packed {
 
@@ -36,42 +36,6 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr float kLog2e = 1.44269504088896341F;
 constexpr float kLn2 = 0.69314718055994531F;
-
-/// A sequence's tokens: queries, and keys (as many as are filled).
-struct Span {
-    int first_query;
-    int queries;
-    int first_key;
-    int keys;
-};
-
-/// Starts that do not fit the operands are cut to them, so that no access leaves
-/// them whatever the numbers say.
-__device__ __forceinline__ Span span_of(const PackedArgs& args, int sequence) {
-    Span s;
-    s.first_query = min(max(args.starts[sequence], 0), args.tokens);
-    s.queries = min(max(args.starts[sequence + 1], s.first_query), args.tokens) - s.first_query;
-    s.first_key = min(max(args.kv_starts[sequence], 0), args.kv_tokens);
-    s.keys = min(max(args.kv_starts[sequence + 1], s.first_key), args.kv_tokens) - s.first_key;
-    if (args.kv_lengths != nullptr) {
-        s.keys = min(max(args.kv_lengths[sequence], 0), s.keys);
-    }
-    return s;
-}
-
-/// The sequence and tile of slot @p slot, each sequence's rows being cut into tiles
-/// of @p rows: sequence s owns the slots from starts[s] * times / rows + s on (which
-/// steps past all its tiles before the next one's), so that the grid needs no
-/// lengths, and a wavefront finds s by comparing 64 starts at a time. -1: none.
-struct Spot {
-    int sequence;
-    int tile;
-};
-
-__device__ __forceinline__ int first_slot(const std::int32_t* starts, int sequence, int limit, int times, int rows) {
-    const std::int64_t row = static_cast<std::int64_t>(min(max(starts[sequence], 0), limit)) * times;
-    return static_cast<int>(static_cast<std::uint32_t>(row) / static_cast<std::uint32_t>(rows)) + sequence;
-}
 
 __device__ __forceinline__ Spot find(const std::int32_t* starts, int sequences, int limit, int times, int rows,
                                      int slot) {
@@ -96,32 +60,6 @@ __device__ __forceinline__ Spot find(const std::int32_t* starts, int sequences, 
     low = __builtin_amdgcn_readfirstlane(low);
     return {low, __builtin_amdgcn_readfirstlane(slot - first_slot(starts, low, limit, times, rows))};
 }
-
-/// Slots that cover tokens * times rows of any sequences.
-inline std::int64_t slots(int tokens, int times, int rows, int sequences) {
-    return static_cast<std::int64_t>(tokens) * times / rows + sequences;
-}
-
-/// Which key head and slot a workgroup takes: a head's slots follow each other on
-/// one XCD (workgroup b runs on XCD b % 8), whose L2 then holds its keys and values.
-/// With @p Uneven (causal: late tiles have more keys) late and early slots alternate,
-/// so that the XCDs' shares are alike.
-struct Item {
-    int head;
-    int slot;
-};
-
-__device__ __forceinline__ Item item_of(std::uint32_t block, int slots, int heads, bool uneven) {
-    const int slot = static_cast<int>(block / static_cast<std::uint32_t>(heads));
-    const int head = static_cast<int>(block) - slot * heads;
-    if (slot >= slots) {
-        return {-1, 0};
-    }
-    return {head, uneven ? slots - 1 - slot : slot};
-}
-
-/// Workgroups that item_of() needs.
-inline std::int64_t items(std::int64_t slots, int heads) { return (slots * heads + 7) / 8 * 8; }
 
 /// Tiles of rows of up to D values of type T in LDS.
 template <typename T, int D> struct Rows {

@@ -183,6 +183,56 @@ void launch_gated_backward(const std::uint16_t* preactivations, const std::uint1
                            std::uint16_t* grad_preactivations, const GatedProblem& problem,
                            hipStream_t stream = nullptr);
 
+/// The product that keeps its preactivations in 8 bits, and the gradient from them
+/// (hidden null: the product is not wanted again).
+void launch_gated_checkpoint_gemm(const float* a, const float* b, const float* bias, float* c,
+                                  std::uint8_t* codes, std::uint8_t* scales,
+                                  const GatedProblem& problem, hipStream_t stream = nullptr);
+void launch_gated_checkpoint_gemm(const std::uint16_t* a, const std::uint16_t* b, const float* bias,
+                                  std::uint16_t* c, std::uint8_t* codes, std::uint8_t* scales,
+                                  const GatedProblem& problem, hipStream_t stream = nullptr);
+void launch_gated_checkpoint_backward(const std::uint8_t* codes, const std::uint8_t* scales,
+                                      const float* grad, float* grad_preactivations, float* hidden,
+                                      const GatedProblem& problem, hipStream_t stream = nullptr);
+void launch_gated_checkpoint_backward(const std::uint8_t* codes, const std::uint8_t* scales,
+                                      const std::uint16_t* grad, std::uint16_t* grad_preactivations,
+                                      std::uint16_t* hidden, const GatedProblem& problem,
+                                      hipStream_t stream = nullptr);
+
+// Attention over packed sequences (extensions; cuvit/capi.h).
+using PackedAttentionProblem = cuvit_packed_attention_problem;
+
+/// Where the sequences lie, in device memory (kv_starts null: starts; kv_lengths null:
+/// all keys), and the call's workspace.
+struct PackedSequences {
+    const std::int32_t* starts = nullptr;
+    const std::int32_t* kv_starts = nullptr;
+    const std::int32_t* kv_lengths = nullptr;
+    void* workspace = nullptr;
+    std::int64_t workspace_bytes = 0;
+};
+
+void launch_packed_attention(const float* q, const float* k, const float* v,
+                             const PackedSequences& sequences, float* out, float* lse,
+                             const PackedAttentionProblem& problem, hipStream_t stream = nullptr);
+void launch_packed_attention(const std::uint16_t* q, const std::uint16_t* k, const std::uint16_t* v,
+                             const PackedSequences& sequences, std::uint16_t* out, float* lse,
+                             const PackedAttentionProblem& problem, hipStream_t stream = nullptr);
+
+void launch_packed_attention_backward(const float* q, const float* k, const float* v,
+                                      const PackedSequences& sequences, const float* out,
+                                      const float* lse, const float* grad_out, float* grad_q,
+                                      float* grad_k, float* grad_v,
+                                      const PackedAttentionProblem& problem,
+                                      hipStream_t stream = nullptr);
+void launch_packed_attention_backward(const std::uint16_t* q, const std::uint16_t* k,
+                                      const std::uint16_t* v, const PackedSequences& sequences,
+                                      const std::uint16_t* out, const float* lse,
+                                      const std::uint16_t* grad_out, std::uint16_t* grad_q,
+                                      std::uint16_t* grad_k, std::uint16_t* grad_v,
+                                      const PackedAttentionProblem& problem,
+                                      hipStream_t stream = nullptr);
+
 /// Throws the exception matching a C-ABI status (no-op on CUVIT_OK).
 void throw_on_error(int status);
 
