@@ -609,8 +609,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q,
 }
 
 /// How a call is divided, by its sizes alone: into the largest tiles of rows that still
-/// give every CU work, and for few rows into as many parts of the keys as fill the chip
-/// twice, of two blocks or more on average.
+/// give every CU work, and for few rows over long keys into as many parts of them as give
+/// the chip eight single wavefronts a CU, of four blocks or more on average. us for
+/// kMiddle / kLarge / parts of single queries: 64 over 8192 keys, 12 heads on 4 of 128 240
+/// / 280 / 200 (4 parts), 256 over 2048, 32 on 8 389 / 405 / 450, 1024 over 577, 12 of 64
+/// 303 / 311 / 470.
 struct Plan {
     Kind kind;
     int parts;
@@ -619,14 +622,17 @@ struct Plan {
 template <typename T, int D> Plan plan(const PackedArgs& args) {
     const std::int64_t units = compute_units();
     const auto tiles = [&](int rows) { return slots(args.tokens, args.group, rows, args.sequences) * args.kv_heads; };
-    if (tiles(Division<T, D, Kind::kLarge>::kRows) >= 2 * units) {
-        return {Kind::kLarge, 1};
-    }
-    if (tiles(Division<T, D, Kind::kMiddle>::kRows) >= units) {
-        return {Kind::kMiddle, 1};
-    }
     const std::int64_t lengths = args.kv_tokens / args.sequences; // on average
     const std::int64_t most = lengths / (4 * Division<T, D, Kind::kParts>::kKeys);
+    // Where a sequence's rows fit the smallest tile on average, larger ones are no fewer.
+    const bool small = static_cast<std::int64_t>(args.tokens) * args.group <=
+                       static_cast<std::int64_t>(args.sequences) * Division<T, D, Kind::kParts>::kRows;
+    if (!small && tiles(Division<T, D, Kind::kLarge>::kRows) >= 2 * units) {
+        return {Kind::kLarge, 1};
+    }
+    if (tiles(Division<T, D, Kind::kMiddle>::kRows) >= (small && most >= 16 ? 2 : 1) * units) {
+        return {Kind::kMiddle, 1};
+    }
     const std::int64_t wanted = 8 * units / tiles(Division<T, D, Kind::kParts>::kRows);
     const std::int64_t parts = wanted < most ? wanted : most;
     return parts >= 4 ? Plan{Kind::kParts, static_cast<int>(parts)} : Plan{Kind::kFew, 1};

@@ -173,6 +173,60 @@ def test_caches_with_room(cuvit, device, dtype, heads, kv_heads, head_dim, queri
 
 
 @TYPES
+@pytest.mark.parametrize("queries,keys,heads,kv_heads,head_dim", [
+    ([1] * 16, [2000] * 15 + [700], 12, 4, 128),   # parts of the keys, joined
+    ([2] * 3, [5000, 0, 130], 4, 2, 64),
+    ([1], [6000], 2, 1, 80),
+    ([1] * 90, [60] * 90, 12, 12, 64),             # many single queries: pairs of wavefronts
+    ([150] * 40, [150] * 40, 12, 4, 64),           # whole tiles
+], ids=["parts", "parts_of_uneven_keys", "parts_of_one", "pairs", "tiles"])
+def test_divisions(cuvit, device, dtype, queries, keys, heads, kv_heads, head_dim):
+    both(cuvit, device, Packed(queries, heads, head_dim, kv_heads=kv_heads, keys=keys, causal=True), dtype)
+
+
+@TYPES
+def test_bad_values_in_parts_of_the_keys(cuvit, device, dtype):
+    """As below, where a query's keys are in parts: rows that meet them are taken again."""
+    p = Packed([3], 2, 64, keys=[4000], causal=True)
+    q, k, v = operands(p, dtype, 22)
+    clean, bound, lse, lse_bound = forward(p, q, k, v, dtype)
+    v[3999], k[3998, 0] = math.inf, math.nan
+    call = Call(cuvit, device, p, q, k, v)
+    assert cuvit.packed_attention_workspace(call.problem) > 0
+    call.forward()
+    out = call.out.cpu()
+    assert worst(out[0], clean[0], bound[0]) <= 1.0
+    assert worst(call.lse.cpu()[0], lse[0], lse_bound[0]) <= 1.0
+    assert bool(torch.isnan(out[1, 0]).all()) and worst(out[1, 1], clean[1, 1], bound[1, 1]) <= 1.0
+    assert not bool(torch.isfinite(out[2]).any())
+
+
+@TYPES
+def test_no_keys_and_no_queries_at_all(cuvit, device, dtype):
+    """kv_tokens 0: zeros, -infinity and zero gradients; tokens 0: zero gradients of the keys."""
+    starts = numbers([0, 2, 5], device)
+    nothing = numbers([0, 0, 0], device)
+    p = cuvit.packed_attention_problem(2, 5, 4, 64, kv_heads=2, kv_tokens=0)
+    x = torch.ones(5, 4, 64, dtype=dtype, device=device)
+    out, lse = torch.full_like(x, 7.0), torch.full((5, 4), 7.0, device=device)
+    cuvit.packed_attention(x, None, None, starts, out, p, kv_starts=nothing, lse=lse)
+    assert bool((out == 0.0).all()) and bool((lse == -math.inf).all())
+    grad = torch.full_like(x, 7.0)
+    size = cuvit.packed_attention_backward_workspace(p)
+    cuvit.packed_attention_backward(x, None, None, starts, out, lse, x, grad, None, None, p, kv_starts=nothing,
+                                    workspace=torch.zeros(size, dtype=torch.uint8, device=device))
+    assert bool((grad == 0.0).all())
+    p = cuvit.packed_attention_problem(2, 0, 4, 64, kv_heads=2, kv_tokens=5)
+    k = torch.ones(5, 2, 64, dtype=dtype, device=device)
+    grads = [torch.full_like(k, 7.0) for _ in range(2)]
+    assert cuvit.packed_attention_backward_workspace(p) == 0
+    cuvit.packed_attention(None, k, k, nothing, None, p, kv_starts=starts, bf16=dtype == torch.bfloat16)
+    cuvit.packed_attention_backward(None, k, k, nothing, None, None, None, None, *grads, p, kv_starts=starts,
+                                    bf16=dtype == torch.bfloat16)
+    assert all(bool((g == 0.0).all()) for g in grads)
+
+
+@TYPES
 def test_rows_outside_are_not_read(cuvit, device, dtype):
     """NaN behind the last sequence and in other sequences stays there."""
     p = Packed([65, 30, 100], 2, 64, causal=True, spare=40)
