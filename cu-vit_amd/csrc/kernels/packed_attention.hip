@@ -96,7 +96,7 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
         for (int i = 0; i < 4; ++i) {
             value[i] *= kept / sum;
         }
-#pragma clang loop unroll(disable)
+#pragma unroll 8
         for (int key = 0; key < there; ++key) {
             const float s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), key));
             const T* const row = v + (first + key) * v_token;
@@ -106,6 +106,14 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
                     value[i] = fmaf(s, Elem<T>::load(row + lane + kWave * i), value[i]);
                 }
             }
+        }
+        bool open = false; // whether any value is one yet
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            open = open || (lane + kWave * i < head_dim && value[i] == value[i]);
+        }
+        if (!__any(open)) {
+            break; // NaN, whatever follows
         }
     }
 #pragma unroll

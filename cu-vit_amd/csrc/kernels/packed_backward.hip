@@ -37,6 +37,8 @@ __device__ __forceinline__ bool add_up(float* lds, int wave, int lane,
                                        typename Mma<T>::Acc (&acc)[Rows<T, D>::kTiles]) {
     if constexpr (Shared > 1) {
         constexpr int kSums = Rows<T, D>::kTiles * kRegisters<T>;
+        static_assert(kWaves / Shared * (Shared - 1) * kSums * kWave * 4 <= Division<T, D, Shared>::kBlocks,
+                      "the blocks' LDS holds them");
         float* const sums = lds + wave / Shared * (Shared - 1) * kSums * kWave + lane;
         const int share = wave % Shared;
         __syncthreads();

@@ -2,6 +2,8 @@
 // test_packed_places_cpu.py.
 #include "kernels/packed_places.hpp"
 
+#include "binding/reach.hpp"
+
 using namespace cuvit::detail;
 using namespace cuvit::detail::packed;
 
@@ -36,6 +38,12 @@ void packed_item(std::uint32_t block, int slots, int heads, int last_first, std:
     const Item item = item_of(block, slots, heads, last_first != 0);
     out[0] = item.head;
     out[1] = item.slot;
+}
+
+/// The elements that the native binding lets a launch touch, or -1 where it refuses.
+std::int64_t packed_reach(int tokens, int heads, int head_dim, std::int64_t token, std::int64_t head) {
+    std::int64_t reach = 0;
+    return cuvit::binding::rows_reach(tokens, heads, head_dim, {token, head}, &reach) ? reach : -1;
 }
 
 } // extern "C"

@@ -83,6 +83,21 @@ def test_spans_stay_within_the_operands(places):
             assert 0 <= out[2] and 0 <= out[3] and out[2] + out[3] <= keys
 
 
+@pytest.mark.parametrize("tokens,heads,head_dim", [(1, 1, 64), (5, 3, 80), (2 ** 31 - 1, 1, 256), (3, 65535, 256)])
+def test_what_operands_reach(places, tokens, heads, head_dim):
+    places.packed_reach.restype = ctypes.c_int64
+    places.packed_reach.argtypes = [ctypes.c_int] * 3 + [ctypes.c_int64] * 2
+    strides = [0, 1, 64, 2 ** 22, 2 ** 31, 2 ** 40, 2 ** 40 + 1, 2 ** 62, 2 ** 63 - 1, -1, -2 ** 63]
+    for token in strides:
+        for head in strides:
+            produced = places.packed_reach(tokens, heads, head_dim, token, head)
+            exact = (tokens - 1) * (token or heads * head_dim) + (heads - 1) * (head or head_dim) + head_dim
+            assert produced == -1 if min(token, head) < 0 else produced in (-1, exact)
+            if 0 <= min(token, head) and max(token, head) <= 64 and exact < 2 ** 31:
+                assert produced == exact
+    assert places.packed_reach(0, heads, head_dim, 0, 0) == -1
+
+
 PROGRAM = r"""
 #include <cuvit/kernels.hpp>
 #include <cstdio>
