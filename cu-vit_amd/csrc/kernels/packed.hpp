@@ -41,7 +41,7 @@ __device__ __forceinline__ Spot find(const std::int32_t* starts, int sequences, 
                                      int slot) {
     int low = 0;
     int count = sequences;
-    while (true) {
+    while (count > 1) {
         const int step = (count + kWave - 1) / kWave;
         const int probe = low + lane_id() * step;
         const bool before = probe < low + count && first_slot(starts, probe, limit, times, rows) <= slot;
@@ -51,14 +51,12 @@ __device__ __forceinline__ Spot find(const std::int32_t* starts, int sequences, 
         }
         const int last = 63 - __builtin_clzll(those);
         const int at = low + last * step;
-        count = min(step, low + count - at);
+        count = step == 1 ? 1 : min(step, low + count - at);
         low = at;
-        if (step == 1) {
-            break;
-        }
     }
     low = __builtin_amdgcn_readfirstlane(low);
-    return {low, __builtin_amdgcn_readfirstlane(slot - first_slot(starts, low, limit, times, rows))};
+    const int tile = __builtin_amdgcn_readfirstlane(slot - first_slot(starts, low, limit, times, rows));
+    return tile >= 0 ? Spot{low, tile} : Spot{-1, 0};
 }
 
 /// Tiles of rows of up to D values of type T in LDS.
