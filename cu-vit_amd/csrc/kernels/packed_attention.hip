@@ -133,6 +133,7 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
 /// (kLarge, 128 of them), pairs do for fewer (kMiddle), all four for the fewest (kFew;
 /// pairs of the widest heads, whose blocks would not fit otherwise); in fp32, whose
 /// MFMAs leave nothing to overlap with in one wavefront, pairs do however many rows there are.
+/// kParts: single wavefronts, each a part of the keys, joined by a second launch (plan()).
 /// us, kFew / kMiddle / kLarge: bf16 64 x 577 tokens, 12 heads of 64 250 / 135 / 123,
 /// 1 x 3136 72 / 65 / 84, 4 x 577 with 6 heads 10.1 / 10.9 / 15, 8192 tokens, 16 heads of
 /// 128 1555 / 652 / 537; fp32 (kFew, pairs, none) 4 x 577 with 6 heads 34.6 / 29.2 / 33.9,
