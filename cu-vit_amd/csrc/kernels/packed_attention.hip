@@ -235,10 +235,9 @@ __global__ __launch_bounds__(S::kThreads, S::kShare) void packed_attention_kerne
     int most = __builtin_amdgcn_readfirstlane(sees(tile_row + S::kRows - 1));
     int start = 0;
     if constexpr (Parts) {
-        const int blocks = (most + K - 1) / K;
-        const int of_part = (blocks + parts - 1) / parts;
-        start = min(part * of_part * K, most);
-        most = min(start + of_part * K, most);
+        const Part mine = part_of(most, part, parts, K);
+        start = __builtin_amdgcn_readfirstlane(mine.first);
+        most = __builtin_amdgcn_readfirstlane(mine.last);
     }
 
     const T* const k_head = k + span.first_key * args.k.token + item.head * args.k.head;
@@ -518,7 +517,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q,
         const int query = row / args.group;
         const int head = item.head * args.group + row % args.group;
         const std::int64_t token = static_cast<std::int64_t>(span.first_query) + query;
-        const int seen = args.causal ? min(max(query + 1 + span.keys - span.queries, 0), span.keys) : span.keys;
+        const int seen = seen_by(query, span.keys - span.queries, span.keys, args.causal);
         const float* const from = partial + partial_at(args, token * args.heads + head, parts, 0);
         const int step = args.head_dim + 2;
         float shift = INFINITY; // no logit above -infinity yet

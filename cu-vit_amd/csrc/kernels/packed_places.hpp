@@ -31,6 +31,27 @@ __host__ __device__ inline Span span_of(const PackedArgs& args, int sequence) {
     return s;
 }
 
+/// How many of a sequence's @p keys its query @p query sees, @p behind being the keys less
+/// the queries (added up otherwise, query + keys may pass 2^31).
+__host__ __device__ inline int seen_by(int query, int behind, int keys, bool causal) {
+    return causal ? smaller(larger(query + 1 + behind, 0), keys) : keys;
+}
+
+/// The keys that part @p part of @p parts takes of the first @p keys, whole blocks of
+/// @p block but for the last one. In 64 bits: parts * of_part * block passes keys.
+struct Part {
+    int first;
+    int last;
+};
+
+__host__ __device__ inline Part part_of(int keys, int part, int parts, int block) {
+    const std::int64_t blocks = (static_cast<std::int64_t>(keys) + block - 1) / block;
+    const std::int64_t of_part = (blocks + parts - 1) / parts * block;
+    const std::int64_t first = part * of_part;
+    const std::int64_t last = first + of_part;
+    return {first < keys ? static_cast<int>(first) : keys, last < keys ? static_cast<int>(last) : keys};
+}
+
 /// The sequence and tile of slot @p slot, each sequence's rows being cut into tiles
 /// of @p rows: sequence s owns the slots from starts[s] * times / rows + s on (which
 /// steps past all its tiles before the next one's), so that the grid needs no

@@ -1,0 +1,48 @@
+"""Which keys the parts and the queries of packed attention take, up to the longest
+caches that a call accepts (kernels/packed_places.hpp)."""
+
+from __future__ import annotations
+
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from conftest import ROOT
+
+MOST = 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def choice():
+    library = Path(ROOT) / "tests" / "cpp" / "bin" / "libpacked_choice.so"
+    if not library.exists():
+        subprocess.run(["make", "-s", "-C", str(library.parents[1])], check=True)
+    return ctypes.CDLL(str(library))
+
+
+@pytest.mark.parametrize("keys", [0, 1, 31, 32, 33, 4096, 12545, 2 ** 30 + 7, 2 ** 31 - 4096, MOST - 99, MOST - 31,
+                                  MOST - 30, MOST])
+@pytest.mark.parametrize("parts", [4, 7, 64, 512, 2048, 2432])
+def test_parts_cover_the_keys(choice, keys, parts):
+    """One behind the other, from the first key to the last, whole blocks each but the last one."""
+    out = (ctypes.c_int32 * 2)()
+    at = 0
+    for part in range(parts):
+        choice.packed_part(keys, part, parts, 32, out)
+        assert out[0] == at and at <= out[1] <= keys
+        assert out[0] == keys or out[0] % 32 == 0
+        at = out[1]
+    assert at == keys
+
+
+def test_keys_that_a_query_sees(choice):
+    counts = [0, 1, 2, 5000, 2 ** 30, 2 ** 31 - 4096, MOST]
+    for queries in counts[1:]:
+        for keys in counts:
+            for query in {0, 1, queries // 2, queries - 1}:
+                if query < queries:
+                    expected = min(max(query + 1 + keys - queries, 0), keys)
+                    assert choice.packed_seen(query, queries, keys, 1) == expected
+                    assert choice.packed_seen(query, queries, keys, 0) == keys
