@@ -15,7 +15,8 @@
 // they are summed. A row whose sums overflowed (values beyond 2^128 / (keys
 // 2^kHeadroom)), or that met an infinity or NaN, which may lie in a key it does not see
 // (0 times infinity), is taken again by itself over its own keys. A row without keys is
-// zeros, its log-sum-exp -infinity; a row whose every logit is -infinity is NaN.
+// zeros, its log-sum-exp -infinity, whatever its tile's other rows see; a row whose every
+// logit is -infinity is NaN.
 #include "packed.hpp"
 
 namespace cuvit::detail {
@@ -119,7 +120,7 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (lane + kWave * i < head_dim) {
-            Elem<T>::store(out + lane + kWave * i, sum > 0.F ? value[i] : __builtin_nanf(""));
+            Elem<T>::store(out + lane + kWave * i, sum > 0.F || keys == 0 ? value[i] : __builtin_nanf(""));
         }
     }
     if (lse != nullptr && lane == 0) {
@@ -175,7 +176,7 @@ __device__ __forceinline__ std::int64_t partial_at(const PackedArgs& args, std::
 /// The result and log-sum-exp of a row from its sums, or false where they are of no use
 /// (see the top). @p largest is the largest size among the accumulators.
 __device__ __forceinline__ bool usable(int seen, float largest, float total) {
-    return seen == 0 || (largest < INFINITY && total > 0.F && total < INFINITY);
+    return largest < INFINITY && (seen == 0 || (total > 0.F && total < INFINITY));
 }
 __device__ __forceinline__ float log_sum_exp(int seen, float total, float shift) {
     return seen > 0 ? (__builtin_amdgcn_logf(total) - shift) * kLn2 : -INFINITY;
