@@ -15,6 +15,9 @@ namespace {
 constexpr int kMaxHeads = 65535;
 constexpr int kMaxHeadDim = 256;
 constexpr std::int64_t kMaxRows = 0x7FFFFFFF;
+/// Tokens of either side: the kernels' walks count them in 32 bits and step past the last
+/// one by a block.
+constexpr int kMaxTokens = 0x7FFFFFFF - 4095;
 /// A token's stride, so that a tile of rows stays within a load's 32-bit offsets.
 constexpr std::int64_t kMaxTokenBytes = std::int64_t{1} << 23;
 
@@ -75,6 +78,9 @@ int check_problem(const cuvit_packed_attention_problem& p, std::int64_t size, de
     if (static_cast<std::int64_t>(p.tokens) * p.heads > kMaxRows ||
         static_cast<std::int64_t>(p.kv_tokens) * p.kv_heads > kMaxRows) {
         return fail(CUVIT_ERROR_LENGTH, "Packed attention takes at most 2^31 - 1 tokens times heads");
+    }
+    if (p.tokens > kMaxTokens || p.kv_tokens > kMaxTokens) {
+        return fail(CUVIT_ERROR_LENGTH, "Packed attention takes at most 2^31 - 4096 tokens");
     }
     *args = detail::PackedArgs{};
     args->sequences = p.sequences;

@@ -408,9 +408,10 @@ void cuvit_packed_attention_problem_projection(cuvit_packed_attention_problem* p
  * aligned; out and lse overlap no other operand. The workspace, of
  * cuvit_packed_attention_workspace() bytes (null where that is 0) and 16-byte
  * aligned, is used by one call at a time: calls that may overlap, replays of
- * captured ones among them, take one each. More than 65535 heads, or 2^31 - 1
- * tokens times heads of either side, or 2^32 threads (2^24 tiles of 32 rows in
- * fp32, 128 in bf16, a sequence starting a new one) are CUVIT_ERROR_LENGTH. */
+ * captured ones among them, take one each. More than 65535 heads, or 2^31 - 4096
+ * tokens or 2^31 - 1 tokens times heads of either side, or 2^32 threads (2^24
+ * tiles of 32 rows in fp32, 128 in bf16, a sequence starting a new one) are
+ * CUVIT_ERROR_LENGTH. */
 int64_t cuvit_packed_attention_workspace(const cuvit_packed_attention_problem* problem);
 int cuvit_packed_attention_f32(const float* q, const float* k, const float* v,
                                const int32_t* starts, const int32_t* kv_starts,

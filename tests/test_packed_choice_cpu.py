@@ -1,5 +1,5 @@
 """Which keys the parts and the queries of packed attention take, up to the longest
-caches that a call accepts (kernels/packed_places.hpp)."""
+caches that a call accepts (kernels/packed_places.hpp), and that none longer is."""
 
 from __future__ import annotations
 
@@ -9,7 +9,9 @@ from pathlib import Path
 
 import pytest
 
+import cuvit_amd as cuvit
 from conftest import ROOT
+from test_packed_attention_cpu import CALLS, ADDRESS, forward_call
 
 MOST = 2 ** 31 - 1
 
@@ -46,3 +48,26 @@ def test_keys_that_a_query_sees(choice):
                     expected = min(max(query + 1 + keys - queries, 0), keys)
                     assert choice.packed_seen(query, queries, keys, 1) == expected
                     assert choice.packed_seen(query, queries, keys, 0) == keys
+
+
+LONGEST = 2 ** 31 - 4096
+
+
+def single_head(tokens, kv_tokens):
+    return cuvit.packed_attention_problem(1, tokens, 1, 8, kv_tokens=kv_tokens)
+
+
+@CALLS
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("tokens,kv_tokens", [(1, LONGEST + 1), (LONGEST + 1, 1), (1, MOST), (MOST, 1), (MOST, MOST)])
+def test_lengths_near_2_to_31(lib, call, bf16, tokens, kv_tokens):
+    """The walks over keys and queries step past the last one in 32 bits."""
+    assert call(lib, single_head(tokens, kv_tokens), bf16=bf16, kv_starts=ADDRESS) == cuvit.ERROR_LENGTH
+    assert b"2^31 - 4096" in lib.cuvit_last_error()
+
+
+def test_the_longest_lengths_are_taken(lib):
+    """Refused only for what is checked behind the lengths."""
+    for tokens, kv_tokens in ((1, LONGEST), (LONGEST, 1), (LONGEST, LONGEST)):
+        assert forward_call(lib, single_head(tokens, kv_tokens), kv_starts=ADDRESS, q=ADDRESS + 8) == cuvit.ERROR_INVALID_ARGUMENT
+        assert b"aligned" in lib.cuvit_last_error()

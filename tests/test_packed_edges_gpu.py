@@ -49,3 +49,39 @@ def test_rows_without_keys_beside_bad_values(cuvit, device, dtype, bad, queries,
     assert bool((produced[unseen] == -math.inf).all())
     assert worst(out[untouched], clean[untouched], bound[untouched]) <= 1.0
     assert worst(produced[untouched], lse[untouched], lse_bound[untouched]) <= 1.0
+
+
+@pytest.mark.parametrize("queries", [1, 33])
+def test_the_longest_cache(cuvit, device, queries):
+    """2^31 - 4096 keys of 8 values in bf16, 34 GB, in parts that are joined. Keys and
+    values are zeros but for the last key's, whose logit is 30: only the last query sees
+    it, and 2^31 weights of exp(-30), 2e-4 in all, beside it; the others sum ones."""
+    keys = 2 ** 31 - 4096
+    if torch.cuda.mem_get_info()[0] < 80e9:
+        pytest.skip("needs 80 GB of memory")
+    k = torch.zeros(keys, 1, 8, dtype=torch.bfloat16, device=device)
+    v = torch.zeros_like(k)
+    k[-1], v[-1] = 4.0, torch.arange(1, 9, device=device).to(torch.bfloat16)
+    q = torch.ones(queries, 1, 8, dtype=torch.bfloat16, device=device)
+    p = cuvit.packed_attention_problem(1, queries, 1, 8, kv_tokens=keys, scale=30.0 / 32.0, causal=True)
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((queries, 1), 7.0, device=device)
+    size = cuvit.packed_attention_workspace(p)
+    assert size > 0
+    cuvit.packed_attention(q, k, v, torch.tensor([0, queries], dtype=torch.int32, device=device), out, p,
+                           kv_starts=torch.tensor([0, keys], dtype=torch.int32, device=device), lse=lse,
+                           workspace=torch.zeros(size, dtype=torch.uint8, device=device))
+    out, lse = out[:, 0].cpu().double(), lse[:, 0].cpu().double()
+    del k, v
+    torch.cuda.empty_cache()
+    # A lane's sums are multiples of 16 below 2^28, or of 1 below 2^24: exact. A weight of
+    # exp(-30) is off by its argument's rounding, 2^-24 of 43 a factor of it and as many
+    # again in the maxima, below 2^-14 in all; the log-sum-exp by its factors' roundings.
+    small = (keys - 1) * math.exp(-30.0)
+    value = torch.arange(1, 9).double() / (1.0 + small)
+    assert worst(out[-1], value, (2.0 ** -8 + 2.0 ** -14) * value) <= 1.0
+    assert abs(float(lse[-1]) - (30.0 + math.log1p(small))) <= 2.0 ** -14 * small + 8 * 2.0 ** -24 * 30.0
+    if queries > 1:
+        seen = keys - queries + torch.arange(1, queries).double()
+        assert bool((out[:-1] == 0.0).all())
+        assert float((lse[:-1] - torch.log(seen)).abs().max()) <= 8 * 2.0 ** -24 * 30.0
