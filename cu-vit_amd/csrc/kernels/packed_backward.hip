@@ -432,33 +432,37 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
             }
             return run(Division<T, D, 2>{});
         };
+        // Each launch's kernel, tiles and LDS for @p each.
+        auto queries = [&](auto&& each) -> hipError_t {
+            return divided(args.tokens, args.group, args.kv_tokens, [&](auto division) -> hipError_t {
+                using S = decltype(division);
+                return each(KernelConstant<query_gradient_kernel<T, D, S>>{},
+                            slots(args.tokens, args.group, S::kTile, args.sequences), S::kBlocks);
+            });
+        };
+        auto keys = [&](auto&& each) -> hipError_t {
+            return divided(args.kv_tokens, 1, static_cast<std::int64_t>(args.tokens) * args.group, [&](auto division) -> hipError_t {
+                using S = decltype(division);
+                return each(KernelConstant<key_gradient_kernel<T, D, S>>{},
+                            slots(args.kv_tokens, 1, S::kTile, args.sequences),
+                            S::kBlocks + 4 * S::kCount * sizeof(float));
+            });
+        };
+        // What is refused is so before the first launch, which overwrites grad_q.
+        auto check = [&](auto kernel_constant, std::int64_t tiles, std::size_t lds) -> hipError_t {
+            return launchable(items(tiles, args.kv_heads), kThreads) ? allow_lds<decltype(kernel_constant)::kValue>(lds)
+                                                                     : hipErrorInvalidConfiguration;
+        };
         auto start = [&](auto kernel_constant, std::int64_t tiles, std::size_t lds) -> hipError_t {
             constexpr auto kernel = decltype(kernel_constant)::kValue;
-            const std::int64_t blocks = items(tiles, args.kv_heads);
-            if (!launchable(blocks, kThreads)) {
-                return hipErrorInvalidConfiguration;
-            }
-            if (const hipError_t opted = allow_lds<kernel>(lds); opted != hipSuccess) {
-                return opted;
-            }
-            kernel<<<static_cast<unsigned int>(blocks), kThreads, lds, stream>>>(q, k, v, gradients, args,
-                                                                                static_cast<int>(tiles));
+            kernel<<<static_cast<unsigned int>(items(tiles, args.kv_heads)), kThreads, lds, stream>>>(
+                q, k, v, gradients, args, static_cast<int>(tiles));
             return hipGetLastError();
         };
-        const hipError_t first = divided(args.tokens, args.group, args.kv_tokens, [&](auto division) -> hipError_t {
-            using S = decltype(division);
-            return start(KernelConstant<query_gradient_kernel<T, D, S>>{},
-                         slots(args.tokens, args.group, S::kTile, args.sequences), S::kBlocks);
-        });
-        if (first != hipSuccess) {
-            return first;
-        }
-        return divided(args.kv_tokens, 1, static_cast<std::int64_t>(args.tokens) * args.group, [&](auto division) -> hipError_t {
-            using S = decltype(division);
-            return start(KernelConstant<key_gradient_kernel<T, D, S>>{},
-                         slots(args.kv_tokens, 1, S::kTile, args.sequences),
-                         S::kBlocks + 4 * S::kCount * sizeof(float));
-        });
+        hipError_t result = queries(check);
+        result = result == hipSuccess ? keys(check) : result;
+        result = result == hipSuccess ? queries(start) : result;
+        return result == hipSuccess ? keys(start) : result;
     });
 }
 

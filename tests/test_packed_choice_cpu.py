@@ -11,7 +11,7 @@ import pytest
 
 import cuvit_amd as cuvit
 from conftest import ROOT
-from test_packed_attention_cpu import CALLS, ADDRESS, forward_call
+from test_packed_attention_cpu import ADDRESS, CALLS, backward_call, forward_call
 
 MOST = 2 ** 31 - 1
 
@@ -71,3 +71,11 @@ def test_the_longest_lengths_are_taken(lib):
     for tokens, kv_tokens in ((1, LONGEST), (LONGEST, 1), (LONGEST, LONGEST)):
         assert forward_call(lib, single_head(tokens, kv_tokens), kv_starts=ADDRESS, q=ADDRESS + 8) == cuvit.ERROR_INVALID_ARGUMENT
         assert b"aligned" in lib.cuvit_last_error()
+
+
+def test_gradients_are_refused_before_any_launch(lib):
+    """Keys for more than 2^32 threads, queries for few: nothing is overwritten. (Without a
+    GPU the rows' launch would end the call with another error.)"""
+    p = cuvit.packed_attention_problem(1, 1, 1, 8, kv_tokens=2 ** 30)
+    assert backward_call(lib, p, bf16=False, kv_starts=ADDRESS) == cuvit.ERROR_LENGTH
+    assert b"2^32 threads" in lib.cuvit_last_error()
