@@ -18,6 +18,7 @@
 // zeros, its log-sum-exp -infinity, whatever its tile's other rows see; a row whose every
 // logit is -infinity is NaN.
 #include "packed.hpp"
+#include "packed_choice.hpp"
 
 namespace cuvit::detail {
 namespace packed {
@@ -128,21 +129,18 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
     }
 }
 
-/// How a workgroup's four wavefronts divide its work: kShared of them take the same
-/// rows, each its own keys of every block, and add up at the end, which shortens a
-/// tile's walk where tiles are few. In bf16 none share where there are rows enough
+/// How a workgroup's four wavefronts divide its work (packed_choice.hpp): kShared of them
+/// take the same rows, each its own keys of every block, and add up at the end, which
+/// shortens a tile's walk where tiles are few. In bf16 none share where there are rows enough
 /// (kLarge, 128 of them), pairs do for fewer (kMiddle), all four for the fewest (kFew;
 /// pairs of the widest heads, whose blocks would not fit otherwise); in fp32, whose
 /// MFMAs leave nothing to overlap with in one wavefront, pairs do however many rows there are.
-/// kParts: single wavefronts, each a part of the keys, joined by a second launch (plan()).
 /// us, kFew / kMiddle / kLarge: bf16 64 x 577 tokens, 12 heads of 64 250 / 135 / 123,
 /// 1 x 3136 72 / 65 / 84, 4 x 577 with 6 heads 10.1 / 10.9 / 15, 8192 tokens, 16 heads of
 /// 128 1555 / 652 / 537; fp32 (kFew, pairs, none) 4 x 577 with 6 heads 34.6 / 29.2 / 33.9,
 /// 4096 tokens, 16 heads 713 / 588 / 611. (Two tiles of rows a wavefront, whose MFMAs
 /// share fragments, halve what LDS is read for, but leave two wavefronts a SIMD: 146 for
 /// 123 at 64 x 577, 335 for 357 at 8192 tokens and 16 heads of 64.)
-enum class Kind { kParts, kFew, kMiddle, kLarge };
-
 template <typename T, int D, Kind Way> struct Division {
     using R = Rows<T, D>;
     static constexpr bool kInParts = Way == Kind::kParts;
@@ -166,6 +164,8 @@ template <typename T, int D, Kind Way> struct Division {
     static constexpr int kExchange = kWaves / kShared * (kShared - 1) * kSums * kWave * 4;
     static constexpr int kLds = 4 * Loads::kBytes > kExchange ? 4 * Loads::kBytes : kExchange;
     static_assert(kLds <= 128 * 1024, "two blocks of keys and values, or the sums");
+    static_assert(Way == Kind::kFew || kRows == tile_rows(Way, sizeof(T) == 4), "as the rules count them");
+    static_assert(!kInParts || kKeys == kPartKeys, "as the rules count them");
 };
 
 /// A row's partial sums in the workspace: head_dim floats and the shift and the sum.
@@ -617,42 +617,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const T* __restrict__ q,
     }
 }
 
-/// How a call is divided, by its sizes alone: into the largest tiles of rows that still
-/// give every CU work, and for few rows over long keys into as many parts of them as give
-/// the chip eight single wavefronts a CU, of four blocks or more on average. us for
-/// kMiddle / kLarge / parts of single queries: 64 over 8192 keys, 12 heads on 4 of 128 240
-/// / 280 / 200 (4 parts), 256 over 2048, 32 on 8 389 / 405 / 450, 1024 over 577, 12 of 64
-/// 303 / 311 / 470.
-struct Plan {
-    Kind kind;
-    int parts;
-};
-
-template <typename T, int D> Plan plan(const PackedArgs& args) {
-    const std::int64_t units = compute_units();
-    const auto tiles = [&](int rows) { return slots(args.tokens, args.group, rows, args.sequences) * args.kv_heads; };
-    const std::int64_t lengths = args.kv_tokens / args.sequences; // on average
-    const std::int64_t most = lengths / (4 * Division<T, D, Kind::kParts>::kKeys);
-    // Where a sequence's rows fit the smallest tile on average, larger ones are no fewer.
-    const bool small = static_cast<std::int64_t>(args.tokens) * args.group <=
-                       static_cast<std::int64_t>(args.sequences) * Division<T, D, Kind::kParts>::kRows;
-    if (!small && tiles(Division<T, D, Kind::kLarge>::kRows) >= 2 * units) {
-        return {Kind::kLarge, 1};
-    }
-    if (tiles(Division<T, D, Kind::kMiddle>::kRows) >= (small && most >= 16 ? 2 : 1) * units) {
-        return {Kind::kMiddle, 1};
-    }
-    const std::int64_t wanted = 8 * units / tiles(Division<T, D, Kind::kParts>::kRows);
-    const std::int64_t parts = wanted < most ? wanted : most;
-    return parts >= 4 ? Plan{Kind::kParts, static_cast<int>(parts)} : Plan{Kind::kFew, 1};
-}
-
 template <typename T>
 hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, float* workspace, const PackedArgs& args,
                   hipStream_t stream) {
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
-        const Plan chosen = plan<T, D>(args);
+        const Plan chosen = choose_forward(args, sizeof(T) == 4, compute_units());
         auto run = [&](auto division) -> hipError_t {
             using S = decltype(division);
             constexpr auto kernel = packed_attention_kernel<T, D, S>;
@@ -686,17 +656,11 @@ hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, float*
     });
 }
 
-template <typename T> std::int64_t workspace_of(const PackedArgs& args) {
-    std::int64_t bytes = 0;
-    (void)with_width(args.head_dim, [&](auto width) -> hipError_t {
-        const Plan chosen = plan<T, decltype(width)::value>(args);
-        if (chosen.parts > 1) {
-            bytes = static_cast<std::int64_t>(args.tokens) * args.heads * chosen.parts * (args.head_dim + 2) *
-                    static_cast<std::int64_t>(sizeof(float));
-        }
-        return hipSuccess;
-    });
-    return bytes;
+std::int64_t workspace_of(const PackedArgs& args, bool single) {
+    const Plan chosen = choose_forward(args, single, compute_units());
+    return chosen.parts > 1 ? static_cast<std::int64_t>(args.tokens) * args.heads * chosen.parts * (args.head_dim + 2) *
+                                  static_cast<std::int64_t>(sizeof(float))
+                            : 0;
 }
 
 } // namespace
@@ -713,8 +677,8 @@ hipError_t packed_attention(const std::uint16_t* q, const std::uint16_t* k, cons
 }
 
 std::int64_t packed_attention_workspace(const PackedArgs& args) {
-    const std::int64_t single = packed::workspace_of<float>(args);
-    const std::int64_t half = packed::workspace_of<std::uint16_t>(args);
+    const std::int64_t single = packed::workspace_of(args, true);
+    const std::int64_t half = packed::workspace_of(args, false);
     return single > half ? single : half;
 }
 

@@ -10,6 +10,7 @@
 // fix, at the cost of computing logits and d.v twice (7 products for 5); sums across
 // workgroups would need atomics, whose order changes results, or fp32 copies of grad_q.
 #include "packed.hpp"
+#include "packed_choice.hpp"
 
 namespace cuvit::detail {
 namespace packed {
@@ -410,23 +411,16 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
     return with_width(args.head_dim, [&](auto width) -> hipError_t {
         constexpr int D = decltype(width)::value;
         const std::int64_t units = compute_units();
-        /// @p run with the largest tiles of rows (keys) that give the CUs two workgroups
-        /// each (one in fp32), or the smallest ones. Where a tile's walk, @p walk rows of the other side
-        /// on average, is short, splitting it gains less than it costs, and in fp32 pairs
-        /// of wavefronts share whatever the size (packed_attention.hip). us for 1 / 2 / 4
-        /// wavefronts to the same keys: 32 x 197 tokens, 3 heads of 64 21.7 / 22.6 / 28.9;
-        /// 1 x 3136, causal, 12 heads on 4 of 80 385 / 240 / 186, 4 of them of 128 663 /
-        /// 655 / 686; fp32 4 x 577, 6 heads 104.7 / 95.5 / 103.6.
-        auto divided = [&](int tokens, int times, std::int64_t walk, auto&& run) -> hipError_t {
-            const auto enough = [&](int rows) {
-                return slots(tokens, times, rows, args.sequences) * args.kv_heads >= (sizeof(T) == 2 ? 2 : 1) * units;
-            };
-            constexpr int kLeast = sizeof(T) == 2 ? 1 : 2;
-            if (walk < 512 * args.sequences || enough(Division<T, D, kLeast>::kTile)) {
-                return run(Division<T, D, kLeast>{});
+        /// @p run with @p sharing wavefronts to a tile (packed_choice.hpp).
+        auto divided = [&](int sharing, auto&& run) -> hipError_t {
+            static_assert(kMostShared<T, D> == most_sharing(D), "as the rules count them");
+            if constexpr (sizeof(T) == 2) {
+                if (sharing == 1) {
+                    return run(Division<T, D, 1>{});
+                }
             }
             if constexpr (kMostShared<T, D> > 2) {
-                if (!enough(Division<T, D, 2>::kTile)) {
+                if (sharing > 2) {
                     return run(Division<T, D, kMostShared<T, D>>{});
                 }
             }
@@ -434,14 +428,14 @@ hipError_t launch(const T* q, const T* k, const T* v, const PackedGradients<T>& 
         };
         // Each launch's kernel, tiles and LDS for @p each.
         auto queries = [&](auto&& each) -> hipError_t {
-            return divided(args.tokens, args.group, args.kv_tokens, [&](auto division) -> hipError_t {
+            return divided(choose_query_sharing(args, sizeof(T) == 4, units), [&](auto division) -> hipError_t {
                 using S = decltype(division);
                 return each(KernelConstant<query_gradient_kernel<T, D, S>>{},
                             slots(args.tokens, args.group, S::kTile, args.sequences), S::kBlocks);
             });
         };
         auto keys = [&](auto&& each) -> hipError_t {
-            return divided(args.kv_tokens, 1, static_cast<std::int64_t>(args.tokens) * args.group, [&](auto division) -> hipError_t {
+            return divided(choose_key_sharing(args, sizeof(T) == 4, units), [&](auto division) -> hipError_t {
                 using S = decltype(division);
                 return each(KernelConstant<key_gradient_kernel<T, D, S>>{},
                             slots(args.kv_tokens, 1, S::kTile, args.sequences),

@@ -1,5 +1,7 @@
-"""Which keys the parts and the queries of packed attention take, up to the longest
-caches that a call accepts (kernels/packed_places.hpp), and that none longer is."""
+"""How packed attention is divided (kernels/packed_choice.hpp) on the 256 compute units of
+an MI355X: that the GPU tests reach every kernel, and the measured sizes theirs. Which keys
+the parts and the queries take (kernels/packed_places.hpp), up to the longest caches that a
+call accepts; and that none longer is."""
 
 from __future__ import annotations
 
@@ -11,9 +13,35 @@ import pytest
 
 import cuvit_amd as cuvit
 from conftest import ROOT
+from packed_support import Packed
 from test_packed_attention_cpu import ADDRESS, CALLS, backward_call, forward_call
+from test_packed_divisions_gpu import FORWARD, GRADIENTS, HEAD_DIMS
 
 MOST = 2 ** 31 - 1
+UNITS = 256
+KINDS = ["parts", "few", "middle", "large"]
+WIDTHS = [32, 64, 96, 128, 256]  # that kernels are built for
+
+
+def sizes(sequences, tokens, kv_tokens, heads, kv_heads, head_dim):
+    return (ctypes.c_int32 * 6)(sequences, tokens, kv_tokens, heads, kv_heads, head_dim)
+
+
+def width(head_dim):
+    return next(w for w in WIDTHS if head_dim <= w)
+
+
+def sizes_of(case, head_dim):
+    queries, keys, heads, kv_heads = case
+    p = Packed(queries, heads, head_dim, kv_heads=kv_heads, keys=keys)
+    return sizes(len(queries), p.tokens, p.kv_tokens, heads, kv_heads, head_dim)
+
+
+def forward_kind(choice, problem, single):
+    parts = ctypes.c_int32()
+    kind = KINDS[choice.packed_forward_choice(problem, single, UNITS, ctypes.byref(parts))]
+    assert (parts.value >= 4) == (kind == "parts")
+    return kind
 
 
 @pytest.fixture(scope="module")
@@ -79,3 +107,35 @@ def test_gradients_are_refused_before_any_launch(lib):
     p = cuvit.packed_attention_problem(1, 1, 1, 8, kv_tokens=2 ** 30)
     assert backward_call(lib, p, bf16=False, kv_starts=ADDRESS) == cuvit.ERROR_LENGTH
     assert b"2^32 threads" in lib.cuvit_last_error()
+
+
+@pytest.mark.parametrize("single", [0, 1])
+def test_the_gpu_cases_reach_every_forward(choice, single):
+    reached = set()
+    for name, case in FORWARD.items():
+        for head_dim in HEAD_DIMS:
+            kind = forward_kind(choice, sizes_of(case, head_dim), single)
+            assert kind == name.split("_")[0], (name, head_dim)
+            reached.add((kind, width(head_dim)))
+    assert reached == {(kind, w) for kind in KINDS for w in WIDTHS}
+
+
+@pytest.mark.parametrize("single", [0, 1])
+def test_the_gpu_cases_reach_every_gradient(choice, single):
+    rows, keys = set(), set()
+    for name, case in GRADIENTS.items():
+        for head_dim in HEAD_DIMS:
+            problem = sizes_of(case, head_dim)
+            rows.add((choice.packed_query_sharing(problem, single, UNITS), width(head_dim)))
+            keys.add((choice.packed_key_sharing(problem, single, UNITS), width(head_dim)))
+    every = {(n, w) for n in ((2, 4) if single else (1, 2, 4)) for w in WIDTHS if n < 4 or w <= 128}
+    assert rows == every and keys == every
+
+
+@pytest.mark.parametrize("sequences,tokens,kv_tokens,heads,kv_heads,head_dim,single,expected", [
+    (1, 197, 197, 3, 3, 64, 1, "few"), (64, 64 * 577, 64 * 577, 12, 12, 64, 0, "large"),
+    (1, 3136, 3136, 12, 12, 64, 0, "middle"), (4, 4 * 577, 4 * 577, 6, 6, 64, 0, "parts"),
+    (16, 16, 16 * 12545, 12, 4, 128, 0, "parts"), (64, 64, 64 * 8192, 12, 4, 128, 0, "parts"),
+    (256, 256, 256 * 2048, 32, 8, 128, 0, "middle"), (1024, 1024, 1024 * 577, 12, 12, 64, 0, "middle")])
+def test_measured_sizes(choice, sequences, tokens, kv_tokens, heads, kv_heads, head_dim, single, expected):
+    assert forward_kind(choice, sizes(sequences, tokens, kv_tokens, heads, kv_heads, head_dim), single) == expected
