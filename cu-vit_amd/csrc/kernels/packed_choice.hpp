@@ -70,7 +70,7 @@ inline int choose_sharing(const PackedArgs& args, bool single, int tokens, int t
         const int rows = (single ? 16 : 32) * 4 / sharing;
         return slots(tokens, times, rows, args.sequences) * args.kv_heads >= (single ? 1 : 2) * units;
     };
-    if (walk < 512 * args.sequences || enough(least_sharing(single))) {
+    if (walk < std::int64_t{512} * args.sequences || enough(least_sharing(single))) {
         return least_sharing(single);
     }
     return most_sharing(args.head_dim) > 2 && !enough(2) ? most_sharing(args.head_dim) : 2;

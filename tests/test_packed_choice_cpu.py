@@ -139,3 +139,12 @@ def test_the_gpu_cases_reach_every_gradient(choice, single):
     (256, 256, 256 * 2048, 32, 8, 128, 0, "middle"), (1024, 1024, 1024 * 577, 12, 12, 64, 0, "middle")])
 def test_measured_sizes(choice, sequences, tokens, kv_tokens, heads, kv_heads, head_dim, single, expected):
     assert forward_kind(choice, sizes(sequences, tokens, kv_tokens, heads, kv_heads, head_dim), single) == expected
+
+
+@pytest.mark.parametrize("single", [0, 1])
+@pytest.mark.parametrize("sequences", [2 ** 20, 2 ** 22 - 1, 2 ** 22, 5_000_000, 2 ** 23 - 1, 2 ** 24])
+def test_short_walks_are_not_shared_however_many_sequences(choice, single, sequences):
+    """(On more compute units than there are tiles, so that the walk alone decides.)"""
+    problem = sizes(sequences, sequences, sequences, 1, 1, 64)
+    for sharing in (choice.packed_query_sharing, choice.packed_key_sharing):
+        assert sharing(problem, single, 2 ** 28) == (2 if single else 1)
