@@ -20,6 +20,8 @@ constexpr std::int64_t kMaxRows = 0x7FFFFFFF;
 constexpr int kMaxTokens = 0x7FFFFFFF - 4095;
 /// A token's stride, so that a tile of rows stays within a load's 32-bit offsets.
 constexpr std::int64_t kMaxTokenBytes = std::int64_t{1} << 23;
+/// The scale times log2(e), the factor of the exponents, is finite.
+constexpr float kMaxScale = 0x1p127F;
 
 hipStream_t as_hip(cuvit_stream_t stream) { return reinterpret_cast<hipStream_t>(stream); }
 
@@ -69,8 +71,9 @@ int check_problem(const cuvit_packed_attention_problem& p, std::int64_t size, de
         return fail(CUVIT_ERROR_INVALID_ARGUMENT,
                     "Packed attention needs a head_dim that is a multiple of 8 and at most 256");
     }
-    if (p.scale != 0.0F && !(p.scale >= FLT_MIN && p.scale <= FLT_MAX)) {
-        return fail(CUVIT_ERROR_INVALID_ARGUMENT, "Packed attention needs a positive normal scale, or 0 for its own");
+    if (p.scale != 0.0F && !(p.scale >= FLT_MIN && p.scale <= kMaxScale)) {
+        return fail(CUVIT_ERROR_INVALID_ARGUMENT,
+                    "Packed attention needs a positive normal scale of at most 2^127, or 0 for its own");
     }
     if (p.heads > kMaxHeads) {
         return fail(CUVIT_ERROR_LENGTH, "Packed attention takes at most 65535 heads");

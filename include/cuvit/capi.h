@@ -385,7 +385,7 @@ typedef struct cuvit_packed_attention_problem {
     int heads;      /* a multiple of kv_heads */
     int kv_heads;
     int head_dim;   /* a multiple of 8, at most 256 */
-    float scale;    /* of the logits, a positive normal float; 0: 1 / sqrt(head_dim) */
+    float scale;    /* positive, normal, at most 2^127; 0: 1 / sqrt(head_dim) */
     uint8_t causal;
     cuvit_token_strides q;
     cuvit_token_strides k;

@@ -148,3 +148,21 @@ def test_short_walks_are_not_shared_however_many_sequences(choice, single, seque
     problem = sizes(sequences, sequences, sequences, 1, 1, 64)
     for sharing in (choice.packed_query_sharing, choice.packed_key_sharing):
         assert sharing(problem, single, 2 ** 28) == (2 if single else 1)
+
+
+@CALLS
+@pytest.mark.parametrize("bf16", [False, True])
+def test_scales_that_leave_the_exponents_no_room(lib, call, bf16):
+    """The exponent's base 2 takes 1.4427 times the scale, which has to be finite."""
+    for scale in (1.8e38, 2.3e38, 2.4e38, 3.4028234663852886e38):
+        p = cuvit.packed_attention_problem(2, 10, 4, 64, kv_heads=2, scale=scale)
+        assert call(lib, p, bf16=bf16) == cuvit.ERROR_INVALID_ARGUMENT
+        assert b"scale" in lib.cuvit_last_error()
+        assert cuvit.packed_attention_workspace(p) == 0 and cuvit.packed_attention_backward_workspace(p) == 0
+
+
+def test_the_largest_and_smallest_scales_are_taken(lib):
+    for scale in (2.0 ** 127, 2.0 ** -126):
+        p = cuvit.packed_attention_problem(2, 10, 4, 64, kv_heads=2, scale=scale)
+        assert forward_call(lib, p, q=ADDRESS + 8) == cuvit.ERROR_INVALID_ARGUMENT
+        assert b"aligned" in lib.cuvit_last_error()

@@ -8,8 +8,8 @@ import pytest
 import torch
 
 from packed_support import Packed, forward
-from blocks_support import worst
-from test_packed_attention_gpu import TYPES, Call, operands
+from blocks_support import seeded, worst
+from test_packed_attention_gpu import TYPES, Call, check_forward, operands
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,19 @@ def test_the_longest_cache(cuvit, device, queries):
         seen = keys - queries + torch.arange(1, queries).double()
         assert bool((out[:-1] == 0.0).all())
         assert float((lse[:-1] - torch.log(seen)).abs().max()) <= 8 * 2.0 ** -24 * 30.0
+
+
+@TYPES
+@pytest.mark.parametrize("scale", [2.0 ** 127, 2.0 ** -126])
+def test_scales_at_their_limits(cuvit, device, dtype, scale):
+    """At the largest, products of 2^-126 times 0 to 4, exact ones, give logits of 0 to 8;
+    at the smallest the logits vanish and every key weighs the same."""
+    p = Packed([40, 70], 2, 64, scale=scale, causal=True)
+    q, k, v = operands(p, dtype, 33)
+    if scale > 1.0:
+        multiples = torch.randint(0, 5, k.shape[:2], generator=seeded(34)).to(dtype)
+        q.zero_()[..., 0] = 2.0 ** -100
+        k.zero_()[..., 0] = multiples * 2.0 ** -26
+    call = Call(cuvit, device, p, q, k, v)
+    call.forward()
+    check_forward(call, q, k, v)
