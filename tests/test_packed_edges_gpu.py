@@ -101,3 +101,60 @@ def test_scales_at_their_limits(cuvit, device, dtype, scale):
     call = Call(cuvit, device, p, q, k, v)
     call.forward()
     check_forward(call, q, k, v)
+
+
+class Guarded:
+    """A tensor of `shape` between two stretches of memory that nobody may write."""
+
+    def __init__(self, shape, dtype, device, value, margin=1 << 18):
+        size = math.prod(shape) * torch.empty(0, dtype=dtype).element_size()
+        self.memory = torch.full((2 * margin + size,), 0x5A, dtype=torch.uint8, device=device)
+        self.tensor = self.memory[margin:margin + size].view(dtype).view(shape)
+        self.tensor.fill_(value)
+        self.margin = margin
+
+    def untouched(self):
+        sides = torch.cat([self.memory[:self.margin], self.memory[-self.margin:]])
+        return bool((sides == 0x5A).all())
+
+
+GUARDED = [  # queries, keys, heads, kv_heads, head_dim: each division of the forward and the gradients
+    ([20, 20, 10, 14], None, 2, 2, 64),
+    ([70, 9, 101], None, 4, 2, 128),
+    ([2, 1, 3], [3000, 40, 700], 4, 2, 80),
+    ([300, 150, 70, 1, 33], None, 24, 12, 64),
+    ([290] + [20, 45, 64, 33, 70] * 7 + [0, 1], None, 24, 12, 32),
+    ([600, 530], None, 4, 2, 96),
+    ([64], [512], 256, 256, 32),
+    ([512], [64], 256, 256, 32),
+]
+
+
+@TYPES
+@pytest.mark.parametrize("fits", [True, False], ids=["starts", "starts_that_do_not_fit"])
+@pytest.mark.parametrize("queries,keys,heads,kv_heads,head_dim", GUARDED, ids=[str(g[0])[:20] for g in GUARDED])
+def test_nothing_beside_the_results_is_written(cuvit, device, dtype, fits, queries, keys, heads, kv_heads, head_dim):
+    """out, lse, the three gradients and both workspaces, with sequences that the operands
+    hold, and with starts and lengths that lead far outside them."""
+    p = Packed(queries, heads, head_dim, kv_heads=kv_heads, keys=keys, causal=True, spare=0)
+    q, k, v = operands(p, dtype, 35)
+    call = Call(cuvit, device, p, q, k, v)
+    out = Guarded(call.out.shape, dtype, device, 0.0)
+    lse = Guarded(call.lse.shape, torch.float32, device, 0.0)
+    grads = [Guarded(x.shape, dtype, device, 0.0) for x in call.operands]
+    sizes = [cuvit.packed_attention_workspace(call.problem), cuvit.packed_attention_backward_workspace(call.problem)]
+    workspaces = [Guarded((size,), torch.uint8, device, 255) if size else None for size in sizes]
+    call.out, call.lse, call.grads = out.tensor, lse.tensor, [g.tensor for g in grads]
+    call.workspace, call.backward_workspace = (w.tensor if w is not None else None for w in workspaces)
+    if not fits:
+        count = len(queries)
+        call.starts.copy_(torch.tensor(([-9, 2 ** 31 - 1, p.tokens - 3, p.tokens + 100, -2 ** 31] * count)[:count + 1]))
+        call.caches["kv_starts"] = torch.tensor(([5, p.kv_tokens + 64, -7, 2 ** 31 - 1] * count)[:count + 1],
+                                                dtype=torch.int32, device=device)
+        call.caches["kv_lengths"] = torch.tensor(([2 ** 31 - 1, 40, -5] * count)[:count], dtype=torch.int32, device=device)
+    call.forward()
+    call.backward(torch.ones_like(call.out))
+    torch.cuda.synchronize()
+    for name, guarded in (("out", out), ("lse", lse), ("grad_q", grads[0]), ("grad_k", grads[1]), ("grad_v", grads[2]),
+                          ("workspace", workspaces[0]), ("backward workspace", workspaces[1])):
+        assert guarded is None or guarded.untouched(), name
