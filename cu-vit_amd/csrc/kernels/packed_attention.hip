@@ -146,7 +146,7 @@ template <typename T, int D, Kind Way> struct Division {
     static constexpr bool kInParts = Way == Kind::kParts;
     static constexpr int kWaves = kInParts ? 1 : packed::kWaves;
     static constexpr int kThreads = kWaves * kWave;
-    static constexpr int kPairs = kInParts || (Way == Kind::kLarge && sizeof(T) == 2) ? 1 : 2;
+    static constexpr int kPairs = kInParts || Way == Kind::kLarge ? 1 : 2;
     static constexpr int kShared =
         Way == Kind::kFew && R::kPitch <= 256 * static_cast<int>(sizeof(T)) / 2 ? 4 : kPairs;
     static constexpr int kRows = R::kE * kWaves / kShared; // of a workgroup
@@ -157,12 +157,13 @@ template <typename T, int D, Kind Way> struct Division {
     static constexpr int kTiles = kKeys / R::kE / kShared; // of keys, a wavefront's
     /// Wavefronts that share a SIMD. From two on the compiler keeps every accumulator in
     /// the registers that the VALU reads, instead of moving logits and weights over.
-    static constexpr int kShare = D > 128 ? 1 : D > 64 ? 2 : sizeof(T) == 2 && Way == Kind::kLarge ? 4 : 3;
+    static constexpr int kShare = D > 128 ? 1 : D > 64 ? 2 : Way == Kind::kLarge ? 4 : 3;
     using Loads = Stage<T, D, kKeys, kWaves>;
     // The sums of the wavefronts that add up: accumulators, shift and sum of each lane.
     static constexpr int kSums = R::kTiles * kRegisters<T> + 2;
     static constexpr int kExchange = kWaves / kShared * (kShared - 1) * kSums * kWave * 4;
     static constexpr int kLds = 4 * Loads::kBytes > kExchange ? 4 * Loads::kBytes : kExchange;
+    static_assert(Way != Kind::kLarge || sizeof(T) == 2, "in fp32 it would be kMiddle");
     static_assert(kLds <= 128 * 1024, "two blocks of keys and values, or the sums");
     static_assert(Way == Kind::kFew || kRows == tile_rows(Way, sizeof(T) == 4), "as the rules count them");
     static_assert(!kInParts || kKeys == kPartKeys, "as the rules count them");
@@ -639,7 +640,11 @@ hipError_t launch(const T* q, const T* k, const T* v, T* out, float* lse, float*
             return hipGetLastError();
         };
         switch (chosen.kind) {
-        case Kind::kLarge: return run(Division<T, D, Kind::kLarge>{});
+        case Kind::kLarge:
+            if constexpr (sizeof(T) == 2) {
+                return run(Division<T, D, Kind::kLarge>{});
+            }
+            [[fallthrough]];
         case Kind::kMiddle: return run(Division<T, D, Kind::kMiddle>{});
         case Kind::kFew: return run(Division<T, D, Kind::kFew>{});
         default: break;

@@ -6,8 +6,8 @@
 namespace cuvit::detail::packed {
 
 /// How a workgroup's four wavefronts divide their work in the forward: kFew, kMiddle and
-/// kLarge have all four, pairs or (in bf16) none of them on the same rows; in kParts they
-/// are single ones, each with a part of the keys, joined by a second launch
+/// kLarge (bf16 alone) have all four, pairs or none of them on the same rows; in kParts
+/// they are single ones, each with a part of the keys, joined by a second launch
 /// (packed_attention.hip).
 enum class Kind { kParts, kFew, kMiddle, kLarge };
 
@@ -19,7 +19,7 @@ struct Plan {
 /// Rows of a workgroup's tile, of fp32 (@p single) or bf16. (kFew's are those of kParts,
 /// twice as many for heads above 128, and count in no rule.)
 constexpr int tile_rows(Kind kind, bool single) {
-    return kind == Kind::kLarge ? (single ? 32 : 128) : kind == Kind::kMiddle ? (single ? 32 : 64) : single ? 16 : 32;
+    return kind == Kind::kLarge ? 128 : kind == Kind::kMiddle ? (single ? 32 : 64) : single ? 16 : 32;
 }
 
 /// Keys of a block of a part.
@@ -40,7 +40,7 @@ inline Plan choose_forward(const PackedArgs& args, bool single, std::int64_t uni
     // Where a sequence's rows fit the smallest tile on average, larger ones are no fewer.
     const bool small = static_cast<std::int64_t>(args.tokens) * args.group <=
                        static_cast<std::int64_t>(args.sequences) * tile_rows(Kind::kParts, single);
-    if (!small && tiles(Kind::kLarge) >= 2 * units) {
+    if (!single && !small && tiles(Kind::kLarge) >= 2 * units) {
         return {Kind::kLarge, 1};
     }
     if (tiles(Kind::kMiddle) >= (small && most >= 16 ? 2 : 1) * units) {

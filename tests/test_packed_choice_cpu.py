@@ -115,9 +115,10 @@ def test_the_gpu_cases_reach_every_forward(choice, single):
     for name, case in FORWARD.items():
         for head_dim in HEAD_DIMS:
             kind = forward_kind(choice, sizes_of(case, head_dim), single)
-            assert kind == name.split("_")[0], (name, head_dim)
+            # (fp32 has no larger tiles than the pairs'.)
+            assert kind == ("middle" if single and name == "large" else name.split("_")[0]), (name, head_dim)
             reached.add((kind, width(head_dim)))
-    assert reached == {(kind, w) for kind in KINDS for w in WIDTHS}
+    assert reached == {(kind, w) for kind in KINDS for w in WIDTHS if not single or kind != "large"}
 
 
 @pytest.mark.parametrize("single", [0, 1])
