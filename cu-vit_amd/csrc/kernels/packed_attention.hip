@@ -98,7 +98,6 @@ __device__ __forceinline__ void attend_alone(const T* q, const T* k, const T* v,
         for (int i = 0; i < 4; ++i) {
             value[i] *= kept / sum;
         }
-#pragma unroll 8
         for (int key = 0; key < there; ++key) {
             const float s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), key));
             const T* const row = v + (first + key) * v_token;
