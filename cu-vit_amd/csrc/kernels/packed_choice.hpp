@@ -25,12 +25,20 @@ constexpr int tile_rows(Kind kind, bool single) {
 /// Keys of a block of a part.
 constexpr int kPartKeys = 32;
 
-/// By the call's sizes alone: into the largest tiles of rows that still
-/// give every CU work, and for few rows over long keys into as many parts of them as give
-/// the chip eight single wavefronts a CU, of four blocks or more on average. us for
+/// By the call's sizes alone, which know a cache's room but not what is filled of it: into
+/// the largest tiles of rows that still give every CU work, and for few rows over long keys
+/// into as many parts of them as give the chip eight single wavefronts a CU, of four blocks
+/// or more on average. us for
 /// kMiddle / kLarge / parts of single queries: 64 over 8192 keys, 12 heads on 4 of 128 240
 /// / 280 / 200 (4 parts), 256 over 2048, 32 on 8 389 / 405 / 450, 1024 over 577, 12 of 64
 /// 303 / 311 / 470.
+///
+/// kFew walks a key in about 7.5 ns (heads of 64; fp32 19) and a join takes 2 us and 0.7 ns
+/// for each of a row's parts (more in fp32, whose parts wait for MFMAs too): so parts where
+/// there are at most 10 of these (20) for each key above 800. us for kFew / parts, bf16: 4 x
+/// 577 tokens, 6 heads of 64 10.8 / 49, 1 query over 577 keys 8.8 / 10.7, 64 over 2048
+/// 16.9 / 14.9, 256 over 2048 16.9 / 20.8, 577 over 12545 103 / 49; fp32 4 x 64 over 2048 47
+/// / 34, 1 x 577 over 2048 36 / 51.
 inline Plan choose_forward(const PackedArgs& args, bool single, std::int64_t units) {
     const auto tiles = [&](Kind kind) {
         return slots(args.tokens, args.group, tile_rows(kind, single), args.sequences) * args.kv_heads;
@@ -48,7 +56,8 @@ inline Plan choose_forward(const PackedArgs& args, bool single, std::int64_t uni
     }
     const std::int64_t wanted = 8 * units / tiles(Kind::kParts);
     const std::int64_t parts = wanted < most ? wanted : most;
-    return parts >= 4 ? Plan{Kind::kParts, static_cast<int>(parts)} : Plan{Kind::kFew, 1};
+    const bool longer = static_cast<std::int64_t>(args.tokens) * args.heads * parts <= (single ? 20 : 10) * (lengths - 800);
+    return parts >= 4 && longer ? Plan{Kind::kParts, static_cast<int>(parts)} : Plan{Kind::kFew, 1};
 }
 
 /// Wavefronts that share a tile of rows, or of keys, in the gradients: at most (what the

@@ -135,7 +135,7 @@ def test_the_gpu_cases_reach_every_gradient(choice, single):
 
 @pytest.mark.parametrize("sequences,tokens,kv_tokens,heads,kv_heads,head_dim,single,expected", [
     (1, 197, 197, 3, 3, 64, 1, "few"), (64, 64 * 577, 64 * 577, 12, 12, 64, 0, "large"),
-    (1, 3136, 3136, 12, 12, 64, 0, "middle"), (4, 4 * 577, 4 * 577, 6, 6, 64, 0, "parts"),
+    (1, 3136, 3136, 12, 12, 64, 0, "middle"), (4, 4 * 577, 4 * 577, 6, 6, 64, 0, "few"),
     (16, 16, 16 * 12545, 12, 4, 128, 0, "parts"), (64, 64, 64 * 8192, 12, 4, 128, 0, "parts"),
     (256, 256, 256 * 2048, 32, 8, 128, 0, "middle"), (1024, 1024, 1024 * 577, 12, 12, 64, 0, "middle")])
 def test_measured_sizes(choice, sequences, tokens, kv_tokens, heads, kv_heads, head_dim, single, expected):
@@ -149,6 +149,20 @@ def test_short_walks_are_not_shared_however_many_sequences(choice, single, seque
     problem = sizes(sequences, sequences, sequences, 1, 1, 64)
     for sharing in (choice.packed_query_sharing, choice.packed_key_sharing):
         assert sharing(problem, single, 2 ** 28) == (2 if single else 1)
+
+
+@pytest.mark.parametrize("sequences,queries,keys,heads,kv_heads,head_dim,single,expected", [
+    # Prompts, and few queries over short caches: the join would take longer than the walk.
+    (4, 577, 577, 6, 6, 64, 0, "few"), (1, 577, 577, 6, 6, 64, 0, "few"), (1, 785, 785, 12, 4, 128, 0, "few"),
+    (1, 577, 577, 6, 6, 64, 1, "few"), (4, 256, 2048, 6, 6, 64, 0, "few"), (1, 577, 2048, 6, 6, 64, 1, "few"),
+    (1, 256, 2048, 12, 4, 128, 1, "few"), (1, 1, 577, 6, 6, 64, 0, "few"), (4, 16, 577, 12, 4, 128, 1, "few"),
+    # Few rows over long ones.
+    (1, 1, 2048, 6, 6, 64, 0, "parts"), (1, 64, 2048, 6, 6, 64, 0, "parts"), (4, 16, 2048, 12, 4, 128, 1, "parts"),
+    (4, 64, 2048, 6, 6, 64, 1, "parts"), (1, 577, 12545, 6, 6, 64, 0, "parts"), (4, 1, 12545, 12, 4, 128, 1, "parts")])
+def test_parts_where_the_join_is_the_shorter(choice, sequences, queries, keys, heads, kv_heads, head_dim, single,
+                                             expected):
+    problem = sizes(sequences, sequences * queries, sequences * keys, heads, kv_heads, head_dim)
+    assert forward_kind(choice, problem, single) == expected
 
 
 @CALLS
