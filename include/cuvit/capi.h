@@ -408,7 +408,9 @@ void cuvit_packed_attention_problem_projection(cuvit_packed_attention_problem* p
  * aligned; out and lse overlap no other operand. The workspace, of
  * cuvit_packed_attention_workspace() bytes (null where that is 0) and 16-byte
  * aligned, is used by one call at a time: calls that may overlap, replays of
- * captured ones among them, take one each. More than 65535 heads, or 2^31 - 4096
+ * captured ones among them, take one each. It and the division of the work follow
+ * from the problem's sizes alone, kv_tokens / sequences standing for the length of
+ * the keys: a cache with much room is divided as a full one. More than 65535 heads, or 2^31 - 4096
  * tokens or 2^31 - 1 tokens times heads of either side, or 2^32 threads (2^24
  * tiles of 32 rows in fp32, 128 in bf16, a sequence starting a new one) are
  * CUVIT_ERROR_LENGTH. */
