@@ -158,3 +158,36 @@ def test_nothing_beside_the_results_is_written(cuvit, device, dtype, fits, queri
     for name, guarded in (("out", out), ("lse", lse), ("grad_q", grads[0]), ("grad_k", grads[1]), ("grad_v", grads[2]),
                           ("workspace", workspaces[0]), ("backward workspace", workspaces[1])):
         assert guarded is None or guarded.untouched(), name
+
+
+@TYPES
+def test_a_captured_call_while_caches_fill(cuvit, device, dtype):
+    """Single queries over caches with room, in parts: one graph replayed as the caches grow
+    from nothing to full, with eager calls between the replays."""
+    room, sequences, heads, kv_heads, head_dim = 3000, 3, 4, 2, 64
+    full = Packed([1] * sequences, heads, head_dim, kv_heads=kv_heads, keys=[room - 1] * sequences,
+                  rooms=[room] * sequences, causal=True, spare=0)
+    q, k, v = operands(full, dtype, 41)
+    call = Call(cuvit, device, full, q, k, v)
+    assert cuvit.packed_attention_workspace(call.problem) > 0
+    call.forward()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call.forward()
+    for lengths in ([0, 0, 0], [1, 0, 2], [64, 65, 1], [127, 2999, 0], [500, 1280, 2048], [room, room, room]):
+        p = Packed([1] * sequences, heads, head_dim, kv_heads=kv_heads, keys=lengths, rooms=[room] * sequences,
+                   causal=True, spare=0)
+        fresh = operands(p, dtype, 42 + sum(lengths))[0]
+        eager = Call(cuvit, device, p, fresh, k, v)
+        eager.caches["kv_lengths"] = torch.tensor(lengths, dtype=torch.int32, device=device)
+        eager.forward()
+        call.operands[0].copy_(fresh)
+        call.caches["kv_lengths"].copy_(eager.caches["kv_lengths"])
+        call.out.fill_(7.0)
+        call.lse.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(call.out, eager.out) and torch.equal(call.lse, eager.lse)
+        call.p = p
+        check_forward(call, fresh, k, v)
