@@ -361,8 +361,9 @@ int cuvit_gated_checkpoint_backward_bf16(const uint8_t* codes, const uint8_t* sc
  * device memory, [sequences + 1], [sequences + 1] and [sequences]; a null
  * kv_starts is starts (kv_tokens is then tokens), a null kv_lengths all keys.
  * Starts do not decrease; numbers that leave the operands are cut to them. A
- * length may be 0. Rows outside every sequence are not read, and their results
- * and gradients stay as they were.
+ * length may be 0. Rows outside every sequence, the room behind a cache's filled
+ * keys among them, are not read, and their results and gradients stay as they
+ * were.
  *
  * Query head h sees key head h / (heads / kv_heads). Causal: the last query sees
  * the last key, the one before it all keys but that, and so on. A query that sees
