@@ -39,7 +39,8 @@ int check_strides(const detail::TokenStrides& s, int head_dim, std::int64_t size
     if (s.token < 0 || s.head < 0) {
         return fail(CUVIT_ERROR_INVALID_ARGUMENT, "Packed attention strides cannot be negative");
     }
-    if (s.token * size % 16 != 0 || s.head * size % 16 != 0 || s.token < head_dim) {
+    const std::int64_t piece = 16 / size;
+    if (s.token % piece != 0 || s.head % piece != 0 || s.token < head_dim) {
         return fail(CUVIT_ERROR_INVALID_ARGUMENT,
                     "Packed attention strides are whole 16-byte pieces, a token's at least head_dim");
     }

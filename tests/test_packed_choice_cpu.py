@@ -181,3 +181,16 @@ def test_the_largest_and_smallest_scales_are_taken(lib):
         p = cuvit.packed_attention_problem(2, 10, 4, 64, kv_heads=2, scale=scale)
         assert forward_call(lib, p, q=ADDRESS + 8) == cuvit.ERROR_INVALID_ARGUMENT
         assert b"aligned" in lib.cuvit_last_error()
+
+
+@CALLS
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("name", ["q", "k", "v", "out"])
+def test_strides_near_2_to_63(lib, call, bf16, name):
+    """Whole pieces or not, without a product that overflows."""
+    for stride, expected in ((2 ** 62, cuvit.ERROR_LENGTH), (2 ** 63 - 8, cuvit.ERROR_LENGTH),
+                             (2 ** 63 - 1, cuvit.ERROR_INVALID_ARGUMENT), (2 ** 61 + 1, cuvit.ERROR_INVALID_ARGUMENT)):
+        for field in ("token", "head"):
+            p = cuvit.packed_attention_problem(2, 10, 4, 64, kv_heads=2)
+            setattr(getattr(p, name), field, stride)
+            assert call(lib, p, bf16=bf16) == expected
